@@ -335,6 +335,123 @@ vw_status vw_head_sample(vw_handle* handle, const void* hidden, int64_t hidden_s
                          const vw_options* options, int32_t n_options, float* out_logits, void* stream);
 
 /*
+ * A decoder layer's attention over a paged key/value cache, between the projections the caller runs: what
+ * DecoderStack.ForwardSegments (src/Voxwerk/Talker/DecoderStack.cs:144-228) does with its head-major KvCache (:21), for
+ * a batch of sequences whose keys and values lie in pages of one cache.  Per layer:
+ *   vw_rope_append        per-head norm and rotary positions of q and k; k and v into the cache, q out
+ *   vw_prompt_attention   rows of several tokens per sequence (whole prompts, or the next piece of one), causal
+ *   vw_decode_attention   one row per sequence; groups of sequences may share a prefix (a voice prompt)
+ * All pointers in these structs are device memory of the handle's device; tensors of 16-bit elements are bf16 bits.
+ * stream as in vw_sample: NULL runs on the handle's stream and returns device-side errors, a stream enqueues.  Device-
+ * side errors: a page outside the cache or a position outside the table gives VW_ERR_OUT_OF_RANGE; key counts, row
+ * offsets or group offsets that do not fit give VW_ERR_INVALID_ARG (the reference throws when a cache is full,
+ * DecoderStack.cs:154).  Nothing outside the cache and the outputs is read or written in either case.
+ * Calls of one handle on different streams are ordered by the library (they share the handle's workspace); work that a
+ * caller captures into CUDA graphs it orders itself.
+ */
+
+/* The cache: keys and values [n_pages, page_size, n_kv_heads, head_dim] bf16, by the strides given (elements, the same
+ * for k and v, multiples of 8; the last dimension contiguous, both pointers 16-byte aligned).  page_size: a power of
+ * two from 16 to 256. */
+typedef struct vw_kv_cache {
+    void* k;
+    void* v;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+} vw_kv_cache;
+
+/* A batch of sequences: sequence s holds kv_lens[s] keys (those of the call's own rows included), key j in page
+ * page_table[s * page_table_stride + j / page_size].  Its rows of the call are q_offsets[s] .. q_offsets[s + 1) and
+ * are its last keys; q_offsets NULL: row s, one per sequence.  Rows past the last offset are left alone. */
+typedef struct vw_kv_batch {
+    const int32_t* page_table;   /* [n_seqs, page_table_stride], max_pages of them valid */
+    int64_t page_table_stride;
+    int32_t max_pages;
+    int32_t n_seqs;
+    const int32_t* kv_lens;      /* [n_seqs] */
+    const int32_t* q_offsets;    /* [n_seqs + 1] or NULL */
+    int32_t n_rows;
+} vw_kv_batch;
+
+/* Shared prefixes: the sequences group_offsets[g] .. group_offsets[g + 1) of a batch also see the lens[g] keys of page
+ * table g, ahead of their own (each sequence's kv_lens then counts its own keys only).  Sequences outside every group
+ * have no prefix. */
+typedef struct vw_kv_prefix {
+    const int32_t* page_table;   /* [n_groups, page_table_stride], max_pages of them valid */
+    int64_t page_table_stride;
+    int32_t max_pages;
+    int32_t n_groups;
+    const int32_t* lens;           /* [n_groups] */
+    const int32_t* group_offsets;  /* [n_groups + 1], ascending */
+} vw_kv_prefix;
+
+/* The rows of a vw_rope_append: element (r, head, i) of q is q[r * q_row_stride + head * q_head_stride + i]; k and v
+ * likewise (the three may be parts of one fused projection). */
+typedef struct vw_rope_rows {
+    const void* q;               /* [n_rows, n_q_heads, head_dim] of dtype (vw_dtype) */
+    const void* k;               /* [n_rows, n_kv_heads, head_dim] */
+    const void* v;
+    int64_t q_row_stride, q_head_stride;
+    int64_t k_row_stride, k_head_stride;
+    int64_t v_row_stride, v_head_stride;
+    int32_t dtype;
+    int32_t n_q_heads;
+    const float* q_norm;         /* [head_dim] RMS-norm weight of every query head, or NULL: no norm */
+    const float* k_norm;
+    float eps;
+    int32_t n_positions;         /* rows of the tables below */
+    const float* cos_table;      /* [n_positions, rotary_dim / 2] */
+    const float* sin_table;
+    const int32_t* positions;    /* [n_rows] rows of the tables, or NULL: a row's position is its key's index */
+    int32_t rotary_dim;          /* even, 0 .. head_dim; the dims past it are not turned */
+    int32_t interleaved;         /* 0: pairs (i, i + rotary_dim / 2); 1: pairs (2 i, 2 i + 1) */
+    void* q_out;                 /* [n_rows, n_q_heads, head_dim] bf16 */
+    int64_t q_out_row_stride, q_out_head_stride;
+} vw_rope_rows;
+
+/*
+ * For every row: q and k normalised (x rsqrt(mean(x^2) + eps) weight over each head), turned to the row's position,
+ * rounded to bf16 once; q goes to q_out, k and v to the row's place in the cache.  head_dim even, at most 256.  Scaled
+ * positions for long contexts are a matter of the table's values.
+ */
+vw_status vw_rope_append(vw_handle* handle, const vw_kv_cache* cache, const vw_kv_batch* batch,
+                         const vw_rope_rows* rows, void* stream);
+
+/* The rows of an attention call: q and out [n_rows, n_q_heads, head_dim] bf16 by their strides (elements, multiples
+ * of 8, pointers 16-byte aligned); n_q_heads a multiple of the cache's n_kv_heads, consecutive query heads sharing a
+ * key head, at most 64 of them; head_dim a multiple of 8, at most 128. */
+typedef struct vw_attn_rows {
+    const void* q;
+    int64_t q_row_stride, q_head_stride;
+    int32_t n_q_heads;
+    float scale;                 /* of the scores: softmax(scale * q k^T) */
+    void* out;
+    int64_t out_row_stride, out_head_stride;
+    float* lse;                  /* optional [n_rows, n_q_heads]: log sum exp of each row's scaled scores */
+} vw_attn_rows;
+
+/*
+ * Causal attention of packed sequences: row i of the n rows of a sequence with m keys sees its keys j <= m - n + i.  A
+ * row that sees no key gets out = 0 and lse = -inf.  Rounding: scores and sums in fp32, the probabilities rounded to
+ * bf16 for their product with the values, out rounded once.  A value that is not finite reaches the rows of its own
+ * sequence only, but there also rows before it.
+ */
+vw_status vw_prompt_attention(vw_handle* handle, const vw_kv_cache* cache, const vw_kv_batch* batch,
+                              const vw_attn_rows* rows, void* stream);
+
+/*
+ * One row per sequence (batch->q_offsets is ignored, n_rows >= n_seqs): row s sees all of sequence s's keys and, with a
+ * prefix (nullable), those of its group's prefix, whose keys are read once for the whole group.  Other rules as above.
+ */
+vw_status vw_decode_attention(vw_handle* handle, const vw_kv_cache* cache, const vw_kv_batch* batch,
+                              const vw_kv_prefix* prefix, const vw_attn_rows* rows, void* stream);
+
+/*
  * Single-row mirrors of the reference's Sampler methods, for callers that keep the reference's call shape.
  * Pointers follow `mem`; the calls are synchronous.
  */

@@ -23,6 +23,8 @@ _NATIVE = {
                                "TalkerBatchSampler", "frame_embedding", "head_logits", "head_sample", "sample_rows", "sample_rows_static",
                                "vw_options")},
     **{n: ".batch_state" for n in ("DeviceBatchState",)},
+    **{n: ".attention" for n in ("KvBatch", "KvCache", "KvPrefix", "RopeTable", "decode_attention", "prompt_attention",
+                                 "rope_append")},
 }
 
 

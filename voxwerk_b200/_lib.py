@@ -57,6 +57,9 @@ EXPORTED = (
     "vw_batch_code_embedding",
     "vw_batch_frame_embedding",
     "vw_batch_get_codes",
+    "vw_rope_append",
+    "vw_prompt_attention",
+    "vw_decode_attention",
 )
 
 
@@ -118,6 +121,95 @@ class VwEmbedOut(ctypes.Structure):
         ("hidden", ctypes.c_int32),
         ("out", ctypes.c_void_p),
         ("out_stride", ctypes.c_int64),
+    ]
+
+
+class VwKvCache(ctypes.Structure):
+    """vw_kv_cache: pages of keys and values."""
+
+    _fields_ = [
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+        ("head_stride", ctypes.c_int64),
+        ("n_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+    ]
+
+
+class VwKvBatch(ctypes.Structure):
+    """vw_kv_batch: the sequences of a call and their pages."""
+
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int32),
+        ("n_seqs", ctypes.c_int32),
+        ("kv_lens", ctypes.c_void_p),
+        ("q_offsets", ctypes.c_void_p),
+        ("n_rows", ctypes.c_int32),
+    ]
+
+
+class VwKvPrefix(ctypes.Structure):
+    """vw_kv_prefix: prefixes that groups of sequences share."""
+
+    _fields_ = [
+        ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int32),
+        ("n_groups", ctypes.c_int32),
+        ("lens", ctypes.c_void_p),
+        ("group_offsets", ctypes.c_void_p),
+    ]
+
+
+class VwRopeRows(ctypes.Structure):
+    """vw_rope_rows: the queries, keys and values of a vw_rope_append."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("k_row_stride", ctypes.c_int64),
+        ("k_head_stride", ctypes.c_int64),
+        ("v_row_stride", ctypes.c_int64),
+        ("v_head_stride", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("n_q_heads", ctypes.c_int32),
+        ("q_norm", ctypes.c_void_p),
+        ("k_norm", ctypes.c_void_p),
+        ("eps", ctypes.c_float),
+        ("n_positions", ctypes.c_int32),
+        ("cos_table", ctypes.c_void_p),
+        ("sin_table", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("rotary_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("q_out", ctypes.c_void_p),
+        ("q_out_row_stride", ctypes.c_int64),
+        ("q_out_head_stride", ctypes.c_int64),
+    ]
+
+
+class VwAttnRows(ctypes.Structure):
+    """vw_attn_rows: the queries and outputs of an attention call."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_row_stride", ctypes.c_int64),
+        ("q_head_stride", ctypes.c_int64),
+        ("n_q_heads", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("out", ctypes.c_void_p),
+        ("out_row_stride", ctypes.c_int64),
+        ("out_head_stride", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
     ]
 
 
@@ -209,7 +301,13 @@ def _load() -> ctypes.CDLL:
                        ("vw_batch_frame_embedding", [vp, i32, vp, vp, i32, vp, vp, vp]),
                        ("vw_batch_get_codes", [vp, vp]),
                        ("vw_head_sample", [vp, vp, i64, i32, vp, i64, ctypes.POINTER(VwSegment),
-                                           ctypes.POINTER(VwOptions), i32, vp, vp])):
+                                           ctypes.POINTER(VwOptions), i32, vp, vp]),
+                       ("vw_rope_append", [vp, ctypes.POINTER(VwKvCache), ctypes.POINTER(VwKvBatch),
+                                           ctypes.POINTER(VwRopeRows), vp]),
+                       ("vw_prompt_attention", [vp, ctypes.POINTER(VwKvCache), ctypes.POINTER(VwKvBatch),
+                                                ctypes.POINTER(VwAttnRows), vp]),
+                       ("vw_decode_attention", [vp, ctypes.POINTER(VwKvCache), ctypes.POINTER(VwKvBatch),
+                                                ctypes.POINTER(VwKvPrefix), ctypes.POINTER(VwAttnRows), vp])):
         getattr(lib, name).restype = ctypes.c_int
         getattr(lib, name).argtypes = args
     return lib

@@ -1,0 +1,96 @@
+// vw_handle.h -- the handle behind the C ABI and the helpers its entry points share (vw_api.cpp, vw_attention.cpp).
+// Not part of the public ABI.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <string>
+#include <vector>
+
+#include <cuda_runtime.h>
+
+#include "../../include/vwsampler.h"
+#include "vw_internal.h"
+
+#define VW_EXPORT extern "C" __attribute__((visibility("default")))
+
+constexpr int kCopyStreams = 3;   // host -> device copies of VW_MEM_HOST calls run on this many copy engines
+
+struct vw_handle {
+    int device = -1;
+    cudaStream_t stream = nullptr;
+    cudaStream_t copy_streams[kCopyStreams] = {};
+    cudaEvent_t copy_events[kCopyStreams + 1] = {};   // one per copy stream, and the fork point
+    int sm_count = 0;
+    unsigned* d_err = nullptr;      // device error word (kErr* bits)
+    unsigned* h_err = nullptr;      // pinned mirror
+    char* d_scratch = nullptr;      // general-path scratch, one slice per CTA
+    size_t scratch_bytes = 0;
+    char* d_stage = nullptr;        // VW_MEM_HOST: device copies of the caller's arrays
+    char* d_logits = nullptr;       // vw_head_sample: the GEMM's logits when the caller keeps none
+    size_t logits_bytes = 0;
+    int32_t* d_defer = nullptr;     // four counters + the rows the warp-per-row kernel defers
+    size_t defer_cap = 0;
+    size_t stage_bytes = 0;
+    vw::DevOptions* d_opts = nullptr;
+    vw::DevOptions* h_opts = nullptr;   // pinned upload buffer for option tables > kInlineOptions
+    size_t opts_cap = 0;
+    cudaEvent_t opts_done = nullptr;
+    unsigned long long* d_stats = nullptr;   // vw::kNumStats per-path row counters
+    unsigned long long* d_guess = nullptr;   // candidate thresholds carried from call to call
+    int force_exact = 0;                     // VW_FORCE_EXACT at creation
+    int test_stall_row = -1;                 // VW_TEST_STALL_ROW at creation (first vw_sample call only)
+    unsigned long long h2d_bytes = 0;        // host -> device input bytes of VW_MEM_HOST calls (vw_stats.h2d_bytes)
+    std::vector<vw_batch*> batches;          // live batches created on this handle (released by vw_destroy)
+    std::string last_error;
+};
+
+// Restores the caller's current device on scope exit.
+class DeviceGuard {
+  public:
+    explicit DeviceGuard(int dev) {
+        if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+        ok_ = cudaSetDevice(dev) == cudaSuccess;
+    }
+    ~DeviceGuard() {
+        if (prev_ >= 0) cudaSetDevice(prev_);
+    }
+    bool ok() const { return ok_; }
+
+  private:
+    int prev_ = -1;
+    bool ok_ = false;
+};
+
+inline vw_status fail(vw_handle* h, vw_status s, const std::string& msg) {
+    if (h) h->last_error = msg;
+    return s;
+}
+
+inline vw_status cuda_fail(vw_handle* h, cudaError_t e, const char* where) {
+    return fail(h, VW_ERR_CUDA, std::string(where) + ": " + cudaGetErrorString(e));
+}
+
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+
+inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+// Grows a buffer of the handle to `need` bytes (waits for the handle's stream before it frees the old one).
+inline vw_status grow(vw_handle* h, char** buf, size_t* cap, size_t need, const char* what) {
+    if (need <= *cap) return VW_OK;
+    if (*buf) {
+        cudaError_t e = cudaStreamSynchronize(h->stream);
+        if (e != cudaSuccess) return cuda_fail(h, e, what);
+        cudaFree(*buf);
+        *buf = nullptr;
+        *cap = 0;
+    }
+    const size_t n = round_up(need + need / 4, 1 << 20);
+    cudaError_t e = cudaMalloc(reinterpret_cast<void**>(buf), n);
+    if (e != cudaSuccess) return cuda_fail(h, e, what);
+    *cap = n;
+    return VW_OK;
+}
+
+// Waits for `st` and turns, then clears, the device error word.
+vw_status read_device_error(vw_handle* h, cudaStream_t st);

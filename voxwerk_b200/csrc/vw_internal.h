@@ -40,6 +40,9 @@ enum : unsigned {
     kErrBadOption = 4u,   // a row's option index outside the table
     kErrHistOffsets = 8u, // a row's history offsets negative or decreasing (the row is sampled without history)
     kErrCodeRange = 16u,  // a frame code outside its codebook (vw_frame_embedding; the row is not written)
+    kErrPageRange = 32u,  // a page table names a page outside the key/value cache
+    kErrPosition = 64u,   // a row's position is outside the rotation table (vw_rope_append; the row is not written)
+    kErrKvLens = 128u,    // key counts, row offsets or group offsets that do not fit the batch they describe
 };
 
 constexpr int kMaxCodeGroups = 16;     // codebooks per frame (Qwen3TtsConfig.NumCodeGroups)
