@@ -539,6 +539,7 @@ VW_EXPORT vw_status vw_create(int32_t device, vw_handle** out) {
     if (e == cudaSuccess) e = cudaMallocHost(&h->h_err, sizeof(unsigned));
     if (e == cudaSuccess) e = cudaMemset(h->d_err, 0, sizeof(unsigned));
     if (e == cudaSuccess) e = cudaEventCreateWithFlags(&h->opts_done, cudaEventDisableTiming);
+    if (e == cudaSuccess) e = cudaEventCreateWithFlags(&h->attn_done, cudaEventDisableTiming);
     for (int i = 0; i < kCopyStreams && e == cudaSuccess; ++i)
         e = cudaStreamCreateWithFlags(&h->copy_streams[i], cudaStreamNonBlocking);
     for (int i = 0; i <= kCopyStreams && e == cudaSuccess; ++i)
@@ -572,6 +573,8 @@ VW_EXPORT vw_status vw_destroy(vw_handle* h) {
         if (h->d_scratch) cudaFree(h->d_scratch);
         if (h->d_stage) cudaFree(h->d_stage);
         if (h->d_logits) cudaFree(h->d_logits);
+        if (h->d_attn) cudaFree(h->d_attn);
+        if (h->attn_done) cudaEventDestroy(h->attn_done);
         if (h->d_opts) cudaFree(h->d_opts);
         if (h->h_opts) cudaFreeHost(h->h_opts);
         if (h->d_err) cudaFree(h->d_err);

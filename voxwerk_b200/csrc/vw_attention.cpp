@@ -70,6 +70,50 @@ vw::AttnRowsDev rows_dev(const vw_attn_rows& r) {
             static_cast<__nv_bfloat16*>(r.out), r.out_row_stride, r.out_head_stride, r.lse, r.n_q_heads, r.scale};
 }
 
+// The attention workspace is one buffer of the handle: a call on another stream than the last one waits for it.  Inside
+// a stream capture no order is added (an event of uncaptured work cannot be waited for there): the caller orders its
+// graphs.
+cudaError_t enter_workspace(vw_handle* h, cudaStream_t st, bool* capturing) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    cudaError_t e = cudaStreamIsCapturing(st, &cap);
+    *capturing = cap != cudaStreamCaptureStatusNone;
+    if (e == cudaSuccess && !*capturing && h->attn_stream && h->attn_stream != st)
+        e = cudaStreamWaitEvent(st, h->attn_done, 0);
+    return e;
+}
+cudaError_t leave_workspace(vw_handle* h, cudaStream_t st, bool capturing) {
+    if (capturing) return cudaSuccess;
+    h->attn_stream = st;
+    return cudaEventRecord(h->attn_done, st);
+}
+
+constexpr size_t kAttnHeader = 256;   // counters (zero between calls), units_per_cta
+
+// Room for a plan's partial results; the buffer grows outside captures only.
+vw_status tile_work(vw_handle* h, const vw::TilePlan& plan, cudaStream_t st, vw::TileWork* w) {
+    const size_t ends = round_up(static_cast<size_t>(plan.unit_ends) * 8, 256);
+    const size_t lse = round_up(static_cast<size_t>(plan.part_rows) * 4, 256);
+    const size_t need = kAttnHeader + ends + lse + static_cast<size_t>(plan.part_rows) * plan.dim * 4;
+    if (need > h->attn_bytes) {
+        cudaError_t e = cudaDeviceSynchronize();   // an earlier call, on any stream, may still use the old buffer
+        if (e == cudaSuccess && h->d_attn) e = cudaFree(h->d_attn);
+        h->d_attn = nullptr;
+        h->attn_bytes = 0;
+        const size_t bytes = round_up(need + need / 4, 1 << 20);
+        if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&h->d_attn), bytes);
+        if (e == cudaSuccess) e = cudaMemsetAsync(h->d_attn, 0, kAttnHeader, st);
+        if (e != cudaSuccess) return cuda_fail(h, e, "attention workspace");
+        h->attn_bytes = bytes;
+    }
+    char* at = h->d_attn;
+    w->counters = reinterpret_cast<int32_t*>(at);
+    w->units_per_cta = reinterpret_cast<int64_t*>(at + 64);
+    w->unit_end = reinterpret_cast<int64_t*>(at + kAttnHeader);
+    w->part_lse = reinterpret_cast<float*>(at + kAttnHeader + ends);
+    w->part_o = reinterpret_cast<float*>(at + kAttnHeader + ends + lse);
+    return VW_OK;
+}
+
 }  // namespace
 
 VW_EXPORT vw_status vw_rope_append(vw_handle* h, const vw_kv_cache* cache, const vw_kv_batch* batch,
@@ -152,7 +196,15 @@ VW_EXPORT vw_status vw_prompt_attention(vw_handle* h, const vw_kv_cache* cache, 
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
     vw::AttnParams p{rows_dev(*rows), cache_dev(*cache), batch_dev(*batch), vw::KvPrefixDev{}, h->d_err};
     cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess) e = vw::launch_prompt_attention(p, st);
+    bool capturing = false;
+    if (e == cudaSuccess) e = enter_workspace(h, st, &capturing);
+    if (e != cudaSuccess) return cuda_fail(h, e, "prompt attention");
+    const vw::TilePlan plan = vw::plan_prompt(p, h->sm_count);
+    vw::TileWork w{};
+    r = tile_work(h, plan, st, &w);
+    if (r != VW_OK) return r;
+    e = vw::launch_prompt_attention(p, plan, w, st);
+    if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
     if (e != cudaSuccess) return cuda_fail(h, e, "prompt attention");
     if (!stream) return read_device_error(h, st);
     return VW_OK;

@@ -1,95 +1,949 @@
-// vw_prompt.cu -- attention over a paged key/value cache (include/vwsampler.h, vw_prompt_attention and
-// vw_decode_attention): softmax(scale q k^T) v of each row over the keys it sees.
+// vw_prompt.cu -- attention of many rows over a paged key/value cache on the tensor cores (include/vwsampler.h):
+// vw_prompt_attention, and the shared prefixes of vw_decode_attention.
 //
-// One warp per (row, query head), each lane four dims of the head, one pass over the keys with the running maximum m
-// and sum l of the softmax in fp32: o and l are scaled by exp(m - m') when the maximum rises to m'.
+// out = softmax(scale Q K^T) V in one pass over the keys: a block of query rows keeps the running maximum m and sum l
+// of its scores in registers and its output O in tensor memory; a tile of 128 keys adds P V with P = exp2(c S - c m),
+// c = scale log2(e).  O and l are brought to a new maximum only when it has risen by more than 2^8 (P then stays below
+// 2^8, far inside bf16's and fp32's range, and the factor cancels in O / l), so O is hardly ever touched.
+//
+// A block is two tiles of up to 128 rows of one key head: the rows of a tile are (token, query head) pairs, so grouped
+// heads share every key and value read.  One CTA per SM, 12 warps:
+//   warp 0     schedules the blocks and loads by TMA: Q once per block, then K and V tiles (page boxes) into a ring;
+//   warp 1     one thread issues every tcgen05.mma: S = Q K^T (operands in shared memory) and O += P V (P from tensor
+//              memory); the two row tiles alternate, so one tile's products run while the other's softmax does;
+//   warp 2     clears the rows past a sequence's last key in its last V tile (pages end inside a tile, and what lies
+//              there may be anything: 0 * NaN would reach every row);
+//   warps 4-7, 8-11   one warpgroup per row tile, one thread per row: S from tensor memory, maximum, exponentials, P
+//              back over S as bf16, and at the end O / l to the output.
+// Tensor memory (512 columns): S0 S1 (128 fp32 columns each, P over their first halves), O0 O1.
+//
+// Schedule.  Blocks in order of decreasing key count from a ticket counter, so that the last ones are short.  Where
+// there are too few blocks for the SMs, the (block, tile) units are dealt evenly instead, a block's pieces leave
+// partial results (O / l and log2-sum in fp32), and a join kernel, or the decode kernel, weighs them together.
+//
+// Every mbarrier wait is bounded; on expiry an error bit is set, every role stops and drains, tensor memory is freed.
 
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdint>
 
 #include "vw_attention.h"
 #include "vw_internal.h"
+#include "vw_tc.cuh"
 
 namespace vw {
 namespace {
 
-struct Softmax {
-    float m = -INFINITY, l = 0.0f, o[4] = {};
+constexpr int kThreads384 = 384;
+constexpr int kKeys = 128;        // keys per tile
+constexpr int kRows = 128;        // rows per row tile
+constexpr int kWholeKeys = 512;   // sequences of at most this many keys are never split
+constexpr int kMinPromptUnits = 2;
+constexpr int kFeedRegs = 96, kSoftmaxRegs = 200;   // registers per thread of warps 0-3 and 4-11
+constexpr float kLn2 = 0.693147180559945309f;
+constexpr int kItemSlots = 3;
+constexpr int kItemReaders = 10;  // MMA thread, warp 2, eight softmax warps
+
+template <int DP>   // head_dim padded to 64 or 128 (the TMA fills the rest with zeros)
+struct TileCfg {
+    static constexpr int kHalves = DP / 64;
+    static constexpr uint32_t kHalfBytes = 128 * 128;   // 128 rows of 64 bf16, 128-byte swizzle
+    static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
+    static constexpr int kStages = DP == 128 ? 5 : 8;
+    static constexpr uint32_t kOffKv = 2 * kTileBytes;   // after the two Q tiles
+    static constexpr uint32_t kOffBar = kOffKv + kStages * kTileBytes;
+    // kv_full[S] kv_empty[S] q_full q_empty s_full[2] p_full[2] o_full[2] v_tail v_fixed item_full[3] item_empty[3] done
+    static constexpr uint32_t kBars = 2 * kStages + 17;
+    static constexpr uint32_t kOffItems = kOffBar + 8 * kBars;
+    static constexpr uint32_t kOffMisc = kOffItems + kItemSlots * 64;
+    static constexpr uint32_t kBytes = kOffMisc + 16;
+    static_assert(kBytes + 1024 <= 232448, "shared memory");
 };
 
-__device__ void attend(const AttnParams& p, const int32_t* table, int keys, int kv_head, int d0, const float* q,
-                       Softmax& s) {
-    const KvCacheDev& c = p.cache;
-    for (int j = 0; j < keys; ++j) {
-        const int page = table[j >> c.page_shift];
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.n_pages)) {
-            atomicOr(p.err, kErrPageRange);
-            continue;
+struct Item {            // a block, or a piece of one
+    int32_t valid;
+    int32_t row0, tokens;        // first row of the call, tokens (rows per query head) of the block
+    int32_t pos0, kv;            // index of the first token among the sequence's keys; keys of the sequence
+    int32_t seq, kv_head;
+    int32_t tile0, end[2];       // key tiles [tile0, end[q]) of row tile q
+    int32_t part_row;            // first partial row, or -1: the result goes to the output
+};
+static_assert(sizeof(Item) <= 64, "item slots");
+
+struct TileParams {
+    AttnParams a;
+    int32_t group;               // query heads per key head
+    int32_t tile_tokens;         // tokens per row tile: floor(128 / group)
+    int32_t split;               // units dealt evenly (pieces) instead of whole blocks by ticket
+    int32_t min_units;           // fewest units a CTA takes (split)
+    float c;                     // |scale| log2(e), not 0
+    int32_t negate;              // scale < 0
+    TileWork w;
+};
+
+struct Seq {
+    int32_t row0, n, kv, past;   // first row, tokens, keys, keys before the first token's own
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+template <bool kPrefix>
+__device__ Seq load_seq(const TileParams& p, int s) {
+    Seq q{0, 0, 0, 0};
+    const AttnParams& a = p.a;
+    const int shift = a.cache.page_shift;
+    const int32_t* o = kPrefix ? a.prefix.group_offsets : a.batch.q_offsets;
+    const int limit = kPrefix ? a.batch.n_seqs : a.batch.n_rows;
+    int begin = s, end = min(s + 1, limit);
+    if (o) {
+        begin = o[s];
+        end = o[s + 1];
+    }
+    q.kv = kPrefix ? checked_len(a.prefix.lens[s], a.prefix.max_pages, shift, a.err, kErrKvLens)
+                   : checked_len(a.batch.kv_lens[s], a.batch.max_pages, shift, a.err, kErrKvLens);
+    if (begin < 0 || end < begin || end > limit) {
+        atomicOr(a.err, kErrKvLens);
+        return q;
+    }
+    q.row0 = begin;
+    q.n = end - begin;
+    q.past = q.kv - q.n;
+    return q;
+}
+
+// Keys that tokens [.., t) of a sequence see together
+template <bool kPrefix>
+__device__ __forceinline__ int keys_seen(const Seq& q, int t) {
+    return kPrefix ? q.kv : min(max(q.past + min(q.n, t), 0), q.kv);
+}
+// Units of a sequence's block i (split): its key tiles, at least one for a prompt's block (its rows are written)
+template <bool kPrefix>
+__device__ __forceinline__ int block_units(const Seq& q, int i, int block_tokens) {
+    return max(ceil_div(keys_seen<kPrefix>(q, (i + 1) * block_tokens), kKeys), kPrefix ? 0 : 1);
+}
+template <bool kPrefix>
+__device__ int64_t seq_units(const Seq& q, int block_tokens, int kv_heads) {
+    const int blocks = ceil_div(q.n, block_tokens);
+    int64_t u = 0;
+    if (kPrefix)
+        u = static_cast<int64_t>(blocks) * block_units<kPrefix>(q, 0, block_tokens);
+    else
+        for (int i = 0; i < blocks; ++i) u += block_units<kPrefix>(q, i, block_tokens);
+    return u * kv_heads;
+}
+
+__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+// The whole warp fills an item from block i of sequence s, key tiles [t0, t1) of it.
+template <bool kPrefix>
+__device__ Item make_item(const TileParams& p, const Seq& q, int s, int i, int kv_head, int t0, int t1, bool whole,
+                          int cta) {
+    const int tt = p.tile_tokens, first = 2 * tt * i;
+    Item it;
+    it.valid = 1;
+    it.row0 = q.row0 + first;
+    it.tokens = min(2 * tt, q.n - first);
+    it.pos0 = q.past + first;
+    it.kv = q.kv;
+    it.seq = s;
+    it.kv_head = kv_head;
+    it.tile0 = t0;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int n = min(max(it.tokens - h * tt, 0), tt);
+        const int end = n ? ceil_div(keys_seen<kPrefix>(q, first + h * tt + n), kKeys) : 0;
+        it.end[h] = max(min(end, t1), t0);
+    }
+    const int rows = it.tokens * p.group;
+    it.part_row = whole && !kPrefix ? -1
+                                    : q.row0 * p.a.rows.n_q_heads + i * p.a.cache.n_kv_heads * 2 * tt * p.group +
+                                          kv_head * rows + cta * kPartRows;
+    return it;
+}
+
+// The schedule, walked by the 32 lanes of warp 0 together.
+template <bool kPrefix>
+struct Scheduler {
+    const TileParams& p;
+    int lane, n_seqs, block_tokens, kv_heads;
+    // by ticket
+    int ticket, level, base;
+    int64_t before;
+    // split
+    int64_t unit, unit_end, seq_first;   // the CTA's units; the first unit of sequence `seq`
+    int seq;
+
+    __device__ Scheduler(const TileParams& params, int l) : p(params), lane(l) {
+        n_seqs = kPrefix ? p.a.prefix.n_groups : p.a.batch.n_seqs;
+        block_tokens = 2 * p.tile_tokens;
+        kv_heads = p.a.cache.n_kv_heads;
+        if (p.split) {
+            int64_t total = 0;
+            for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+                const int s = s0 + lane;
+                int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p, s), block_tokens, kv_heads) : 0;
+                u = warp_scan(u, lane);
+                if (blockIdx.x == 0 && s < n_seqs) p.w.unit_end[s] = total + u;   // for the kernels that join
+                total += __shfl_sync(0xffffffffu, u, 31);
+            }
+            const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(p.min_units));
+            if (blockIdx.x == 0 && lane == 0) *p.w.units_per_cta = per;
+            unit = min(per * blockIdx.x, total);
+            unit_end = min(unit + per, total);
+            seq = 0;
+            seq_first = 0;
+            if (unit < unit_end) {   // the sequence that holds `unit`
+                for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+                    const int s = s0 + lane;
+                    const int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p, s), block_tokens, kv_heads) : 0;
+                    const int64_t sum = warp_scan(u, lane);
+                    const unsigned m = __ballot_sync(0xffffffffu, seq_first + sum > unit);
+                    if (m) {
+                        const int at = __ffs(m) - 1;
+                        seq = s0 + at;
+                        seq_first += __shfl_sync(0xffffffffu, sum - u, at);
+                        break;
+                    }
+                    seq_first += __shfl_sync(0xffffffffu, sum, 31);
+                }
+            }
+        } else {
+            ticket = blockIdx.x;
+            int top = -1;
+            for (int s = lane; s < n_seqs; s += 32) {
+                const Seq q = load_seq<kPrefix>(p, s);
+                if (q.n > 0) top = max(top, first_level(q) + ceil_div(q.n, block_tokens) - 1);
+            }
+            level = __reduce_max_sync(0xffffffffu, top);
+            base = 0;
+            before = 0;
         }
-        const int64_t at = page * c.page_stride + (j & (c.page_size - 1)) * c.token_stride + kv_head * c.head_stride + d0;
-        float x = 0.0f;
-        if (d0 < c.head_dim)
-            for (int i = 0; i < 4; ++i) x = __fmaf_rn(q[i], __bfloat162float(c.k[at + i]), x);
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        const float m = fmaxf(s.m, x);
-        const float w = expf(x - m), f = expf(s.m - m);
-        s.m = m;
-        s.l = __fmaf_rn(s.l, f, w);
-        if (d0 < c.head_dim)
-            for (int i = 0; i < 4; ++i) s.o[i] = __fmaf_rn(s.o[i], f, w * __bfloat162float(c.v[at + i]));
+    }
+    // Blocks are taken level by level from the highest: a block's level is its key count in units of block tokens
+    __device__ int first_level(const Seq& q) const { return max(q.past, 0) / block_tokens; }
+
+    __device__ Item next() {
+        Item none;
+        none.valid = 0;
+        if (p.split) return unit < unit_end ? next_piece() : none;
+        while (level >= 0) {
+            const int s = base + lane;
+            Seq q{0, 0, 0, 0};
+            int i = -1;
+            if (s < n_seqs) {
+                q = load_seq<kPrefix>(p, s);
+                i = level - first_level(q);
+                if (q.n <= 0 || i >= ceil_div(q.n, block_tokens)) i = -1;
+            }
+            const unsigned m = __ballot_sync(0xffffffffu, i >= 0);
+            const int64_t slot = ticket / kv_heads - before;
+            if (slot < __popc(m)) {
+                const int at = __fns(m, 0, static_cast<int>(slot) + 1);
+                q.row0 = __shfl_sync(0xffffffffu, q.row0, at);
+                q.n = __shfl_sync(0xffffffffu, q.n, at);
+                q.kv = __shfl_sync(0xffffffffu, q.kv, at);
+                q.past = __shfl_sync(0xffffffffu, q.past, at);
+                i = __shfl_sync(0xffffffffu, i, at);
+                const Item it = make_item<kPrefix>(p, q, base + at, i, ticket % kv_heads, 0, INT32_MAX, true, 0);
+                if (lane == 0) ticket = gridDim.x + atomicAdd(p.w.counters, 1);
+                ticket = __shfl_sync(0xffffffffu, ticket, 0);
+                return it;
+            }
+            before += __popc(m);
+            base += 32;
+            if (base >= n_seqs) {
+                base = 0;
+                --level;
+            }
+        }
+        return none;
+    }
+
+    __device__ Item next_piece() {
+        Seq q = load_seq<kPrefix>(p, seq);   // every lane the same
+        int64_t units = seq_units<kPrefix>(q, block_tokens, kv_heads);
+        while (unit >= seq_first + units) {   // on to the sequence that holds `unit`
+            seq_first += units;
+            q = load_seq<kPrefix>(p, ++seq);
+            units = seq_units<kPrefix>(q, block_tokens, kv_heads);
+        }
+        int64_t first = seq_first;
+        int i = 0, cost;
+        if (kPrefix) {
+            cost = block_units<kPrefix>(q, 0, block_tokens);
+            i = static_cast<int>((unit - first) / (static_cast<int64_t>(cost) * kv_heads));
+            first += static_cast<int64_t>(i) * cost * kv_heads;
+        } else {
+            for (;; ++i) {
+                cost = block_units<kPrefix>(q, i, block_tokens);
+                if (unit < first + static_cast<int64_t>(cost) * kv_heads) break;
+                first += static_cast<int64_t>(cost) * kv_heads;
+            }
+        }
+        const int kv_head = static_cast<int>((unit - first) / cost);
+        first += static_cast<int64_t>(kv_head) * cost;
+        const int t0 = static_cast<int>(unit - first);
+        const int t1 = static_cast<int>(min(unit_end - first, static_cast<int64_t>(cost)));
+        unit = first + t1;
+        return make_item<kPrefix>(p, q, seq, i, kv_head, t0, t1, t0 == 0 && t1 == cost, blockIdx.x);
+    }
+};
+
+// value matrix descriptor: N-major (64 head dims contiguous), 128-byte swizzle; 64-dim halves kHalfBytes apart (LBO),
+// 8-key groups 1024 bytes apart (SBO)
+__device__ __forceinline__ uint64_t value_desc(uint32_t saddr) {
+    return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>((128 * 128) >> 4) << 16) |
+           (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tmem_load32(uint32_t addr, float* f) {
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, "
+        "%13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, "
+        "[%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]),
+          "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]),
+          "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const float* f) {
+    const uint32_t* v = reinterpret_cast<const uint32_t*>(f);
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22; -inf gives 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <int DP, bool kPrefix>
+__global__ void __launch_bounds__(kThreads384, 1)
+attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                      const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TileParams p) {
+    using C = TileCfg<DP>;
+    constexpr int S = C::kStages;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = s32(sm);
+    const uint32_t kv_full = sbase + C::kOffBar, kv_empty = kv_full + 8 * S;
+    const uint32_t q_full = kv_empty + 8 * S, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 16,
+                   o_full = p_full + 16, v_tail = o_full + 16, v_fixed = v_tail + 8, item_full = v_fixed + 8,
+                   item_empty = item_full + 8 * kItemSlots, done = item_empty + 8 * kItemSlots;
+    Item* items = reinterpret_cast<Item*>(sm + C::kOffItems);   // 64 bytes apart
+    auto item_slot = [&](uint32_t n) { return reinterpret_cast<Item*>(reinterpret_cast<uint8_t*>(items) + 64 * (n % kItemSlots)); };
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
+    volatile int32_t* abort = reinterpret_cast<volatile int32_t*>(sm + C::kOffMisc + 4);
+    unsigned* err = p.a.err;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
+        for (int s = 0; s < 2 * S; ++s) init(kv_full + 8 * s, 1);
+        init(q_full, 1);
+        init(q_empty, 1);
+        for (int q = 0; q < 2; ++q) {
+            init(s_full + 8 * q, 1);
+            init(p_full + 8 * q, 4);
+            init(o_full + 8 * q, 1);
+        }
+        init(v_tail, 1);
+        init(v_fixed, 1);
+        for (int s = 0; s < kItemSlots; ++s) {
+            init(item_full + 8 * s, 1);
+            init(item_empty + 8 * s, kItemReaders);
+        }
+        init(done, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *abort = 0;
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s32(tmem_slot)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    // one setmaxnreg for each warpgroup
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFeedRegs));
+        if (warp == 0) {
+            // ---------------- schedule and loads
+            const KvCacheDev& cache = p.a.cache;
+            const int shift = cache.page_shift;
+            const int boxes = cache.page_size >= kKeys ? 1 : kKeys >> shift;      // page boxes of a key tile
+            const int box_rows = min(cache.page_size, kKeys);
+            const int32_t* tables = kPrefix ? p.a.prefix.page_table : p.a.batch.page_table;
+            const int64_t table_stride = kPrefix ? p.a.prefix.page_table_stride : p.a.batch.page_table_stride;
+            Scheduler<kPrefix> sched(p, lane);
+            uint32_t n_items = 0, n_q = 0, st = 0;
+            bool stop = false;
+            while (!stop) {
+                const Item it = sched.next();
+                if (n_items >= kItemSlots &&
+                    !wait_bounded(item_empty + 8 * (n_items % kItemSlots), (n_items / kItemSlots - 1) & 1, abort, err))
+                    stop = true;
+                if (__any_sync(0xffffffffu, stop)) break;
+                if (lane == 0) {
+                    *item_slot(n_items) = it;
+                    arrive(item_full + 8 * (n_items % kItemSlots));
+                }
+                __syncwarp();
+                ++n_items;
+                if (!it.valid) break;
+                const int end = max(it.end[0], it.end[1]);
+                if (end <= it.tile0) continue;
+                // page of this lane's box of a key tile; past the block's last key: no box
+                const int seen = kPrefix ? it.kv : min(max(it.pos0 + it.tokens, 0), it.kv);
+                const int32_t* table = tables + it.seq * table_stride;
+                auto page_of = [&](int t) {
+                    const int key = t * kKeys + lane * box_rows;
+                    if (lane >= boxes || key >= seen || t >= end) return -1;
+                    const int page = table[key >> shift];
+                    if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.n_pages)) {
+                        atomicOr(err, kErrPageRange);
+                        return cache.n_pages;   // past the map's end: zeros
+                    }
+                    return page;
+                };
+                int page = page_of(it.tile0);
+                if (n_q > 0 && !wait_bounded(q_empty, (n_q - 1) & 1, abort, err)) stop = true;
+                if (__any_sync(0xffffffffu, stop)) break;
+                ++n_q;
+                if (lane == 0) {
+                    const int tiles = it.end[1] > it.tile0 ? 2 : 1;   // row tile 1 sees at least row tile 0's keys
+                    const uint32_t box = C::kHalves * 128 * p.tile_tokens * p.group;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(q_full), "r"(tiles * box)
+                                 : "memory");
+                    for (int q = 0; q < tiles; ++q)
+                        for (int h = 0; h < C::kHalves; ++h)
+                            tma_load_3d(sbase + q * C::kTileBytes + h * C::kHalfBytes, &map_q, 64 * h, it.kv_head * p.group,
+                                        it.row0 + q * p.tile_tokens, q_full);
+                }
+                for (int t = it.tile0; t < end && !stop; ++t) {
+                    const int next = page_of(t + 1);
+                    const uint32_t mine = __ballot_sync(0xffffffffu, page >= 0);
+                    const uint32_t bytes = __popc(mine) * box_rows * 128 * C::kHalves;
+    #pragma unroll
+                    for (int kv = 0; kv < 2; ++kv, ++st) {
+                        const uint32_t s = st % S;
+                        if (st >= S && !wait_bounded(kv_empty + 8 * s, (st / S - 1) & 1, abort, err)) stop = true;
+                        if (__any_sync(0xffffffffu, stop)) {
+                            stop = true;
+                            break;
+                        }
+                        if (lane == 0)
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kv_full + 8 * s),
+                                         "r"(bytes)
+                                         : "memory");
+                        __syncwarp();
+                        if (page >= 0) {
+                            const int token = (t * kKeys) & (cache.page_size - 1);
+    #pragma unroll
+                            for (int h = 0; h < C::kHalves; ++h)
+                                tma_load_4d(sbase + C::kOffKv + s * C::kTileBytes + h * C::kHalfBytes + lane * box_rows * 128,
+                                            kv ? &map_v : &map_k, 64 * h, token, it.kv_head, page, kv_full + 8 * s);
+                        }
+                    }
+                    page = next;
+                }
+            }
+            // teardown: the copies in flight land before the CTA may exit
+            if (lane == 0) {
+                if (n_q > 0) drain_wait(q_full, (n_q - 1) & 1);
+                for (uint32_t j = st > S ? st - S : 0; j < st; ++j) drain_wait(kv_full + 8 * (j % S), (j / S) & 1);
+            }
+            __syncwarp();
+        } else if (warp == 1) {
+            // ---------------- matrix products (one thread)
+            if (lane == 0) {
+                const int D = p.a.cache.head_dim;
+                const int k_steps = (D + 15) / 16;                        // of Q K^T
+                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kRows >> 4) << 24);   // fp32 += bf16 x bf16
+                const uint32_t idesc_pv = idesc | (1u << 16) | (static_cast<uint32_t>(2 * k_steps) << 17);   // V is N-major
+                uint32_t st = 0, n_q = 0, n_p[2] = {0, 0}, n_fixed = 0;
+                bool stop = false;
+                for (uint32_t n = 0; !stop; ++n) {
+                    if (!wait_bounded(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err)) break;
+                    const Item it = *item_slot(n);
+                    arrive(item_empty + 8 * (n % kItemSlots));
+                    if (!it.valid) break;
+                    const int end = max(it.end[0], it.end[1]);
+                    if (end <= it.tile0) continue;
+                    int seen[2];   // keys the tile's last row sees
+                    for (int q = 0; q < 2; ++q)
+                        seen[q] = kPrefix ? it.kv : min(max(it.pos0 + min(it.tokens, (q + 1) * p.tile_tokens), 0), it.kv);
+                    const int all = max(seen[0], seen[1]);
+                    const bool fix = ((all + 15) & ~15) > it.kv;   // the last tile's value rows past it.kv are cleared
+                    if (!wait_bounded(q_full, n_q++ & 1, abort, err)) break;
+                    for (int t = it.tile0; t <= end && !stop; ++t) {
+                        // tile t: S(t) after P V(t - 1), so that P's columns are free for S
+                        const uint32_t sk = st % S, sv = (st + S - 1) % S;   // stages of K(t) and V(t - 1)
+                        if (t > it.tile0) {
+                            if (!wait_bounded(kv_full + 8 * sv, ((st - 1) / S) & 1, abort, err)) {
+                                stop = true;
+                                break;
+                            }
+                            if (fix && t == (all + kKeys - 1) / kKeys) {
+                                arrive(v_tail);   // V(t - 1) has landed: warp 2 may clear its tail
+                                if (!wait_bounded(v_fixed, n_fixed++ & 1, abort, err)) {
+                                    stop = true;
+                                    break;
+                                }
+                            }
+                        }
+                        if (t < end && !wait_bounded(kv_full + 8 * sk, (st / S) & 1, abort, err)) {
+                            stop = true;
+                            break;
+                        }
+    #pragma unroll
+                        for (int q = 0; q < 2; ++q) {
+                            if (t > it.tile0 && t - 1 < it.end[q]) {
+                                if (!wait_bounded(p_full + 8 * q, n_p[q]++ & 1, abort, err)) {
+                                    stop = true;
+                                    break;
+                                }
+                                fence_after();
+                                const uint32_t v0 = sbase + C::kOffKv + sv * C::kTileBytes;
+                                const int steps = (min(seen[q] - (t - 1) * kKeys, kKeys) + 15) / 16;
+                                for (int k = 0; k < steps; ++k) {
+                                    const uint32_t accumulate = (t - 1 > it.tile0 || k > 0) ? 1u : 0u;
+                                    asm volatile(
+                                        "{\n\t.reg .pred p;\n\t"
+                                        "setp.ne.b32 p, %4, 0;\n\t"
+                                        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(
+                                            tmem + 256 + 128 * q),
+                                        "r"(tmem + 128 * q + 8 * k), "l"(value_desc(v0 + 2048 * k)), "r"(idesc_pv),
+                                        "r"(accumulate)
+                                        : "memory");
+                                }
+                                if (t == it.end[q]) mma_commit(o_full + 8 * q);
+                            }
+                            if (t < it.end[q]) {
+                                fence_after();
+                                const uint32_t a0 = sbase + q * C::kTileBytes, b0 = sbase + C::kOffKv + sk * C::kTileBytes;
+                                const int n16 = (min(seen[q] - t * kKeys, kKeys) + 15) / 16;
+                                const uint32_t id = idesc | (static_cast<uint32_t>(2 * n16) << 17);
+                                for (int k = 0; k < k_steps; ++k) {
+                                    const uint32_t off = (k >> 2) * C::kHalfBytes + 32 * (k & 3);
+                                    const uint32_t accumulate = k > 0 ? 1u : 0u;
+                                    asm volatile(
+                                        "{\n\t.reg .pred p;\n\t"
+                                        "setp.ne.b32 p, %4, 0;\n\t"
+                                        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + 128 * q),
+                                        "l"(umma_desc(a0 + off)), "l"(umma_desc(b0 + off)), "r"(id), "r"(accumulate)
+                                        : "memory");
+                                }
+                                mma_commit(s_full + 8 * q);
+                            }
+                        }
+                        if (stop) break;
+                        if (t > it.tile0) mma_commit(kv_empty + 8 * sv);
+                        if (t < end) {
+                            mma_commit(kv_empty + 8 * sk);
+                            if (t == end - 1) mma_commit(q_empty);
+                            st += 2;
+                        }
+                    }
+                }
+                // teardown: every product issued has completed before the tensor memory is freed
+                mma_commit(done);
+                drain_wait(done, 0);
+            }
+            __syncwarp();
+        } else if (warp == 2) {
+            // ---------------- clears value rows past a sequence's last key
+            uint32_t st = 0, n_fixed = 0;
+            for (uint32_t n = 0;; ++n) {
+                bool ok = wait_bounded(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                const Item it = *item_slot(n);
+                __syncwarp();
+                if (lane == 0) arrive(item_empty + 8 * (n % kItemSlots));
+                if (!it.valid) break;
+                const int end = max(it.end[0], it.end[1]);
+                if (end <= it.tile0) continue;
+                const int all = kPrefix ? it.kv : min(max(it.pos0 + it.tokens, 0), it.kv);
+                const int upto = (all + 15) & ~15;
+                if (upto > it.kv && end == (all + kKeys - 1) / kKeys) {
+                    const uint32_t j = st + 2 * (end - 1 - it.tile0) + 1, s = j % S;   // the stage of V(end - 1)
+                    // (its own phase of kv_full: the stage is not released before v_fixed)
+                    ok = wait_bounded(v_tail, n_fixed++ & 1, abort, err) &&
+                         wait_bounded(kv_full + 8 * s, (j / S) & 1, abort, err);
+                    if (!__all_sync(0xffffffffu, ok)) break;
+                    const int r0 = it.kv - (end - 1) * kKeys, rows = upto - it.kv;
+                    for (int h = 0; h < C::kHalves; ++h)
+                        for (int i = lane; i < rows * 8; i += 32)
+                            *reinterpret_cast<uint4*>(sm + C::kOffKv + s * C::kTileBytes + h * C::kHalfBytes + r0 * 128 +
+                                                      16 * i) = make_uint4(0, 0, 0, 0);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // visible to the products
+                    __syncwarp();
+                    if (lane == 0) arrive(v_fixed);
+                }
+                st += 2 * (end - it.tile0);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        // ---------------- softmax: warps 4-7 row tile 0, warps 8-11 row tile 1, a thread per row
+        const int q = (warp - 4) >> 2;
+        const int row = 32 * (warp & 3) + lane;
+        const uint32_t quarter = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+        const uint32_t t_s = tmem + quarter + 128 * q, t_o = tmem + quarter + 256 + 128 * q;
+        const int token = q * p.tile_tokens + row / p.group, sub = row % p.group;
+        const bool in_tile = row < p.tile_tokens * p.group;
+        const float2 c2 = make_float2(p.c, p.c);
+        uint32_t n_s = 0, n_o = 0;
+        bool stop = false;
+        for (uint32_t n = 0; !stop; ++n) {
+            bool ok = wait_bounded(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const Item it = *item_slot(n);
+            __syncwarp();
+            if (lane == 0) arrive(item_empty + 8 * (n % kItemSlots));
+            if (!it.valid) break;
+            const bool live = in_tile && token < it.tokens;
+            const int limit = !live ? 0 : kPrefix ? it.kv : min(it.pos0 + token + 1, it.kv);   // keys this row sees
+            const bool any_live = __any_sync(0xffffffffu, live);
+            float m = -INFINITY, l = 0.0f;
+            for (int t = it.tile0; t < it.end[q]; ++t, ++n_s) {
+                ok = wait_bounded(s_full + 8 * q, n_s & 1, abort, err);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    stop = true;
+                    break;
+                }
+                fence_after();
+                if (any_live) {
+                    float s[kKeys];
+#pragma unroll
+                    for (int i = 0; i < kKeys; i += 32) tmem_load32(t_s + i, s + i);
+                    tmem_wait_load();
+                    if (p.negate) {
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
+                    }
+                    const int columns = limit - t * kKeys;
+                    if (!__all_sync(0xffffffffu, columns >= kKeys || !live)) {
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i) s[i] = i < columns ? s[i] : -INFINITY;
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(s[j], s[4 + j]);
+#pragma unroll
+                    for (int i = 8; i < kKeys; i += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], fmaxf(s[i + j], s[i + 4 + j]));
+                    const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                    // a first maximum is taken as it is (nothing but zeros was summed); a later one when it rose enough
+                    const bool rise = live && m != -INFINITY && (tile_max - m) * p.c > 8.0f;
+                    if (__any_sync(0xffffffffu, rise)) {   // products up to t - 1 are done: S(t) came after them
+                        const float f = rise ? exp2_fast((m - tile_max) * p.c) : 1.0f;
+                        l *= f;
+                        if (rise) m = tile_max;
+#pragma unroll 1
+                        for (int i = 0; i < DP; i += 32) {
+                            float o[32];
+                            tmem_load32(t_o + i, o);
+                            tmem_wait_load();
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) o[j] *= f;
+                            tmem_store32(t_o + i, o);
+                        }
+                        tmem_wait_store();
+                    }
+                    if (m == -INFINITY) m = tile_max;
+                    const float mc = m == -INFINITY ? 0.0f : -m * p.c;
+                    const float2 mc2 = make_float2(mc, mc);
+                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                    for (int i = 0; i < kKeys; i += 32) {
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 x = fma2(make_float2(s[i + j], s[i + j + 1]), c2, mc2);
+                            const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
+                            pk[j >> 1] = pack_bf16(e.x, e.y);   // the product's operand; the sum keeps fp32
+                        }
+                        tmem_store16(t_s + (i >> 1), pk);
+                    }
+                    const float2 both = add2(sum[0], sum[1]);
+                    l += both.x + both.y;
+                    tmem_wait_store();
+                }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(p_full + 8 * q);
+            }
+            if (stop) break;
+            const bool some = it.end[q] > it.tile0;
+            if (some) {
+                ok = wait_bounded(o_full + 8 * q, n_o++ & 1, abort, err);
+                if (!__all_sync(0xffffffffu, ok)) break;
+                fence_after();
+            }
+            if (!any_live) continue;
+            const float r = l > 0.0f || l != l ? 1.0f / l : 0.0f;   // no key seen: 0 (a NaN stays one)
+            const int D = p.a.cache.head_dim;
+            const int64_t call_row = it.row0 + token;
+            const int head = it.kv_head * p.group + sub;
+            const bool part = it.part_row >= 0;
+            const int64_t part_row = static_cast<int64_t>(it.part_row) + token * p.group + sub;
+            if (live) {
+                const float lse = m * p.c + log2f(l);   // no key seen: -inf
+                if (part)
+                    p.w.part_lse[part_row] = lse;
+                else if (p.a.rows.lse)
+                    p.a.rows.lse[call_row * p.a.rows.n_q_heads + head] = lse * kLn2;
+            }
+            __nv_bfloat16* out = p.a.rows.out + call_row * p.a.rows.out_row + head * p.a.rows.out_head;
+            float* part_o = p.w.part_o + part_row * DP;
+#pragma unroll 1
+            for (int i = 0; i < DP; i += 32) {
+                float o[32];
+                if (some) {
+                    tmem_load32(t_o + i, o);
+                    tmem_wait_load();
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = some ? o[j] * r : 0.0f;
+                if (!live) continue;
+                if (part) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4*>(part_o + i + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        if (i + j < D)
+                            *reinterpret_cast<uint4*>(out + i + j) =
+                                make_uint4(pack_bf16(o[j], o[j + 1]), pack_bf16(o[j + 2], o[j + 3]),
+                                           pack_bf16(o[j + 4], o[j + 5]), pack_bf16(o[j + 6], o[j + 7]));
+                }
+            }
+            fence_before();   // the next block's products may overwrite O once its P is handed over
+        }
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+    if (!p.split && threadIdx.x == 0) {   // the last CTA leaves the ticket counter ready for the next call
+        __threadfence();
+        if (atomicAdd(p.w.counters + 1, 1) == static_cast<int>(gridDim.x) - 1) {
+            p.w.counters[0] = 0;
+            p.w.counters[1] = 0;
+        }
     }
 }
 
-__global__ void __launch_bounds__(128) attention_kernel(const AttnParams p, int decode) {
-    const int lane = threadIdx.x & 31, d0 = 4 * lane;
+// Joins the pieces of the blocks that were split: one warp per (row, query head).
+template <int DP>
+__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileParams p) {
+    const int lane = threadIdx.x & 31;
+    const int heads = p.a.rows.n_q_heads, kv_heads = p.a.cache.n_kv_heads;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int heads = p.rows.n_q_heads, D = p.cache.head_dim;
-    const int64_t row = item / heads;
-    if (item == 0 && lane == 0) {   // the offsets ascend within the rows
-        const int32_t* o = decode ? p.prefix.group_offsets : p.batch.q_offsets;
-        const int n = decode ? p.prefix.n_groups : p.batch.n_seqs, end = decode ? p.batch.n_seqs : p.batch.n_rows;
-        for (int i = 0; o && i < n; ++i)
-            if (o[i] < 0 || o[i + 1] < o[i] || o[i + 1] > end) atomicOr(p.err, kErrKvLens);
-    }
-    const int head = static_cast<int>(item % heads);
-    if (row >= p.batch.n_rows) return;
-    const KvBatchDev& b = p.batch;
-    int seq = static_cast<int>(row), behind = 0;
-    if (b.q_offsets) {
-        for (seq = 0; seq < b.n_seqs && row >= b.q_offsets[seq + 1]; ++seq) {}
-        if (seq < b.n_seqs) behind = max(0, b.q_offsets[seq + 1] - 1 - static_cast<int>(row));
-    }
-    if (seq >= b.n_seqs) return;
-    const int keys = checked_len(b.kv_lens[seq], b.max_pages, p.cache.page_shift, p.err, kErrKvLens) - behind;
-    const int kv_head = head / (heads / p.cache.n_kv_heads);
-    float q[4] = {};
-    if (d0 < D)
-        for (int i = 0; i < 4; ++i)
-            q[i] = __bfloat162float(p.rows.q[row * p.rows.q_row + head * p.rows.q_head + d0 + i]) * p.rows.scale;
-    Softmax s;
-    for (int g = 0; decode && g < p.prefix.n_groups; ++g)
-        if (seq >= p.prefix.group_offsets[g] && seq < p.prefix.group_offsets[g + 1])
-            attend(p, p.prefix.page_table + g * p.prefix.page_table_stride,
-                   checked_len(p.prefix.lens[g], p.prefix.max_pages, p.cache.page_shift, p.err, kErrKvLens), kv_head, d0,
-                   q, s);
-    attend(p, b.page_table + seq * b.page_table_stride, keys, kv_head, d0, q, s);
-    const float r = s.l > 0.0f ? 1.0f / s.l : 0.0f;
-    if (d0 < D)
-        for (int i = 0; i < 4; ++i)
-            p.rows.out[row * p.rows.out_row + head * p.rows.out_head + d0 + i] = __float2bfloat16_rn(s.o[i] * r);
-    if (p.rows.lse && lane == 0) p.rows.lse[row * heads + head] = s.m + logf(s.l);
+    const int row = static_cast<int>(item / heads), head = static_cast<int>(item % heads);
+    if (row >= p.a.batch.n_rows) return;
+    const int s = p.a.batch.q_offsets ? find_sequence(p.a.batch.q_offsets, p.a.batch.n_seqs, row, lane) : row;
+    if (s < 0 || s >= p.a.batch.n_seqs) return;
+    const Seq q = load_seq<false>(p, s);
+    if (row < q.row0 || row >= q.row0 + q.n) return;
+    const int block_tokens = 2 * p.tile_tokens, i = (row - q.row0) / block_tokens, kv_head = head / p.group;
+    int64_t first = s > 0 ? p.w.unit_end[s - 1] : 0;
+    for (int j = 0; j < i; ++j) first += static_cast<int64_t>(kv_heads) * block_units<false>(q, j, block_tokens);
+    const int cost = block_units<false>(q, i, block_tokens);
+    first += static_cast<int64_t>(kv_head) * cost;
+    const int64_t per = *p.w.units_per_cta;
+    const int c0 = static_cast<int>(first / per), c1 = static_cast<int>((first + cost - 1) / per);
+    if (c0 == c1) return;   // whole: written by the tile kernel
+    const int tokens = min(block_tokens, q.n - i * block_tokens);
+    const int64_t part = static_cast<int64_t>(q.row0) * heads + static_cast<int64_t>(i) * kv_heads * block_tokens * p.group +
+                         static_cast<int64_t>(kv_head) * tokens * p.group +
+                         (row - q.row0 - i * block_tokens) * p.group + head % p.group;
+    PartSum<DP> sum;
+    sum.add(p.w, part, c0, c1, lane);
+    sum.write(p.a, row, head, lane);
 }
 
-cudaError_t launch(const AttnParams& p, int decode, cudaStream_t stream) {
-    const int64_t items = static_cast<int64_t>(p.batch.n_rows) * p.rows.n_q_heads;
-    attention_kernel<<<static_cast<unsigned>((items + 3) / 4), 128, 0, stream>>>(p, decode);
+struct Geometry {
+    int group, tile_tokens;
+};
+Geometry geometry(const AttnParams& a) {
+    const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
+    return {group, kRows / group};
+}
+
+bool make_maps(const AttnParams& a, const Geometry& g, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const cuuint64_t D = a.cache.head_dim;
+    const cuuint64_t q_dims[3] = {D, static_cast<cuuint64_t>(a.rows.n_q_heads), static_cast<cuuint64_t>(a.batch.n_rows)};
+    const cuuint64_t q_strides[2] = {static_cast<cuuint64_t>(a.rows.q_head) * 2, static_cast<cuuint64_t>(a.rows.q_row) * 2};
+    const cuuint32_t q_box[3] = {64, static_cast<cuuint32_t>(g.group), static_cast<cuuint32_t>(g.tile_tokens)};
+    const cuuint64_t c_dims[4] = {D, static_cast<cuuint64_t>(a.cache.page_size), static_cast<cuuint64_t>(a.cache.n_kv_heads),
+                                  static_cast<cuuint64_t>(a.cache.n_pages)};
+    const cuuint64_t c_strides[3] = {static_cast<cuuint64_t>(a.cache.token_stride) * 2,
+                                     static_cast<cuuint64_t>(a.cache.head_stride) * 2,
+                                     static_cast<cuuint64_t>(a.cache.page_stride) * 2};
+    const cuuint32_t c_box[4] = {64, static_cast<cuuint32_t>(std::min(a.cache.page_size, kKeys)), 1, 1};
+    auto encode = [&](CUtensorMap* m, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
+                      const cuuint32_t* box) {
+        return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, ones,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    return encode(q, 3, a.rows.q, q_dims, q_strides, q_box) && encode(k, 4, a.cache.k, c_dims, c_strides, c_box) &&
+           encode(v, 4, a.cache.v, c_dims, c_strides, c_box);
+}
+
+template <int DP, bool kPrefix>
+cudaError_t launch_tiles(const TileParams& p, const Geometry& g, int grid, cudaStream_t stream) {
+    CUtensorMap q, k, v;
+    if (!make_maps(p.a, g, &q, &k, &v)) return cudaErrorInvalidValue;
+    const int smem = static_cast<int>(TileCfg<DP>::kBytes) + 1024;
+    static std::atomic<uint64_t> attr_set{0};   // one bit per device ordinal whose attribute is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        cudaFuncAttributes fa;
+        e = cudaFuncGetAttributes(&fa, attention_tile_kernel<DP, kPrefix>);
+        // the warpgroups' register shares must fit what the block is launched with
+        if (e == cudaSuccess && fa.numRegs * kThreads384 < 128 * kFeedRegs + 256 * kSoftmaxRegs)
+            e = cudaErrorInvalidConfiguration;
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(attention_tile_kernel<DP, kPrefix>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
+    }
+    attention_tile_kernel<DP, kPrefix><<<grid, kThreads384, smem, stream>>>(q, k, v, p);
     return cudaGetLastError();
+}
+
+// scale as the kernels use it; 0 becomes a factor that leaves every probability the same
+void set_scale(TileParams& p) {
+    p.negate = p.a.rows.scale < 0.0f;
+    p.c = std::max(std::fabs(p.a.rows.scale) * 1.44269504088896341f, 1e-30f);
 }
 
 }  // namespace
 
-cudaError_t launch_prompt_attention(const AttnParams& p, cudaStream_t stream) { return launch(p, 0, stream); }
-cudaError_t launch_decode_attention(const AttnParams& p, cudaStream_t stream) { return launch(p, 1, stream); }
+// Whole blocks by ticket when there are at least two for each SM, or when no sequence can have more keys than
+// kWholeKeys; otherwise pieces of equal length.
+TilePlan plan_prompt(const AttnParams& a, int sms) {
+    const Geometry g = geometry(a);
+    const int block_tokens = 2 * g.tile_tokens;
+    const int64_t whole = a.batch.n_rows / block_tokens;
+    const int64_t blocks = (a.batch.n_seqs == 1 ? (a.batch.n_rows + block_tokens - 1) / block_tokens
+                                                : std::min<int64_t>(whole + a.batch.n_seqs, a.batch.n_rows)) *
+                           a.cache.n_kv_heads;
+    const int64_t keys = static_cast<int64_t>(a.batch.max_pages) * a.cache.page_size;
+    TilePlan plan{};
+    plan.split = blocks < 2 * sms && keys > kWholeKeys;
+    plan.grid = static_cast<int>(plan.split ? sms : std::min<int64_t>(blocks, sms));
+    if (plan.split) plan.part_rows = static_cast<int64_t>(a.batch.n_rows) * a.rows.n_q_heads + kPartRows * plan.grid;
+    plan.unit_ends = plan.split ? a.batch.n_seqs : 0;
+    plan.dim = a.cache.head_dim <= 64 ? 64 : 128;
+    return plan;
+}
+
+cudaError_t launch_prompt_attention(const AttnParams& a, const TilePlan& plan, const TileWork& w, cudaStream_t stream) {
+    const Geometry g = geometry(a);
+    TileParams p{a, g.group, g.tile_tokens, plan.split, kMinPromptUnits, 0.0f, 0, w};
+    set_scale(p);
+    cudaError_t e = plan.dim == 64 ? launch_tiles<64, false>(p, g, plan.grid, stream)
+                                   : launch_tiles<128, false>(p, g, plan.grid, stream);
+    if (e != cudaSuccess || !plan.split) return e;
+    const int64_t warps = static_cast<int64_t>(a.batch.n_rows) * a.rows.n_q_heads;
+    const unsigned grid = static_cast<unsigned>((warps + 3) / 4);
+    if (plan.dim == 64)
+        join_kernel<64><<<grid, 128, 0, stream>>>(p);
+    else
+        join_kernel<128><<<grid, 128, 0, stream>>>(p);
+    return cudaGetLastError();
+}
 
 }  // namespace vw

@@ -29,22 +29,6 @@ struct RowPlace {
     int32_t pos;
 };
 
-// The sequence whose rows hold `row`: the last s with offsets[s] <= row, found 32 probes at a time by one warp.
-__device__ int find_sequence(const int32_t* offsets, int n_seqs, int row, int lane) {
-    int lo = 0, n = n_seqs;   // the answer is in [lo, lo + n)
-    while (n > 1) {
-        const int step = (n + 31) / 32;
-        const int at = lo + lane * step;
-        const bool le = lane * step < n && offsets[at] <= row;
-        const unsigned m = __ballot_sync(0xffffffffu, le);
-        if (!m) return -1;
-        const int last = 31 - __clz(m);
-        n = min(step, n - last * step);
-        lo += last * step;
-    }
-    return lo;
-}
-
 __device__ RowPlace place_row(const RopeParams& p, int row, int lane) {
     RowPlace r{-1, 0};
     const KvBatchDev& b = p.batch;
