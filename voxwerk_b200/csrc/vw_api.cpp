@@ -297,6 +297,7 @@ vw_status read_device_error(vw_handle* h, cudaStream_t st) {
     if (bits) {
         cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
         if (h->d_defer) cudaMemsetAsync(h->d_defer, 0, kDeferHeader * sizeof(int32_t), st);
+        if (h->d_attn_counts) cudaMemsetAsync(h->d_attn_counts, 0, h->attn_counts_bytes, st);
         cudaStreamSynchronize(st);
     }
     if (bits & vw::kErrTimeout) return fail(h, VW_ERR_TIMEOUT, "a bounded wait in the sampler kernel gave up");
@@ -574,6 +575,7 @@ VW_EXPORT vw_status vw_destroy(vw_handle* h) {
         if (h->d_stage) cudaFree(h->d_stage);
         if (h->d_logits) cudaFree(h->d_logits);
         if (h->d_attn) cudaFree(h->d_attn);
+        if (h->d_attn_counts) cudaFree(h->d_attn_counts);
         if (h->attn_done) cudaEventDestroy(h->attn_done);
         if (h->d_opts) cudaFree(h->d_opts);
         if (h->h_opts) cudaFreeHost(h->h_opts);

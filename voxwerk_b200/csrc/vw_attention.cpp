@@ -87,31 +87,49 @@ cudaError_t leave_workspace(vw_handle* h, cudaStream_t st, bool capturing) {
     return cudaEventRecord(h->attn_done, st);
 }
 
-constexpr size_t kAttnHeader = 256;   // counters (zero between calls), units_per_cta
-
-// Room for a plan's partial results; the buffer grows outside captures only.
-vw_status tile_work(vw_handle* h, const vw::TilePlan& plan, cudaStream_t st, vw::TileWork* w) {
-    const size_t ends = round_up(static_cast<size_t>(plan.unit_ends) * 8, 256);
-    const size_t lse = round_up(static_cast<size_t>(plan.part_rows) * 4, 256);
-    const size_t need = kAttnHeader + ends + lse + static_cast<size_t>(plan.part_rows) * plan.dim * 4;
-    if (need > h->attn_bytes) {
-        cudaError_t e = cudaDeviceSynchronize();   // an earlier call, on any stream, may still use the old buffer
-        if (e == cudaSuccess && h->d_attn) e = cudaFree(h->d_attn);
-        h->d_attn = nullptr;
-        h->attn_bytes = 0;
-        const size_t bytes = round_up(need + need / 4, 1 << 20);
-        if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(&h->d_attn), bytes);
-        if (e == cudaSuccess) e = cudaMemsetAsync(h->d_attn, 0, kAttnHeader, st);
-        if (e != cudaSuccess) return cuda_fail(h, e, "attention workspace");
-        h->attn_bytes = bytes;
-    }
-    char* at = h->d_attn;
-    w->counters = reinterpret_cast<int32_t*>(at);
-    w->units_per_cta = reinterpret_cast<int64_t*>(at + 64);
-    w->unit_end = reinterpret_cast<int64_t*>(at + kAttnHeader);
-    w->part_lse = reinterpret_cast<float*>(at + kAttnHeader + ends);
-    w->part_o = reinterpret_cast<float*>(at + kAttnHeader + ends + lse);
+// Grows one of the two attention buffers (cleared: the one whose contents are zero between calls).
+vw_status reserve(vw_handle* h, char** buf, size_t* have, size_t need, bool clear, cudaStream_t st) {
+    if (need <= *have) return VW_OK;
+    cudaError_t e = cudaDeviceSynchronize();   // an earlier call, on any stream, may still use the old buffer
+    if (e == cudaSuccess && *buf) e = cudaFree(*buf);
+    *buf = nullptr;
+    *have = 0;
+    const size_t bytes = round_up(need + need / 4, 1 << 16);
+    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(buf), bytes);
+    if (e == cudaSuccess && clear) e = cudaMemsetAsync(*buf, 0, bytes, st);
+    if (e != cudaSuccess) return cuda_fail(h, e, "attention workspace");
+    *have = bytes;
     return VW_OK;
+}
+
+constexpr size_t kCountsHeader = 256;   // the tile kernel's counters, then the decode kernel's tickets
+
+vw_status reserve_counts(vw_handle* h, int64_t tickets, cudaStream_t st) {
+    return reserve(h, &h->d_attn_counts, &h->attn_counts_bytes, kCountsHeader + static_cast<size_t>(tickets) * 4, true, st);
+}
+// The parts buffer, carved twice: without a base for its size, then for the pointers.
+template <typename F>
+vw_status reserve_parts(vw_handle* h, cudaStream_t st, F carve) {
+    size_t size = 0;
+    const auto take = [&size](char* base, int64_t bytes) {
+        char* p = base ? base + size : nullptr;
+        size += round_up(static_cast<size_t>(bytes), 256);
+        return p;
+    };
+    carve([&](int64_t bytes) { return take(nullptr, bytes); });
+    const vw_status r = reserve(h, &h->d_attn, &h->attn_bytes, size, false, st);
+    if (r != VW_OK) return r;
+    size = 0;
+    carve([&](int64_t bytes) { return take(h->d_attn, bytes); });
+    return VW_OK;
+}
+template <typename Take>
+void carve_tiles(vw_handle* h, const vw::TilePlan& plan, Take take, vw::TileWork* w) {
+    w->counters = reinterpret_cast<int32_t*>(h->d_attn_counts);
+    w->units_per_cta = reinterpret_cast<int64_t*>(take(8));
+    w->unit_end = reinterpret_cast<int64_t*>(take(plan.unit_ends * 8));
+    w->part_lse = reinterpret_cast<float*>(take(plan.part_rows * 4));
+    w->part_o = reinterpret_cast<float*>(take(plan.part_rows * plan.dim * 4));
 }
 
 }  // namespace
@@ -201,7 +219,8 @@ VW_EXPORT vw_status vw_prompt_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (e != cudaSuccess) return cuda_fail(h, e, "prompt attention");
     const vw::TilePlan plan = vw::plan_prompt(p, h->sm_count);
     vw::TileWork w{};
-    r = tile_work(h, plan, st, &w);
+    r = reserve_counts(h, 0, st);
+    if (r == VW_OK) r = reserve_parts(h, st, [&](auto take) { carve_tiles(h, plan, take, &w); });
     if (r != VW_OK) return r;
     e = vw::launch_prompt_attention(p, plan, w, st);
     if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
@@ -236,7 +255,25 @@ VW_EXPORT vw_status vw_decode_attention(vw_handle* h, const vw_kv_cache* cache, 
         p.prefix = {prefix->page_table, prefix->page_table_stride, prefix->max_pages, prefix->n_groups, prefix->lens,
                     prefix->group_offsets};
     cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess) e = vw::launch_decode_attention(p, st);
+    bool capturing = false;
+    if (e == cudaSuccess) e = enter_workspace(h, st, &capturing);
+    if (e != cudaSuccess) return cuda_fail(h, e, "decode attention");
+    const vw::DecodePlan plan = vw::plan_decode(p, h->sm_count);
+    vw::TilePlan prefix_plan{};
+    if (p.prefix.n_groups > 0) prefix_plan = vw::plan_prefix(p, h->sm_count);
+    vw::DecodeWork w{};
+    r = reserve_counts(h, plan.items, st);
+    if (r == VW_OK)
+        r = reserve_parts(h, st, [&](auto take) {
+            w.tickets = reinterpret_cast<int32_t*>(h->d_attn_counts + kCountsHeader);
+            w.part_lse = reinterpret_cast<float*>(take(plan.part_rows * 4));
+            w.part_o = reinterpret_cast<float*>(take(plan.part_rows * plan.dim * 4));
+            if (p.prefix.n_groups > 0) carve_tiles(h, prefix_plan, take, &w.prefix);
+        });
+    if (r != VW_OK) return r;
+    if (p.prefix.n_groups > 0) e = vw::launch_prefix_attention(p, prefix_plan, w.prefix, st);
+    if (e == cudaSuccess) e = vw::launch_decode_attention(p, plan, w, st);
+    if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
     if (e != cudaSuccess) return cuda_fail(h, e, "decode attention");
     if (!stream) return read_device_error(h, st);
     return VW_OK;

@@ -8,6 +8,8 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include "vw_internal.h"
+
 namespace vw {
 
 struct KvCacheDev {             // vw_kv_cache
@@ -88,14 +90,47 @@ struct TileWork {
     float* part_lse;            // [part_rows] log2 of each partial row's sum, -inf: no key
     float* part_o;              // [part_rows, dim] its softmax-weighted values
 };
+constexpr int kTileKeys = 128, kTileRows = 128;
+struct Geometry {
+    int32_t group;              // query heads per key head
+    int32_t tile_tokens;        // tokens of a row tile; a block has two
+};
+inline Geometry geometry(const AttnParams& a) {
+    const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
+    return {group, kTileRows / group};
+}
+// scale as the kernels use it, for powers of two; 0 becomes a factor that leaves every probability the same
+inline float exp2_scale(float scale) {
+    const float c = (scale < 0.0f ? -scale : scale) * 1.44269504088896341f;
+    return c > 1e-30f ? c : 1e-30f;
+}
 TilePlan plan_prompt(const AttnParams& p, int sms);
+TilePlan plan_prefix(const AttnParams& p, int sms);
+cudaError_t launch_prefix_attention(const AttnParams& p, const TilePlan& plan, const TileWork& w, cudaStream_t stream);
 cudaError_t launch_prompt_attention(const AttnParams& p, const TilePlan& plan, const TileWork& w, cudaStream_t stream);
-cudaError_t launch_decode_attention(const AttnParams& p, cudaStream_t stream);
+
+// ---- the decode kernel (vw_decode.cu)
+struct DecodePlan {
+    int32_t grid;
+    int32_t rows;               // query heads an item takes: min(group, 16)
+    int32_t row_blocks;         // items per key head
+    int32_t dim;
+    int64_t items;              // sequences x key heads x row_blocks
+    int64_t part_rows;
+};
+struct DecodeWork {
+    int32_t* tickets;           // [items] pieces done, 0 between calls
+    float* part_lse;
+    float* part_o;
+    TileWork prefix;            // the prefixes' partial results
+};
+DecodePlan plan_decode(const AttnParams& p, int sms);
+cudaError_t launch_decode_attention(const AttnParams& p, const DecodePlan& plan, const DecodeWork& w, cudaStream_t stream);
 
 #ifdef __CUDACC__
 // A sequence's key count, held inside its page table; a count outside it is reported and clamped.
 __device__ __forceinline__ int checked_len(int len, int max_pages, int page_shift, unsigned* err, unsigned bit) {
-    const int cap = static_cast<int>(min(static_cast<int64_t>(max_pages) << page_shift, static_cast<int64_t>(INT32_MAX)));
+    const int cap = static_cast<int>(min(static_cast<int64_t>(max_pages) << page_shift, int64_t{1} << 30));
     if (len < 0 || len > cap) {
         atomicOr(err, bit);
         return len < 0 ? 0 : cap;
@@ -119,6 +154,96 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n_seqs,
     return lo;
 }
 
+// ---- the tile kernel's units: key tiles of blocks, in the order sequence, block, key head
+struct Seq {
+    int32_t row0, n, kv, past;   // first row, tokens, keys, keys before the first token's own
+};
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+template <bool kPrefix>
+__device__ __forceinline__ Seq load_seq(const AttnParams& a, int s) {
+    Seq q{0, 0, 0, 0};
+    const int shift = a.cache.page_shift;
+    const int32_t* o = kPrefix ? a.prefix.group_offsets : a.batch.q_offsets;
+    const int limit = kPrefix ? a.batch.n_seqs : a.batch.n_rows;
+    int begin = s, end = min(s + 1, limit);
+    if (o) {
+        begin = o[s];
+        end = o[s + 1];
+    }
+    q.kv = kPrefix ? checked_len(a.prefix.lens[s], a.prefix.max_pages, shift, a.err, kErrKvLens)
+                   : checked_len(a.batch.kv_lens[s], a.batch.max_pages, shift, a.err, kErrKvLens);
+    if (begin < 0 || end < begin || end > limit) {
+        atomicOr(a.err, kErrKvLens);
+        return q;
+    }
+    q.row0 = begin;
+    q.n = end - begin;
+    q.past = q.kv - q.n;
+    return q;
+}
+
+// Keys that tokens [.., t) of a sequence see together
+template <bool kPrefix>
+__device__ __forceinline__ int keys_seen(const Seq& q, int t) {
+    return kPrefix ? q.kv : min(max(q.past + min(q.n, t), 0), q.kv);
+}
+// Units of a sequence's block i (split): its key tiles, at least one for a prompt's block (its rows are written)
+template <bool kPrefix>
+__device__ __forceinline__ int block_units(const Seq& q, int i, int block_tokens) {
+    return max(ceil_div(keys_seen<kPrefix>(q, (i + 1) * block_tokens), kTileKeys), kPrefix ? 0 : 1);
+}
+template <bool kPrefix>
+__device__ __forceinline__ int64_t seq_units(const Seq& q, int block_tokens, int kv_heads) {
+    const int blocks = ceil_div(q.n, block_tokens);
+    int64_t u = 0;
+    if (kPrefix)
+        u = static_cast<int64_t>(blocks) * block_units<kPrefix>(q, 0, block_tokens);
+    else
+        for (int i = 0; i < blocks; ++i) u += block_units<kPrefix>(q, i, block_tokens);
+    return u * kv_heads;
+}
+
+__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusive
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+// Where the pieces of one row's block are: piece c (of CTA c) at partial row base + c * kPartRows, c0 <= c <= c1; c0 > c1
+// where the row has none.
+struct PieceSpan {
+    int64_t base;
+    int32_t c0, c1;
+};
+template <bool kPrefix>
+__device__ PieceSpan piece_span(const AttnParams& a, const TileWork& w, int s, int row, int head, int tile_tokens) {
+    PieceSpan at{0, 1, 0};
+    const Seq q = load_seq<kPrefix>(a, s);
+    if (row < q.row0 || row >= q.row0 + q.n) return at;
+    const int kv_heads = a.cache.n_kv_heads, heads = a.rows.n_q_heads, group = heads / kv_heads;
+    const int block_tokens = 2 * tile_tokens, i = (row - q.row0) / block_tokens, kv_head = head / group;
+    const int cost = block_units<kPrefix>(q, i, block_tokens);
+    if (cost == 0) return at;
+    int64_t first = s > 0 ? w.unit_end[s - 1] : 0;
+    if (kPrefix)
+        first += static_cast<int64_t>(i) * kv_heads * cost;
+    else
+        for (int j = 0; j < i; ++j) first += static_cast<int64_t>(kv_heads) * block_units<kPrefix>(q, j, block_tokens);
+    first += static_cast<int64_t>(kv_head) * cost;
+    const int64_t per = *w.units_per_cta;
+    at.c0 = static_cast<int>(first / per);
+    at.c1 = static_cast<int>((first + cost - 1) / per);
+    const int tokens = min(block_tokens, q.n - i * block_tokens);
+    at.base = static_cast<int64_t>(q.row0) * heads + static_cast<int64_t>(i) * kv_heads * block_tokens * group +
+              static_cast<int64_t>(kv_head) * tokens * group + (row - q.row0 - i * block_tokens) * group + head % group;
+    return at;
+}
+
 // A row's partial results weighed together by one warp, DIM / 32 dims a lane: o = sum_i 2^(lse_i - m) o_i / l,
 // l = sum_i 2^(lse_i - m).
 template <int DIM>
@@ -126,11 +251,11 @@ struct PartSum {
     static constexpr int kDims = DIM / 32;
     float m = -INFINITY, l = 0.0f, o[kDims] = {};
 
-    // pieces c0 .. c1 of the row whose piece c is at partial row base + c * kPartRows
-    __device__ void add(const TileWork& w, int64_t base, int c0, int c1, int lane) {
+    // pieces c0 .. c1, piece c at partial row base + c * stride
+    __device__ void add(const float* part_lse, const float* part_o, int64_t base, int stride, int c0, int c1, int lane) {
         for (int c = c0; c <= c1; c += 32) {
             const int n = min(32, c1 - c + 1);
-            const float lse = lane < n ? w.part_lse[base + static_cast<int64_t>(c + lane) * kPartRows] : -INFINITY;
+            const float lse = lane < n ? part_lse[base + static_cast<int64_t>(c + lane) * stride] : -INFINITY;
             float top = lse;
 #pragma unroll
             for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
@@ -139,7 +264,7 @@ struct PartSum {
 #pragma unroll 4
             for (int i = 0; i < n; ++i) {
                 const float f = __shfl_sync(0xffffffffu, mine, i);
-                const float* src = w.part_o + (base + static_cast<int64_t>(c + i) * kPartRows) * DIM + lane * kDims;
+                const float* src = part_o + (base + static_cast<int64_t>(c + i) * stride) * DIM + lane * kDims;
                 float x[kDims];
                 if constexpr (kDims == 4) {
                     const float4 v = *reinterpret_cast<const float4*>(src);

@@ -1,93 +1,520 @@
-// vw_decode.cu -- single-token attention over a paged key/value cache (include/vwsampler.h, vw_decode_attention): softmax(scale q k^T) v of each row over the keys it sees.
+// vw_decode.cu -- single-token attention over a paged key/value cache (include/vwsampler.h, vw_decode_attention).
 //
-// One warp per (row, query head), each lane four dims of the head, one pass over the keys with the running maximum m
-// and sum l of the softmax in fp32: o and l are scaled by exp(m - m') when the maximum rises to m'.
+// out = softmax(scale q K^T) v for one row per sequence, over its own keys here; the keys of a shared prefix are read
+// once for their whole group by the tile kernel (vw_prompt.cu), whose partial results are weighed in at the end.
+//
+// Bound: HBM (each key and value is read once, for the few query heads of its key head).  So the kernel is a stream: an
+// item is (sequence, key head, block of at most 16 of its query heads), its units are tiles of 64 keys, and all units
+// are dealt evenly to two CTAs per SM, whatever the sequences' lengths.  A CTA's producer warp loads its units' K and V
+// by TMA (a lane per page box) into a ring and runs ahead across items; four warps each take 16 keys of a tile:
+// S = Q K^T and O += P V by mma.sync m16n8k16 from shared memory (rows are the query heads; the tensor cores idle most
+// of the time either way, a tile of 32 KB takes an SM about 1400 cycles to fetch), with a running maximum and sum of
+// their own, raised only past 2^8.  At an item's end the four are joined in shared memory, a warp per row.  An item cut
+// by a CTA boundary leaves its pieces in the workspace, and the CTA that finishes last joins them in order.
+//
+// Every mbarrier wait is bounded.
 
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <cstdint>
 
 #include "vw_attention.h"
 #include "vw_internal.h"
+#include "vw_tc.cuh"
 
 namespace vw {
 namespace {
 
-struct Softmax {
-    float m = -INFINITY, l = 0.0f, o[4] = {};
+constexpr int kThreads = 160;     // producer warp, four warps of 16 keys
+constexpr int kKeys = 64;         // keys per tile
+constexpr int kMaxRows = 16;      // query heads per item: the rows of an mma
+constexpr int kItemSlots = 2;
+constexpr int kMinUnits = 2;      // fewest tiles a CTA takes
+constexpr uint32_t kSmemBudget = 113 * 1024;   // two CTAs per SM
+
+template <int DP>
+struct DecodeCfg {
+    static constexpr int kHalves = DP / 64;
+    static constexpr uint32_t kHalfBytes = kKeys * 128;
+    static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;   // K or V
+    static constexpr uint32_t kStageBytes = 2 * kTileBytes;
+    static constexpr uint32_t kQueryHalf = kMaxRows * 128;
+    static constexpr uint32_t kQueryBytes = kHalves * kQueryHalf;
+    static constexpr int kMaxStages = 6;
+    // barriers full[6] empty[6] item_full[2] item_empty[2], item slots, flags
+    static constexpr uint32_t kBarBytes = 8 * (2 * kMaxStages + 2 * kItemSlots);
+    static constexpr uint32_t kTail = kBarBytes + kItemSlots * 64 + 16;
+    // joining four warps: O of `rows` rows each, and (m, l)
+    __host__ __device__ static constexpr uint32_t scratch(int rows) { return 4 * rows * (DP * 4 + 8); }
+    static constexpr int stages(int rows) {
+        const uint32_t room = kSmemBudget - 1024 - kItemSlots * kQueryBytes - kTail - scratch(rows);
+        const int n = static_cast<int>(room / kStageBytes);
+        return n < kMaxStages ? n : kMaxStages;
+    }
+    static constexpr uint32_t bytes(int rows) {
+        return stages(rows) * kStageBytes + kItemSlots * kQueryBytes + kTail + scratch(rows) + 1024;
+    }
+};
+static_assert(DecodeCfg<128>::stages(16) >= 2 && DecodeCfg<64>::stages(16) >= 2, "ring");
+
+struct DecodeItem {
+    int32_t valid, seq, kv_head, row_block;
+    int32_t keys;            // of the sequence
+    int32_t tile0, tile1;    // this piece's tiles
+    int32_t c0, c1;          // CTAs that hold the item's pieces
+    int32_t index;           // of the item
+};
+static_assert(sizeof(DecodeItem) <= 64, "item slots");
+
+struct DecodeParams {
+    AttnParams a;
+    DecodePlan plan;
+    DecodeWork w;
+    int32_t group, tile_tokens, stages, negate, boxes, has_prefix;
+    float c;
 };
 
-__device__ void attend(const AttnParams& p, const int32_t* table, int keys, int kv_head, int d0, const float* q,
-                       Softmax& s) {
-    const KvCacheDev& c = p.cache;
-    for (int j = 0; j < keys; ++j) {
-        const int page = table[j >> c.page_shift];
-        if (static_cast<unsigned>(page) >= static_cast<unsigned>(c.n_pages)) {
-            atomicOr(p.err, kErrPageRange);
-            continue;
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// byte offset of 16-byte chunk `chunk` of row `row` in a tile of 128-byte rows with the TMA's 128-byte swizzle
+__device__ __forceinline__ uint32_t swizzled(int row, int chunk) { return row * 128 + ((chunk ^ (row & 7)) << 4); }
+__device__ __forceinline__ void sync_consumers() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+// the same, and whether any of the 128 threads has gone wrong: they leave together, so none waits for one that left
+__device__ __forceinline__ bool any_failed(bool ok) {
+    int r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.s32 p, %1, 0;\n\t"
+        "barrier.cta.red.or.pred q, 1, 128, p;\n\t"
+        "selp.s32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(ok ? 0 : 1)
+        : "memory");
+    return r != 0;
+}
+
+// One row's sums of one warp: m, l and O (not divided), as PartSum keeps them
+template <int DIM>
+__device__ __forceinline__ void add_raw(PartSum<DIM>& s, float m, float l, const float* o) {
+    s.raise(m);
+    const float f = s.m == -INFINITY ? 0.0f : exp2f(m - s.m);
+    s.l = __fmaf_rn(f, l, s.l);
+#pragma unroll
+    for (int d = 0; d < PartSum<DIM>::kDims; ++d) s.o[d] = __fmaf_rn(f, o[d], s.o[d]);
+}
+
+template <int DP>
+__global__ void __launch_bounds__(kThreads, 2)
+decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+              const __grid_constant__ CUtensorMap map_v, const __grid_constant__ DecodeParams p) {
+    using C = DecodeCfg<DP>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t sbase = s32(sm);
+    const int S = p.stages, rows = p.plan.rows;
+    const uint32_t off_q = S * C::kStageBytes, off_scratch = off_q + kItemSlots * C::kQueryBytes,
+                   off_bar = off_scratch + C::scratch(rows);
+    const uint32_t full = sbase + off_bar, empty = full + 8 * C::kMaxStages, item_full = empty + 8 * C::kMaxStages,
+                   item_empty = item_full + 8 * kItemSlots;
+    uint8_t* item_mem = sm + off_bar + C::kBarBytes;
+    auto item_slot = [&](uint32_t n) { return reinterpret_cast<DecodeItem*>(item_mem + 64 * (n % kItemSlots)); };
+    volatile int32_t* abort = reinterpret_cast<volatile int32_t*>(item_mem + 64 * kItemSlots);
+    volatile int32_t* last = abort + 1;
+    unsigned* err = p.a.err;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
+        for (int s = 0; s < S; ++s) {
+            init(full + 8 * s, 1);
+            init(empty + 8 * s, 4);
         }
-        const int64_t at = page * c.page_stride + (j & (c.page_size - 1)) * c.token_stride + kv_head * c.head_stride + d0;
-        float x = 0.0f;
-        if (d0 < c.head_dim)
-            for (int i = 0; i < 4; ++i) x = __fmaf_rn(q[i], __bfloat162float(c.k[at + i]), x);
-        for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        const float m = fmaxf(s.m, x);
-        const float w = expf(x - m), f = expf(s.m - m);
-        s.m = m;
-        s.l = __fmaf_rn(s.l, f, w);
-        if (d0 < c.head_dim)
-            for (int i = 0; i < 4; ++i) s.o[i] = __fmaf_rn(s.o[i], f, w * __bfloat162float(c.v[at + i]));
+        for (int s = 0; s < kItemSlots; ++s) {
+            init(item_full + 8 * s, 1);
+            init(item_empty + 8 * s, 4);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        *abort = 0;
+    }
+    __syncthreads();
+
+    if (warp == 0) {
+        // ---------------- units and loads
+        const AttnParams& a = p.a;
+        const KvCacheDev& cache = a.cache;
+        const int n_seqs = a.batch.n_seqs, shift = cache.page_shift;
+        const int per_seq = cache.n_kv_heads * p.plan.row_blocks;   // items of a sequence
+        auto keys_of = [&](int s) {
+            return checked_len(a.batch.kv_lens[s], a.batch.max_pages, shift, err, kErrKvLens);
+        };
+        auto tiles_of = [&](int keys) { return max((keys + kKeys - 1) / kKeys, 1); };   // an empty one is written too
+        int64_t total = 0;
+        for (int s = lane; s < n_seqs; s += 32) total += tiles_of(keys_of(s));
+        total = __shfl_sync(0xffffffffu, warp_scan(total, lane), 31) * per_seq;
+        const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kMinUnits));
+        int64_t unit = min(per * blockIdx.x, total);
+        const int64_t unit_end = min(unit + per, total);
+        int64_t first = 0;   // the first unit of sequence `seq`
+        int seq = 0;
+        for (int s0 = 0; unit < unit_end && s0 < n_seqs; s0 += 32) {
+            const int64_t u = s0 + lane < n_seqs ? static_cast<int64_t>(tiles_of(keys_of(s0 + lane))) * per_seq : 0;
+            const int64_t sum = warp_scan(u, lane);
+            const unsigned m = __ballot_sync(0xffffffffu, first + sum > unit);
+            if (m) {
+                const int at = __ffs(m) - 1;
+                seq = s0 + at;
+                first += __shfl_sync(0xffffffffu, sum - u, at);
+                break;
+            }
+            first += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        const int box_rows = min(cache.page_size, kKeys);
+        // a lane's box of a tile: page box, keys or values, half of the head
+        const int box = lane / (2 * C::kHalves), is_v = (lane / C::kHalves) & 1, half = lane % C::kHalves;
+        uint32_t n_items = 0, st = 0;
+        bool stop = false;
+        while (!stop) {
+            DecodeItem it;
+            it.valid = unit < unit_end;
+            if (it.valid) {
+                int keys = keys_of(seq), tiles = tiles_of(keys);
+                while (unit >= first + static_cast<int64_t>(tiles) * per_seq) {
+                    first += static_cast<int64_t>(tiles) * per_seq;
+                    keys = keys_of(++seq);
+                    tiles = tiles_of(keys);
+                }
+                const int j = static_cast<int>((unit - first) / tiles);
+                const int64_t item_first = first + static_cast<int64_t>(j) * tiles;
+                it.seq = seq;
+                it.kv_head = j / p.plan.row_blocks;
+                it.row_block = j % p.plan.row_blocks;
+                it.keys = keys;
+                it.tile0 = static_cast<int>(unit - item_first);
+                it.tile1 = static_cast<int>(min(unit_end - item_first, static_cast<int64_t>(tiles)));
+                it.c0 = static_cast<int>(item_first / per);
+                it.c1 = static_cast<int>((item_first + tiles - 1) / per);
+                it.index = seq * per_seq + j;
+                unit = item_first + it.tile1;
+            }
+            const uint32_t slot = n_items % kItemSlots;
+            if (n_items >= kItemSlots && !wait_bounded(item_empty + 8 * slot, (n_items / kItemSlots - 1) & 1, abort, err))
+                stop = true;
+            if (__any_sync(0xffffffffu, stop)) break;
+            if (lane == 0) {
+                *item_slot(n_items) = it;
+                if (it.valid) {
+                    const uint32_t dst = sbase + off_q + slot * C::kQueryBytes;
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(item_full + 8 * slot),
+                                 "r"(C::kHalves * rows * 128)
+                                 : "memory");
+                    for (int h = 0; h < C::kHalves; ++h)
+                        tma_load_3d(dst + h * C::kQueryHalf, &map_q, 64 * h, it.kv_head * p.group + it.row_block * kMaxRows,
+                                    it.seq, item_full + 8 * slot);
+                } else {
+                    arrive(item_full + 8 * slot);
+                }
+            }
+            __syncwarp();
+            ++n_items;
+            if (!it.valid) break;
+            const int32_t* table = a.batch.page_table + it.seq * a.batch.page_table_stride;
+            auto page_of = [&](int t) {
+                const int key = t * kKeys + box * box_rows;
+                if (box >= p.boxes || key >= it.keys || t >= it.tile1) return -1;
+                const int page = table[key >> shift];
+                if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.n_pages)) {
+                    atomicOr(err, kErrPageRange);
+                    return cache.n_pages;   // past the map's end: zeros
+                }
+                return page;
+            };
+            int page = page_of(it.tile0);
+            for (int t = it.tile0; t < it.tile1; ++t, ++st) {
+                const int next = page_of(t + 1);
+                const uint32_t s = st % S;
+                if (st >= static_cast<uint32_t>(S) && !wait_bounded(empty + 8 * s, (st / S - 1) & 1, abort, err)) stop = true;
+                if (__any_sync(0xffffffffu, stop)) {
+                    stop = true;
+                    break;
+                }
+                const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * box_rows * 128;
+                if (lane == 0)
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full + 8 * s), "r"(bytes)
+                                 : "memory");
+                __syncwarp();
+                if (page >= 0)
+                    tma_load_4d(sbase + s * C::kStageBytes + is_v * C::kTileBytes + half * C::kHalfBytes +
+                                    box * box_rows * 128,
+                                is_v ? &map_v : &map_k, 64 * half, (t * kKeys) & (cache.page_size - 1), it.kv_head, page,
+                                full + 8 * s);
+                page = next;
+            }
+        }
+        // teardown: the copies in flight land before the CTA may exit
+        if (lane == 0) {
+            for (uint32_t j = st > static_cast<uint32_t>(S) ? st - S : 0; j < st; ++j) drain_wait(full + 8 * (j % S), (j / S) & 1);
+            for (uint32_t j = n_items > kItemSlots ? n_items - kItemSlots : 0; j < n_items; ++j)
+                drain_wait(item_full + 8 * (j % kItemSlots), (j / kItemSlots) & 1);
+        }
+        __syncwarp();
+        return;
+    }
+
+    // ---------------- attention: warp w takes keys [16 w, 16 w + 16) of each tile
+    const int w = warp - 1, key0 = 16 * w;
+    const bool upper = rows > 8;   // rows 8-15 of the mma hold query heads
+    float* scratch_o = reinterpret_cast<float*>(sm + off_scratch);                 // [4][rows][DP]
+    float2* scratch_ml = reinterpret_cast<float2*>(scratch_o + 4 * rows * DP);     // [4][rows]
+    uint32_t st = 0;
+    bool waited = false;
+    for (uint32_t n = 0;; ++n) {
+        const uint32_t slot = n % kItemSlots;
+        bool ok = wait_bounded(item_full + 8 * slot, (n / kItemSlots) & 1, abort, err);
+        if (any_failed(ok)) break;
+        const DecodeItem it = *item_slot(n);
+        if (!it.valid) break;
+        uint32_t qf[DP / 16][4];
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+            ldmatrix4(sbase + off_q + slot * C::kQueryBytes + (k >> 2) * C::kQueryHalf +
+                          swizzled(((lane >> 3) & 1) * 8 + (lane & 7), 2 * (k & 3) + (lane >> 4)),
+                      qf[k]);
+        __syncwarp();
+        if (lane == 0) arrive(item_empty + 8 * slot);
+
+        float o[DP / 8][4];
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // rows lane / 4 and lane / 4 + 8
+        for (int t = it.tile0; t < it.tile1; ++t, ++st) {
+            const uint32_t s = st % S;
+            ok = wait_bounded(full + 8 * s, (st / S) & 1, abort, err);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            const int valid = it.keys - t * kKeys - key0;   // of this warp's 16 keys
+            if (valid > 0) {
+                const uint32_t k_base = sbase + s * C::kStageBytes, v_base = k_base + C::kTileBytes;
+                if (valid < 16) {   // what lies past the last key may be anything: 0 * NaN would reach the sums
+                    for (int i = lane; i < (16 - valid) * 8 * C::kHalves; i += 32) {
+                        const int h = i / ((16 - valid) * 8), r = i % ((16 - valid) * 8);
+                        *reinterpret_cast<uint4*>(sm + (v_base - sbase) + h * C::kHalfBytes + (key0 + valid) * 128 + 16 * r) =
+                            make_uint4(0, 0, 0, 0);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before the ring's next copy there
+                    __syncwarp();
+                }
+                float sc[2][4] = {};
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k) {
+                    uint32_t kf[4];
+                    ldmatrix4(k_base + (k >> 2) * C::kHalfBytes +
+                                  swizzled(key0 + (lane >> 4) * 8 + (lane & 7), 2 * (k & 3) + ((lane >> 3) & 1)),
+                              kf);
+                    mma_16x8x16(sc[0], qf[k], kf[0], kf[1]);
+                    mma_16x8x16(sc[1], qf[k], kf[2], kf[3]);
+                }
+                uint32_t pf[4];   // P as the next product's left operand: [row half + 2 * key half]
+                float f[2] = {1.0f, 1.0f};
+                bool rise = false;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    if (h == 1 && !upper) {
+                        pf[1] = pf[3] = 0;
+                        break;
+                    }
+                    float x[4] = {sc[0][2 * h], sc[0][2 * h + 1], sc[1][2 * h], sc[1][2 * h + 1]};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (p.negate) x[i] = -x[i];
+                        const int key = 2 * (lane & 3) + (i & 1) + 8 * (i >> 1);
+                        if (key >= valid) x[i] = -INFINITY;
+                    }
+                    float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    if (m[h] == -INFINITY) {
+                        m[h] = top;
+                    } else if ((top - m[h]) * p.c > 8.0f) {
+                        f[h] = exp2_fast((m[h] - top) * p.c);
+                        m[h] = top;
+                        rise = true;
+                    }
+                    const float mc = m[h] == -INFINITY ? 0.0f : m[h] * p.c;
+                    float e[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) e[i] = exp2_fast(__fmaf_rn(x[i], p.c, -mc));
+                    l[h] = __fmaf_rn(l[h], f[h], (e[0] + e[1]) + (e[2] + e[3]));
+                    pf[h] = pack_bf16(e[0], e[1]);
+                    pf[2 + h] = pack_bf16(e[2], e[3]);
+                }
+                if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+                    for (int i = 0; i < DP / 8; ++i) {
+                        o[i][0] *= f[0];
+                        o[i][1] *= f[0];
+                        o[i][2] *= f[1];
+                        o[i][3] *= f[1];
+                    }
+                }
+#pragma unroll
+                for (int d = 0; d < DP / 16; ++d) {
+                    uint32_t vf[4];
+                    ldmatrix4_t(v_base + (d >> 2) * C::kHalfBytes +
+                                    swizzled(key0 + ((lane >> 3) & 1) * 8 + (lane & 7), 2 * (d & 3) + (lane >> 4)),
+                                vf);
+                    mma_16x8x16(o[2 * d], pf, vf[0], vf[1]);
+                    mma_16x8x16(o[2 * d + 1], pf, vf[2], vf[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) arrive(empty + 8 * s);
+        }
+
+        // ---- the four warps' sums to shared memory, then a warp per row
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int r = (lane >> 2) + 8 * h;
+            float sum = l[h];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (r < rows) {
+                float* dst = scratch_o + (w * rows + r) * DP + 2 * (lane & 3);
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i) *reinterpret_cast<float2*>(dst + 8 * i) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+                if ((lane & 3) == 0) scratch_ml[w * rows + r] = make_float2(m[h] == -INFINITY ? m[h] : m[h] * p.c, sum);
+            }
+        }
+        if (any_failed(ok)) break;
+        const int live_rows = min(rows, p.group - it.row_block * kMaxRows);
+        const bool pieces = it.c0 != it.c1;
+        const int head0 = it.kv_head * p.group + it.row_block * kMaxRows;
+        int group = -1;
+        if (p.has_prefix) {   // the prefixes' partial results are written
+            if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+            waited = true;
+            group = find_sequence(p.a.prefix.group_offsets, p.a.prefix.n_groups, it.seq, lane);
+        }
+        auto finish = [&](PartSum<DP>& sum, int r) {
+            if (group >= 0) {
+                const PieceSpan at = piece_span<true>(p.a, p.w.prefix, group, it.seq, head0 + r, p.tile_tokens);
+                if (at.c0 <= at.c1)
+                    sum.add(p.w.prefix.part_lse, p.w.prefix.part_o, at.base, kPartRows, at.c0, at.c1, lane);
+            }
+            sum.write(p.a, it.seq, head0 + r, lane);
+        };
+        const int64_t part0 = static_cast<int64_t>(it.index) * rows;   // piece c at + c * rows
+        for (int r = w; r < live_rows; r += 4) {
+            PartSum<DP> sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 ml = scratch_ml[i * rows + r];
+                float x[PartSum<DP>::kDims];
+#pragma unroll
+                for (int d = 0; d < PartSum<DP>::kDims; ++d) x[d] = scratch_o[(i * rows + r) * DP + lane * PartSum<DP>::kDims + d];
+                add_raw(sum, ml.x, ml.y, x);
+            }
+            if (!pieces) {
+                finish(sum, r);
+            } else {
+                const int64_t at = part0 + static_cast<int64_t>(blockIdx.x) * rows + r;
+                const float inv = sum.l == 0.0f ? 0.0f : 1.0f / sum.l;
+#pragma unroll
+                for (int d = 0; d < PartSum<DP>::kDims; ++d) p.w.part_o[at * DP + lane * PartSum<DP>::kDims + d] = sum.o[d] * inv;
+                if (lane == 0) p.w.part_lse[at] = sum.m + log2f(sum.l);
+            }
+        }
+        if (pieces) {   // the CTA that comes last joins them
+            __threadfence();
+            sync_consumers();
+            if (threadIdx.x == 32) {
+                const int before = atomicAdd(p.w.tickets + it.index, 1);
+                *last = before == it.c1 - it.c0;
+                if (*last) p.w.tickets[it.index] = 0;
+                __threadfence();
+            }
+            sync_consumers();
+            if (*last)
+                for (int r = w; r < live_rows; r += 4) {
+                    PartSum<DP> sum;
+                    sum.add(p.w.part_lse, p.w.part_o, part0 + r, rows, it.c0, it.c1, lane);
+                    finish(sum, r);
+                }
+        }
+        sync_consumers();   // the scratch may be written again
     }
 }
 
-__global__ void __launch_bounds__(128) attention_kernel(const AttnParams p, int decode) {
-    const int lane = threadIdx.x & 31, d0 = 4 * lane;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int heads = p.rows.n_q_heads, D = p.cache.head_dim;
-    const int64_t row = item / heads;
-    if (item == 0 && lane == 0) {   // the offsets ascend within the rows
-        const int32_t* o = decode ? p.prefix.group_offsets : p.batch.q_offsets;
-        const int n = decode ? p.prefix.n_groups : p.batch.n_seqs, end = decode ? p.batch.n_seqs : p.batch.n_rows;
-        for (int i = 0; o && i < n; ++i)
-            if (o[i] < 0 || o[i + 1] < o[i] || o[i + 1] > end) atomicOr(p.err, kErrKvLens);
+template <int DP>
+cudaError_t launch_dim(DecodeParams& p, cudaStream_t stream) {
+    CUtensorMap q, k, v;
+    if (!make_row_map(&q, p.a, 1, p.plan.rows) || !make_cache_map(&k, p.a.cache, p.a.cache.k, kKeys) ||
+        !make_cache_map(&v, p.a.cache, p.a.cache.v, kKeys))
+        return cudaErrorInvalidValue;
+    p.stages = DecodeCfg<DP>::stages(p.plan.rows);
+    const size_t smem = DecodeCfg<DP>::bytes(p.plan.rows);
+    static std::atomic<uint64_t> attr_set{0};   // one bit per device ordinal whose attribute is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = 1ull << (dev & 63);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        e = cudaFuncSetAttribute(decode_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBudget);
+        if (e != cudaSuccess) return e;
+        attr_set.fetch_or(bit, std::memory_order_acq_rel);
     }
-    const int head = static_cast<int>(item % heads);
-    if (row >= p.batch.n_rows) return;
-    const KvBatchDev& b = p.batch;
-    int seq = static_cast<int>(row), behind = 0;
-    if (b.q_offsets) {
-        for (seq = 0; seq < b.n_seqs && row >= b.q_offsets[seq + 1]; ++seq) {}
-        if (seq < b.n_seqs) behind = max(0, b.q_offsets[seq + 1] - 1 - static_cast<int>(row));
-    }
-    if (seq >= b.n_seqs) return;
-    const int keys = checked_len(b.kv_lens[seq], b.max_pages, p.cache.page_shift, p.err, kErrKvLens) - behind;
-    const int kv_head = head / (heads / p.cache.n_kv_heads);
-    float q[4] = {};
-    if (d0 < D)
-        for (int i = 0; i < 4; ++i)
-            q[i] = __bfloat162float(p.rows.q[row * p.rows.q_row + head * p.rows.q_head + d0 + i]) * p.rows.scale;
-    Softmax s;
-    for (int g = 0; decode && g < p.prefix.n_groups; ++g)
-        if (seq >= p.prefix.group_offsets[g] && seq < p.prefix.group_offsets[g + 1])
-            attend(p, p.prefix.page_table + g * p.prefix.page_table_stride,
-                   checked_len(p.prefix.lens[g], p.prefix.max_pages, p.cache.page_shift, p.err, kErrKvLens), kv_head, d0,
-                   q, s);
-    attend(p, b.page_table + seq * b.page_table_stride, keys, kv_head, d0, q, s);
-    const float r = s.l > 0.0f ? 1.0f / s.l : 0.0f;
-    if (d0 < D)
-        for (int i = 0; i < 4; ++i)
-            p.rows.out[row * p.rows.out_row + head * p.rows.out_head + d0 + i] = __float2bfloat16_rn(s.o[i] * r);
-    if (p.rows.lse && lane == 0) p.rows.lse[row * heads + head] = s.m + logf(s.l);
-}
-
-cudaError_t launch(const AttnParams& p, int decode, cudaStream_t stream) {
-    const int64_t items = static_cast<int64_t>(p.batch.n_rows) * p.rows.n_q_heads;
-    attention_kernel<<<static_cast<unsigned>((items + 3) / 4), 128, 0, stream>>>(p, decode);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.plan.grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // starts as the prefix kernel drains
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.has_prefix ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, decode_kernel<DP>, q, k, v, p);
 }
 
 }  // namespace
 
-cudaError_t launch_decode_attention(const AttnParams& p, cudaStream_t stream) { return launch(p, 1, stream); }
+DecodePlan plan_decode(const AttnParams& a, int sms) {
+    const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
+    DecodePlan plan{};
+    plan.rows = std::min(group, kMaxRows);
+    plan.row_blocks = (group + kMaxRows - 1) / kMaxRows;
+    plan.dim = a.cache.head_dim <= 64 ? 64 : 128;
+    plan.items = static_cast<int64_t>(a.batch.n_seqs) * a.cache.n_kv_heads * plan.row_blocks;
+    const int64_t tiles = (static_cast<int64_t>(a.batch.max_pages) * a.cache.page_size + kKeys - 1) / kKeys;
+    plan.grid = static_cast<int>(std::min<int64_t>((plan.items * tiles + kMinUnits - 1) / kMinUnits, 2 * sms));
+    plan.part_rows = (plan.items + plan.grid) * plan.rows;
+    return plan;
+}
+
+cudaError_t launch_decode_attention(const AttnParams& a, const DecodePlan& plan, const DecodeWork& w, cudaStream_t stream) {
+    const Geometry g = geometry(a);
+    DecodeParams p{a, plan, w, g.group, g.tile_tokens, 0, a.rows.scale < 0.0f,
+                   a.cache.page_size >= kKeys ? 1 : kKeys / a.cache.page_size, a.prefix.n_groups > 0,
+                   exp2_scale(a.rows.scale)};
+    return plan.dim == 64 ? launch_dim<64>(p, stream) : launch_dim<128>(p, stream);
+}
 
 }  // namespace vw

@@ -41,8 +41,10 @@ struct vw_handle {
     int force_exact = 0;                     // VW_FORCE_EXACT at creation
     int test_stall_row = -1;                 // VW_TEST_STALL_ROW at creation (first vw_sample call only)
     unsigned long long h2d_bytes = 0;        // host -> device input bytes of VW_MEM_HOST calls (vw_stats.h2d_bytes)
-    char* d_attn = nullptr;                  // attention workspace: counters, then partial results (vw_attention.cpp)
+    char* d_attn = nullptr;                  // attention: partial results (vw_attention.cpp)
     size_t attn_bytes = 0;
+    char* d_attn_counts = nullptr;           // attention: counters and tickets, zero between calls
+    size_t attn_counts_bytes = 0;
     cudaStream_t attn_stream = nullptr;      // the stream of the last call that used it, and its end on that stream
     cudaEvent_t attn_done = nullptr;
     std::vector<vw_batch*> batches;          // live batches created on this handle (released by vw_destroy)

@@ -38,10 +38,10 @@ namespace vw {
 namespace {
 
 constexpr int kThreads384 = 384;
-constexpr int kKeys = 128;        // keys per tile
-constexpr int kRows = 128;        // rows per row tile
+constexpr int kKeys = kTileKeys;  // keys per tile
+constexpr int kRows = kTileRows;  // rows per row tile
 constexpr int kWholeKeys = 512;   // sequences of at most this many keys are never split
-constexpr int kMinPromptUnits = 2;
+constexpr int kMinPromptUnits = 2, kMinPrefixUnits = 1;   // fewest units a CTA takes
 constexpr int kFeedRegs = 96, kSoftmaxRegs = 200;   // registers per thread of warps 0-3 and 4-11
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr int kItemSlots = 3;
@@ -83,66 +83,6 @@ struct TileParams {
     int32_t negate;              // scale < 0
     TileWork w;
 };
-
-struct Seq {
-    int32_t row0, n, kv, past;   // first row, tokens, keys, keys before the first token's own
-};
-
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
-template <bool kPrefix>
-__device__ Seq load_seq(const TileParams& p, int s) {
-    Seq q{0, 0, 0, 0};
-    const AttnParams& a = p.a;
-    const int shift = a.cache.page_shift;
-    const int32_t* o = kPrefix ? a.prefix.group_offsets : a.batch.q_offsets;
-    const int limit = kPrefix ? a.batch.n_seqs : a.batch.n_rows;
-    int begin = s, end = min(s + 1, limit);
-    if (o) {
-        begin = o[s];
-        end = o[s + 1];
-    }
-    q.kv = kPrefix ? checked_len(a.prefix.lens[s], a.prefix.max_pages, shift, a.err, kErrKvLens)
-                   : checked_len(a.batch.kv_lens[s], a.batch.max_pages, shift, a.err, kErrKvLens);
-    if (begin < 0 || end < begin || end > limit) {
-        atomicOr(a.err, kErrKvLens);
-        return q;
-    }
-    q.row0 = begin;
-    q.n = end - begin;
-    q.past = q.kv - q.n;
-    return q;
-}
-
-// Keys that tokens [.., t) of a sequence see together
-template <bool kPrefix>
-__device__ __forceinline__ int keys_seen(const Seq& q, int t) {
-    return kPrefix ? q.kv : min(max(q.past + min(q.n, t), 0), q.kv);
-}
-// Units of a sequence's block i (split): its key tiles, at least one for a prompt's block (its rows are written)
-template <bool kPrefix>
-__device__ __forceinline__ int block_units(const Seq& q, int i, int block_tokens) {
-    return max(ceil_div(keys_seen<kPrefix>(q, (i + 1) * block_tokens), kKeys), kPrefix ? 0 : 1);
-}
-template <bool kPrefix>
-__device__ int64_t seq_units(const Seq& q, int block_tokens, int kv_heads) {
-    const int blocks = ceil_div(q.n, block_tokens);
-    int64_t u = 0;
-    if (kPrefix)
-        u = static_cast<int64_t>(blocks) * block_units<kPrefix>(q, 0, block_tokens);
-    else
-        for (int i = 0; i < blocks; ++i) u += block_units<kPrefix>(q, i, block_tokens);
-    return u * kv_heads;
-}
-
-__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusive
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    return x;
-}
 
 // The whole warp fills an item from block i of sequence s, key tiles [t0, t1) of it.
 template <bool kPrefix>
@@ -191,7 +131,7 @@ struct Scheduler {
             int64_t total = 0;
             for (int s0 = 0; s0 < n_seqs; s0 += 32) {
                 const int s = s0 + lane;
-                int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p, s), block_tokens, kv_heads) : 0;
+                int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p.a, s), block_tokens, kv_heads) : 0;
                 u = warp_scan(u, lane);
                 if (blockIdx.x == 0 && s < n_seqs) p.w.unit_end[s] = total + u;   // for the kernels that join
                 total += __shfl_sync(0xffffffffu, u, 31);
@@ -205,7 +145,7 @@ struct Scheduler {
             if (unit < unit_end) {   // the sequence that holds `unit`
                 for (int s0 = 0; s0 < n_seqs; s0 += 32) {
                     const int s = s0 + lane;
-                    const int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p, s), block_tokens, kv_heads) : 0;
+                    const int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p.a, s), block_tokens, kv_heads) : 0;
                     const int64_t sum = warp_scan(u, lane);
                     const unsigned m = __ballot_sync(0xffffffffu, seq_first + sum > unit);
                     if (m) {
@@ -221,7 +161,7 @@ struct Scheduler {
             ticket = blockIdx.x;
             int top = -1;
             for (int s = lane; s < n_seqs; s += 32) {
-                const Seq q = load_seq<kPrefix>(p, s);
+                const Seq q = load_seq<kPrefix>(p.a, s);
                 if (q.n > 0) top = max(top, first_level(q) + ceil_div(q.n, block_tokens) - 1);
             }
             level = __reduce_max_sync(0xffffffffu, top);
@@ -241,7 +181,7 @@ struct Scheduler {
             Seq q{0, 0, 0, 0};
             int i = -1;
             if (s < n_seqs) {
-                q = load_seq<kPrefix>(p, s);
+                q = load_seq<kPrefix>(p.a, s);
                 i = level - first_level(q);
                 if (q.n <= 0 || i >= ceil_div(q.n, block_tokens)) i = -1;
             }
@@ -270,11 +210,11 @@ struct Scheduler {
     }
 
     __device__ Item next_piece() {
-        Seq q = load_seq<kPrefix>(p, seq);   // every lane the same
+        Seq q = load_seq<kPrefix>(p.a, seq);   // every lane the same
         int64_t units = seq_units<kPrefix>(q, block_tokens, kv_heads);
         while (unit >= seq_first + units) {   // on to the sequence that holds `unit`
             seq_first += units;
-            q = load_seq<kPrefix>(p, ++seq);
+            q = load_seq<kPrefix>(p.a, ++seq);
             units = seq_units<kPrefix>(q, block_tokens, kv_heads);
         }
         int64_t first = seq_first;
@@ -304,25 +244,6 @@ struct Scheduler {
 __device__ __forceinline__ uint64_t value_desc(uint32_t saddr) {
     return static_cast<uint64_t>((saddr >> 4) & 0x3fffu) | (static_cast<uint64_t>((128 * 128) >> 4) << 16) |
            (64ull << 32) | (1ull << 46) | (2ull << 61);
-}
-
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
-            "r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
-                                            uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
-        "[%6];" ::"r"(dst),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 __device__ __forceinline__ void tmem_load32(uint32_t addr, float* f) {
@@ -361,11 +282,6 @@ __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-__device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22; -inf gives 0
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 // two fp32 operations per instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
@@ -385,12 +301,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 template <int DP, bool kPrefix>
 __global__ void __launch_bounds__(kThreads384, 1)
 attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -411,6 +321,8 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     unsigned* err = p.a.err;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    // the decode kernel that follows the prefixes' may take the SMs as they come free (it waits before it reads here)
+    if (kPrefix) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
         for (int s = 0; s < 2 * S; ++s) init(kv_full + 8 * s, 1);
@@ -821,67 +733,25 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 template <int DP>
 __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileParams p) {
     const int lane = threadIdx.x & 31;
-    const int heads = p.a.rows.n_q_heads, kv_heads = p.a.cache.n_kv_heads;
+    const int heads = p.a.rows.n_q_heads;
     const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
     const int row = static_cast<int>(item / heads), head = static_cast<int>(item % heads);
     if (row >= p.a.batch.n_rows) return;
     const int s = p.a.batch.q_offsets ? find_sequence(p.a.batch.q_offsets, p.a.batch.n_seqs, row, lane) : row;
     if (s < 0 || s >= p.a.batch.n_seqs) return;
-    const Seq q = load_seq<false>(p, s);
-    if (row < q.row0 || row >= q.row0 + q.n) return;
-    const int block_tokens = 2 * p.tile_tokens, i = (row - q.row0) / block_tokens, kv_head = head / p.group;
-    int64_t first = s > 0 ? p.w.unit_end[s - 1] : 0;
-    for (int j = 0; j < i; ++j) first += static_cast<int64_t>(kv_heads) * block_units<false>(q, j, block_tokens);
-    const int cost = block_units<false>(q, i, block_tokens);
-    first += static_cast<int64_t>(kv_head) * cost;
-    const int64_t per = *p.w.units_per_cta;
-    const int c0 = static_cast<int>(first / per), c1 = static_cast<int>((first + cost - 1) / per);
-    if (c0 == c1) return;   // whole: written by the tile kernel
-    const int tokens = min(block_tokens, q.n - i * block_tokens);
-    const int64_t part = static_cast<int64_t>(q.row0) * heads + static_cast<int64_t>(i) * kv_heads * block_tokens * p.group +
-                         static_cast<int64_t>(kv_head) * tokens * p.group +
-                         (row - q.row0 - i * block_tokens) * p.group + head % p.group;
+    const PieceSpan at = piece_span<false>(p.a, p.w, s, row, head, p.tile_tokens);
+    if (at.c0 >= at.c1) return;   // whole (written by the tile kernel), or no row of the sequence
     PartSum<DP> sum;
-    sum.add(p.w, part, c0, c1, lane);
+    sum.add(p.w.part_lse, p.w.part_o, at.base, kPartRows, at.c0, at.c1, lane);
     sum.write(p.a, row, head, lane);
-}
-
-struct Geometry {
-    int group, tile_tokens;
-};
-Geometry geometry(const AttnParams& a) {
-    const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
-    return {group, kRows / group};
-}
-
-bool make_maps(const AttnParams& a, const Geometry& g, CUtensorMap* q, CUtensorMap* k, CUtensorMap* v) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    const cuuint32_t ones[4] = {1, 1, 1, 1};
-    const cuuint64_t D = a.cache.head_dim;
-    const cuuint64_t q_dims[3] = {D, static_cast<cuuint64_t>(a.rows.n_q_heads), static_cast<cuuint64_t>(a.batch.n_rows)};
-    const cuuint64_t q_strides[2] = {static_cast<cuuint64_t>(a.rows.q_head) * 2, static_cast<cuuint64_t>(a.rows.q_row) * 2};
-    const cuuint32_t q_box[3] = {64, static_cast<cuuint32_t>(g.group), static_cast<cuuint32_t>(g.tile_tokens)};
-    const cuuint64_t c_dims[4] = {D, static_cast<cuuint64_t>(a.cache.page_size), static_cast<cuuint64_t>(a.cache.n_kv_heads),
-                                  static_cast<cuuint64_t>(a.cache.n_pages)};
-    const cuuint64_t c_strides[3] = {static_cast<cuuint64_t>(a.cache.token_stride) * 2,
-                                     static_cast<cuuint64_t>(a.cache.head_stride) * 2,
-                                     static_cast<cuuint64_t>(a.cache.page_stride) * 2};
-    const cuuint32_t c_box[4] = {64, static_cast<cuuint32_t>(std::min(a.cache.page_size, kKeys)), 1, 1};
-    auto encode = [&](CUtensorMap* m, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides,
-                      const cuuint32_t* box) {
-        return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, rank, const_cast<void*>(base), dims, strides, box, ones,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-    };
-    return encode(q, 3, a.rows.q, q_dims, q_strides, q_box) && encode(k, 4, a.cache.k, c_dims, c_strides, c_box) &&
-           encode(v, 4, a.cache.v, c_dims, c_strides, c_box);
 }
 
 template <int DP, bool kPrefix>
 cudaError_t launch_tiles(const TileParams& p, const Geometry& g, int grid, cudaStream_t stream) {
     CUtensorMap q, k, v;
-    if (!make_maps(p.a, g, &q, &k, &v)) return cudaErrorInvalidValue;
+    if (!make_row_map(&q, p.a, g.tile_tokens) || !make_cache_map(&k, p.a.cache, p.a.cache.k, kKeys) ||
+        !make_cache_map(&v, p.a.cache, p.a.cache.v, kKeys))
+        return cudaErrorInvalidValue;
     const int smem = static_cast<int>(TileCfg<DP>::kBytes) + 1024;
     static std::atomic<uint64_t> attr_set{0};   // one bit per device ordinal whose attribute is set
     int dev = 0;
@@ -901,12 +771,6 @@ cudaError_t launch_tiles(const TileParams& p, const Geometry& g, int grid, cudaS
     }
     attention_tile_kernel<DP, kPrefix><<<grid, kThreads384, smem, stream>>>(q, k, v, p);
     return cudaGetLastError();
-}
-
-// scale as the kernels use it; 0 becomes a factor that leaves every probability the same
-void set_scale(TileParams& p) {
-    p.negate = p.a.rows.scale < 0.0f;
-    p.c = std::max(std::fabs(p.a.rows.scale) * 1.44269504088896341f, 1e-30f);
 }
 
 }  // namespace
@@ -930,10 +794,26 @@ TilePlan plan_prompt(const AttnParams& a, int sms) {
     return plan;
 }
 
+// The prefixes: their units are dealt evenly whatever their number; every piece leaves a partial result.
+TilePlan plan_prefix(const AttnParams& a, int sms) {
+    TilePlan plan{};
+    plan.split = 1;
+    plan.grid = sms;
+    plan.part_rows = static_cast<int64_t>(a.batch.n_seqs) * a.rows.n_q_heads + kPartRows * plan.grid;
+    plan.unit_ends = a.prefix.n_groups;
+    plan.dim = a.cache.head_dim <= 64 ? 64 : 128;
+    return plan;
+}
+
+cudaError_t launch_prefix_attention(const AttnParams& a, const TilePlan& plan, const TileWork& w, cudaStream_t stream) {
+    const Geometry g = geometry(a);
+    TileParams p{a, g.group, g.tile_tokens, 1, kMinPrefixUnits, exp2_scale(a.rows.scale), a.rows.scale < 0.0f, w};
+    return plan.dim == 64 ? launch_tiles<64, true>(p, g, plan.grid, stream) : launch_tiles<128, true>(p, g, plan.grid, stream);
+}
+
 cudaError_t launch_prompt_attention(const AttnParams& a, const TilePlan& plan, const TileWork& w, cudaStream_t stream) {
     const Geometry g = geometry(a);
-    TileParams p{a, g.group, g.tile_tokens, plan.split, kMinPromptUnits, 0.0f, 0, w};
-    set_scale(p);
+    TileParams p{a, g.group, g.tile_tokens, plan.split, kMinPromptUnits, exp2_scale(a.rows.scale), a.rows.scale < 0.0f, w};
     cudaError_t e = plan.dim == 64 ? launch_tiles<64, false>(p, g, plan.grid, stream)
                                    : launch_tiles<128, false>(p, g, plan.grid, stream);
     if (e != cudaSuccess || !plan.split) return e;

@@ -8,6 +8,7 @@
 #include <cstdint>
 #include <mutex>
 
+#include "vw_attention.h"
 #include "vw_internal.h"
 
 namespace vw {
@@ -64,6 +65,36 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+            "r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w,
+                                            uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {   // relative error 2^-22; -inf gives 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -97,6 +128,36 @@ inline bool make_map(CUtensorMap* m, CUtensorMapDataType type, size_t esize, con
     const cuuint32_t estr[2] = {1, 1};
     return fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// A cache's keys or values in boxes of 64 dims x min(page_size, max_rows) tokens of one head of one page; dims past
+// head_dim read zeros
+inline bool make_cache_map(CUtensorMap* m, const KvCacheDev& c, const void* base, int max_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(c.head_dim), static_cast<cuuint64_t>(c.page_size),
+                                static_cast<cuuint64_t>(c.n_kv_heads), static_cast<cuuint64_t>(c.n_pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(c.token_stride) * 2, static_cast<cuuint64_t>(c.head_stride) * 2,
+                                   static_cast<cuuint64_t>(c.page_stride) * 2};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(c.page_size < max_rows ? c.page_size : max_rows), 1, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, ones,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// The query rows in boxes of 64 dims x box_heads heads (0: a whole group's) x box_rows rows
+inline bool make_row_map(CUtensorMap* m, const AttnParams& a, int box_rows, int box_heads = 0) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {static_cast<cuuint64_t>(a.cache.head_dim), static_cast<cuuint64_t>(a.rows.n_q_heads),
+                                static_cast<cuuint64_t>(a.batch.n_rows)};
+    const cuuint64_t strides[2] = {static_cast<cuuint64_t>(a.rows.q_head) * 2, static_cast<cuuint64_t>(a.rows.q_row) * 2};
+    const cuuint32_t heads = box_heads ? box_heads : a.rows.n_q_heads / a.cache.n_kv_heads;
+    const cuuint32_t box[3] = {64, heads, static_cast<cuuint32_t>(box_rows)};
+    const cuuint32_t ones[3] = {1, 1, 1};
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<__nv_bfloat16*>(a.rows.q), dims, strides, box, ones,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
