@@ -144,7 +144,7 @@ __device__ __forceinline__ int find_sequence(const int32_t* offsets, int n_seqs,
     while (n > 1) {
         const int step = (n + 31) / 32;
         const int at = lo + lane * step;
-        const bool le = lane * step < n && offsets[at] <= row;
+        const bool le = lane * step < n && __ldg(offsets + at) <= row;
         const unsigned m = __ballot_sync(0xffffffffu, le);
         if (!m) return -1;
         const int last = 31 - __clz(m);
@@ -169,11 +169,11 @@ __device__ __forceinline__ Seq load_seq(const AttnParams& a, int s) {
     const int limit = kPrefix ? a.batch.n_seqs : a.batch.n_rows;
     int begin = s, end = min(s + 1, limit);
     if (o) {
-        begin = o[s];
-        end = o[s + 1];
+        begin = __ldg(o + s);
+        end = __ldg(o + s + 1);
     }
-    q.kv = kPrefix ? checked_len(a.prefix.lens[s], a.prefix.max_pages, shift, a.err, kErrKvLens)
-                   : checked_len(a.batch.kv_lens[s], a.batch.max_pages, shift, a.err, kErrKvLens);
+    q.kv = kPrefix ? checked_len(__ldg(a.prefix.lens + s), a.prefix.max_pages, shift, a.err, kErrKvLens)
+                   : checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, shift, a.err, kErrKvLens);
     if (begin < 0 || end < begin || end > limit) {
         atomicOr(a.err, kErrKvLens);
         return q;

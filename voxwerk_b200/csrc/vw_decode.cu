@@ -164,7 +164,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         const int n_seqs = a.batch.n_seqs, shift = cache.page_shift;
         const int per_seq = cache.n_kv_heads * p.plan.row_blocks;   // items of a sequence
         auto keys_of = [&](int s) {
-            return checked_len(a.batch.kv_lens[s], a.batch.max_pages, shift, err, kErrKvLens);
+            return checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, shift, err, kErrKvLens);
         };
         auto tiles_of = [&](int keys) { return max((keys + kKeys - 1) / kKeys, 1); };   // an empty one is written too
         int64_t total = 0;
@@ -240,7 +240,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             auto page_of = [&](int t) {
                 const int key = t * kKeys + box * box_rows;
                 if (box >= p.boxes || key >= it.keys || t >= it.tile1) return -1;
-                const int page = table[key >> shift];
+                const int page = __ldg(table + (key >> shift));
                 if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.n_pages)) {
                     atomicOr(err, kErrPageRange);
                     return cache.n_pages;   // past the map's end: zeros

@@ -29,6 +29,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
+#include <type_traits>
 
 #include "vw_attention.h"
 #include "vw_internal.h"
@@ -43,7 +44,9 @@ constexpr int kRows = kTileRows;  // rows per row tile
 constexpr int kWholeKeys = 512;   // sequences of at most this many keys are never split
 constexpr int kMinPromptUnits = 2, kMinPrefixUnits = 1;   // fewest units a CTA takes
 constexpr int kFeedRegs = 96, kSoftmaxRegs = 200;   // registers per thread of warps 0-3 and 4-11
+constexpr int kPolyPairs = 0;   // pairs of scores of every eight whose power of two is the polynomial
 constexpr float kLn2 = 0.693147180559945309f;
+constexpr uint32_t kOutBytes = 32 * 128;   // a softmax warp's outputs on their way: 32 rows of 128 bytes
 constexpr int kItemSlots = 3;
 constexpr int kItemReaders = 10;  // MMA thread, warp 2, eight softmax warps
 
@@ -52,11 +55,12 @@ struct TileCfg {
     static constexpr int kHalves = DP / 64;
     static constexpr uint32_t kHalfBytes = 128 * 128;   // 128 rows of 64 bf16, 128-byte swizzle
     static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
-    static constexpr int kStages = DP == 128 ? 5 : 8;
+    static constexpr int kStages = DP == 128 ? 4 : 8;
     static constexpr uint32_t kOffKv = 2 * kTileBytes;   // after the two Q tiles
-    static constexpr uint32_t kOffBar = kOffKv + kStages * kTileBytes;
-    // kv_full[S] kv_empty[S] q_full q_empty s_full[2] p_full[2] o_full[2] v_tail v_fixed item_full[3] item_empty[3] done
-    static constexpr uint32_t kBars = 2 * kStages + 17;
+    static constexpr uint32_t kOffOut = kOffKv + kStages * kTileBytes;   // 4 KB per softmax warp
+    static constexpr uint32_t kOffBar = kOffOut + 8 * kOutBytes;
+    // kv_full[S] kv_empty[S] q_full q_empty s_full[2] p_full[2][2] o_full[2] v_tail v_fixed item_full[3] item_empty[3] done
+    static constexpr uint32_t kBars = 2 * kStages + 19;
     static constexpr uint32_t kOffItems = kOffBar + 8 * kBars;
     static constexpr uint32_t kOffMisc = kOffItems + kItemSlots * 64;
     static constexpr uint32_t kBytes = kOffMisc + 16;
@@ -119,6 +123,8 @@ struct Scheduler {
     // by ticket
     int ticket, level, base;
     int64_t before;
+    Seq own;                             // sequence `lane`
+    bool taken = false;                  // the first ticket is the CTA's number
     // split
     int64_t unit, unit_end, seq_first;   // the CTA's units; the first unit of sequence `seq`
     int seq;
@@ -159,9 +165,10 @@ struct Scheduler {
             }
         } else {
             ticket = blockIdx.x;
+            own = lane < n_seqs ? load_seq<kPrefix>(p.a, lane) : Seq{0, 0, 0, 0};
             int top = -1;
             for (int s = lane; s < n_seqs; s += 32) {
-                const Seq q = load_seq<kPrefix>(p.a, s);
+                const Seq q = s < 32 ? own : load_seq<kPrefix>(p.a, s);
                 if (q.n > 0) top = max(top, first_level(q) + ceil_div(q.n, block_tokens) - 1);
             }
             level = __reduce_max_sync(0xffffffffu, top);
@@ -176,12 +183,17 @@ struct Scheduler {
         Item none;
         none.valid = 0;
         if (p.split) return unit < unit_end ? next_piece() : none;
+        if (taken) {
+            if (lane == 0) ticket = gridDim.x + atomicAdd(p.w.counters, 1);
+            ticket = __shfl_sync(0xffffffffu, ticket, 0);
+        }
+        taken = true;
         while (level >= 0) {
             const int s = base + lane;
             Seq q{0, 0, 0, 0};
             int i = -1;
             if (s < n_seqs) {
-                q = load_seq<kPrefix>(p.a, s);
+                q = base == 0 ? own : load_seq<kPrefix>(p.a, s);
                 i = level - first_level(q);
                 if (q.n <= 0 || i >= ceil_div(q.n, block_tokens)) i = -1;
             }
@@ -195,8 +207,6 @@ struct Scheduler {
                 q.past = __shfl_sync(0xffffffffu, q.past, at);
                 i = __shfl_sync(0xffffffffu, i, at);
                 const Item it = make_item<kPrefix>(p, q, base + at, i, ticket % kv_heads, 0, INT32_MAX, true, 0);
-                if (lane == 0) ticket = gridDim.x + atomicAdd(p.w.counters, 1);
-                ticket = __shfl_sync(0xffffffffu, ticket, 0);
                 return it;
             }
             before += __popc(m);
@@ -292,6 +302,32 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
+// 2^x of two values without the special-function unit: x = j + f with j the nearest integer (it lands in the low bits of
+// x + 1.5 * 2^23), 2^f by a polynomial of degree 5 on [-1/2, 1/2] with p(0) = 1 (a minimax fit of the relative error,
+// 1.9e-7 in fp32, as good as ex2.approx), and j added to the exponent.  Below 2^-126 it stays at 2^-126; a NaN gives
+// no NaN.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c);
+__device__ __forceinline__ float2 add2(float2 a, float2 b);
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    const auto both = [](float v) { return make_float2(v, v); };
+    x.x = fmaxf(x.x, -126.0f);
+    x.y = fmaxf(x.y, -126.0f);
+    const float2 t = add2(x, both(12582912.0f));
+    const float2 j = add2(t, both(-12582912.0f));
+    const float2 f = fma2(j, both(-1.0f), x);
+    float2 r = fma2(f, both(0.001326472731307149f), both(0.009671512991189957f));
+    r = fma2(r, f, both(0.05550733581185341f));
+    r = fma2(r, f, both(0.24022242426872253f));
+    r = fma2(r, f, both(0.6931470036506653f));
+    r = fma2(r, f, both(1.0f));
+    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
+                       __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("{\n\t.reg .b64 a, b, d;\n\t"
@@ -301,6 +337,39 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return d;
 }
+// an item read by the whole warp, in a form the compiler knows to be uniform
+__device__ __forceinline__ Item uniform_item(const Item& m) {
+    Item it = m;
+    constexpr unsigned kAll = 0xffffffffu;
+    it.valid = __shfl_sync(kAll, it.valid, 0);
+    it.tokens = __shfl_sync(kAll, it.tokens, 0);
+    it.pos0 = __shfl_sync(kAll, it.pos0, 0);
+    it.kv = __shfl_sync(kAll, it.kv, 0);
+    it.tile0 = __shfl_sync(kAll, it.tile0, 0);
+    it.end[0] = __shfl_sync(kAll, it.end[0], 0);
+    it.end[1] = __shfl_sync(kAll, it.end[1], 0);
+    return it;
+}
+// products of bf16 operands into fp32 tensor memory: left operand from shared memory, or from tensor memory
+__device__ __forceinline__ void mma_ss(bool pred, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(pred ? 1 : 0)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(bool pred, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(pred ? 1 : 0)
+        : "memory");
+}
+
 template <int DP, bool kPrefix>
 __global__ void __launch_bounds__(kThreads384, 1)
 attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -312,14 +381,14 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const uint32_t sbase = s32(sm);
     const uint32_t kv_full = sbase + C::kOffBar, kv_empty = kv_full + 8 * S;
     const uint32_t q_full = kv_empty + 8 * S, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 16,
-                   o_full = p_full + 16, v_tail = o_full + 16, v_fixed = v_tail + 8, item_full = v_fixed + 8,
+                   o_full = p_full + 32, v_tail = o_full + 16, v_fixed = v_tail + 8, item_full = v_fixed + 8,
                    item_empty = item_full + 8 * kItemSlots, done = item_empty + 8 * kItemSlots;
     Item* items = reinterpret_cast<Item*>(sm + C::kOffItems);   // 64 bytes apart
     auto item_slot = [&](uint32_t n) { return reinterpret_cast<Item*>(reinterpret_cast<uint8_t*>(items) + 64 * (n % kItemSlots)); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
     volatile int32_t* abort = reinterpret_cast<volatile int32_t*>(sm + C::kOffMisc + 4);
     unsigned* err = p.a.err;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
     // the decode kernel that follows the prefixes' may take the SMs as they come free (it waits before it reads here)
     if (kPrefix) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -330,7 +399,8 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         init(q_empty, 1);
         for (int q = 0; q < 2; ++q) {
             init(s_full + 8 * q, 1);
-            init(p_full + 8 * q, 4);
+            init(p_full + 16 * q, 4);
+            init(p_full + 16 * q + 8, 4);
             init(o_full + 8 * q, 1);
         }
         init(v_tail, 1);
@@ -343,6 +413,9 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *abort = 0;
     }
+    if (warp == 0 && lane == 0)
+        for (const CUtensorMap* m : {&map_q, &map_k, &map_v})
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     if (warp == 1) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(s32(tmem_slot)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -366,12 +439,11 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             Scheduler<kPrefix> sched(p, lane);
             uint32_t n_items = 0, n_q = 0, st = 0;
             bool stop = false;
-            while (!stop) {
-                const Item it = sched.next();
+            Item it = sched.next(), following = it;
+            for (; !stop; it = following) {
                 if (n_items >= kItemSlots &&
-                    !wait_bounded(item_empty + 8 * (n_items % kItemSlots), (n_items / kItemSlots - 1) & 1, abort, err))
-                    stop = true;
-                if (__any_sync(0xffffffffu, stop)) break;
+                    !wait_warp(item_empty + 8 * (n_items % kItemSlots), (n_items / kItemSlots - 1) & 1, abort, err))
+                    break;
                 if (lane == 0) {
                     *item_slot(n_items) = it;
                     arrive(item_full + 8 * (n_items % kItemSlots));
@@ -380,14 +452,17 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 ++n_items;
                 if (!it.valid) break;
                 const int end = max(it.end[0], it.end[1]);
-                if (end <= it.tile0) continue;
+                if (end <= it.tile0) {
+                    following = sched.next();
+                    continue;
+                }
                 // page of this lane's box of a key tile; past the block's last key: no box
                 const int seen = kPrefix ? it.kv : min(max(it.pos0 + it.tokens, 0), it.kv);
                 const int32_t* table = tables + it.seq * table_stride;
                 auto page_of = [&](int t) {
                     const int key = t * kKeys + lane * box_rows;
                     if (lane >= boxes || key >= seen || t >= end) return -1;
-                    const int page = table[key >> shift];
+                    const int page = __ldg(table + (key >> shift));
                     if (static_cast<unsigned>(page) >= static_cast<unsigned>(cache.n_pages)) {
                         atomicOr(err, kErrPageRange);
                         return cache.n_pages;   // past the map's end: zeros
@@ -395,8 +470,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     return page;
                 };
                 int page = page_of(it.tile0);
-                if (n_q > 0 && !wait_bounded(q_empty, (n_q - 1) & 1, abort, err)) stop = true;
-                if (__any_sync(0xffffffffu, stop)) break;
+                if (n_q > 0 && !wait_warp(q_empty, (n_q - 1) & 1, abort, err)) break;
                 ++n_q;
                 if (lane == 0) {
                     const int tiles = it.end[1] > it.tile0 ? 2 : 1;   // row tile 1 sees at least row tile 0's keys
@@ -415,8 +489,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     #pragma unroll
                     for (int kv = 0; kv < 2; ++kv, ++st) {
                         const uint32_t s = st % S;
-                        if (st >= S && !wait_bounded(kv_empty + 8 * s, (st / S - 1) & 1, abort, err)) stop = true;
-                        if (__any_sync(0xffffffffu, stop)) {
+                        if (st >= S && !wait_warp(kv_empty + 8 * s, (st / S - 1) & 1, abort, err)) {
                             stop = true;
                             break;
                         }
@@ -434,6 +507,8 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         }
                     }
                     page = next;
+                    // the next block is taken near the end of this one (early tickets would deal the blocks out as by turns)
+                    if (t == max(it.tile0, end - 2)) following = sched.next();
                 }
             }
             // teardown: the copies in flight land before the CTA may exit
@@ -443,98 +518,87 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
             __syncwarp();
         } else if (warp == 1) {
-            // ---------------- matrix products (one thread)
-            if (lane == 0) {
-                const int D = p.a.cache.head_dim;
-                const int k_steps = (D + 15) / 16;                        // of Q K^T
-                const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kRows >> 4) << 24);   // fp32 += bf16 x bf16
-                const uint32_t idesc_pv = idesc | (1u << 16) | (static_cast<uint32_t>(2 * k_steps) << 17);   // V is N-major
-                uint32_t st = 0, n_q = 0, n_p[2] = {0, 0}, n_fixed = 0;
-                bool stop = false;
-                for (uint32_t n = 0; !stop; ++n) {
-                    if (!wait_bounded(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err)) break;
-                    const Item it = *item_slot(n);
-                    arrive(item_empty + 8 * (n % kItemSlots));
-                    if (!it.valid) break;
-                    const int end = max(it.end[0], it.end[1]);
-                    if (end <= it.tile0) continue;
-                    int seen[2];   // keys the tile's last row sees
-                    for (int q = 0; q < 2; ++q)
-                        seen[q] = kPrefix ? it.kv : min(max(it.pos0 + min(it.tokens, (q + 1) * p.tile_tokens), 0), it.kv);
-                    const int all = max(seen[0], seen[1]);
-                    const bool fix = ((all + 15) & ~15) > it.kv;   // the last tile's value rows past it.kv are cleared
-                    if (!wait_bounded(q_full, n_q++ & 1, abort, err)) break;
-                    for (int t = it.tile0; t <= end && !stop; ++t) {
-                        // tile t: S(t) after P V(t - 1), so that P's columns are free for S
-                        const uint32_t sk = st % S, sv = (st + S - 1) % S;   // stages of K(t) and V(t - 1)
-                        if (t > it.tile0) {
-                            if (!wait_bounded(kv_full + 8 * sv, ((st - 1) / S) & 1, abort, err)) {
-                                stop = true;
-                                break;
-                            }
-                            if (fix && t == (all + kKeys - 1) / kKeys) {
-                                arrive(v_tail);   // V(t - 1) has landed: warp 2 may clear its tail
-                                if (!wait_bounded(v_fixed, n_fixed++ & 1, abort, err)) {
-                                    stop = true;
-                                    break;
-                                }
-                            }
-                        }
-                        if (t < end && !wait_bounded(kv_full + 8 * sk, (st / S) & 1, abort, err)) {
-                            stop = true;
-                            break;
-                        }
-    #pragma unroll
-                        for (int q = 0; q < 2; ++q) {
-                            if (t > it.tile0 && t - 1 < it.end[q]) {
-                                if (!wait_bounded(p_full + 8 * q, n_p[q]++ & 1, abort, err)) {
-                                    stop = true;
-                                    break;
-                                }
-                                fence_after();
-                                const uint32_t v0 = sbase + C::kOffKv + sv * C::kTileBytes;
-                                const int steps = (min(seen[q] - (t - 1) * kKeys, kKeys) + 15) / 16;
-                                for (int k = 0; k < steps; ++k) {
-                                    const uint32_t accumulate = (t - 1 > it.tile0 || k > 0) ? 1u : 0u;
-                                    asm volatile(
-                                        "{\n\t.reg .pred p;\n\t"
-                                        "setp.ne.b32 p, %4, 0;\n\t"
-                                        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(
-                                            tmem + 256 + 128 * q),
-                                        "r"(tmem + 128 * q + 8 * k), "l"(value_desc(v0 + 2048 * k)), "r"(idesc_pv),
-                                        "r"(accumulate)
-                                        : "memory");
-                                }
-                                if (t == it.end[q]) mma_commit(o_full + 8 * q);
-                            }
-                            if (t < it.end[q]) {
-                                fence_after();
-                                const uint32_t a0 = sbase + q * C::kTileBytes, b0 = sbase + C::kOffKv + sk * C::kTileBytes;
-                                const int n16 = (min(seen[q] - t * kKeys, kKeys) + 15) / 16;
-                                const uint32_t id = idesc | (static_cast<uint32_t>(2 * n16) << 17);
-                                for (int k = 0; k < k_steps; ++k) {
-                                    const uint32_t off = (k >> 2) * C::kHalfBytes + 32 * (k & 3);
-                                    const uint32_t accumulate = k > 0 ? 1u : 0u;
-                                    asm volatile(
-                                        "{\n\t.reg .pred p;\n\t"
-                                        "setp.ne.b32 p, %4, 0;\n\t"
-                                        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem + 128 * q),
-                                        "l"(umma_desc(a0 + off)), "l"(umma_desc(b0 + off)), "r"(id), "r"(accumulate)
-                                        : "memory");
-                                }
-                                mma_commit(s_full + 8 * q);
-                            }
-                        }
-                        if (stop) break;
-                        if (t > it.tile0) mma_commit(kv_empty + 8 * sv);
-                        if (t < end) {
-                            mma_commit(kv_empty + 8 * sk);
-                            if (t == end - 1) mma_commit(q_empty);
-                            st += 2;
+            // ---------------- matrix products: one thread issues them, the whole warp walks the loop, so that descriptors
+            // and addresses stay in uniform registers (computed in a divergent thread they cost ten cycles apiece to move
+            // there: 4700 cycles a tile pair, against 2048 for its products)
+            const bool leader = lane == 0;
+            const int k_steps = (p.a.cache.head_dim + 15) / 16;       // of Q K^T
+            const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kRows >> 4) << 24);   // fp32 += bf16 x bf16
+            const uint32_t idesc_pv = idesc | (1u << 16) | (static_cast<uint32_t>(2 * k_steps) << 17);   // V is N-major
+            const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
+            uint32_t st = 0, n_q = 0, n_p[2] = {0, 0}, n_fixed = 0;
+            bool ok = true;
+            for (uint32_t n = 0; ok; ++n) {
+                ok = wait_warp(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err);
+                if (!ok) break;
+                const Item it = uniform_item(*item_slot(n));
+                arrive_if(leader, item_empty + 8 * (n % kItemSlots));
+                if (!it.valid) break;
+                const int end = max(it.end[0], it.end[1]);
+                if (end <= it.tile0) continue;
+                int seen[2];   // keys the tile's last row sees
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    seen[q] = kPrefix ? it.kv : min(max(it.pos0 + min(it.tokens, (q + 1) * p.tile_tokens), 0), it.kv);
+                const int all = max(seen[0], seen[1]);
+                const bool fix = ((all + 15) & ~15) > it.kv;   // the last tile's value rows past it.kv are cleared
+                ok = wait_warp(q_full, n_q++ & 1, abort, err);
+                for (int t = it.tile0; t <= end && ok; ++t) {
+                    // tile t: S(t) after P V(t - 1), so that P's columns are free for S
+                    const uint32_t sk = st % S, sv = (st + S - 1) % S;   // stages of K(t) and V(t - 1)
+                    const uint32_t k0 = sbase + C::kOffKv + sk * C::kTileBytes, v0 = sbase + C::kOffKv + sv * C::kTileBytes;
+                    if (t > it.tile0) {
+                        ok = wait_warp(kv_full + 8 * sv, ((st - 1) / S) & 1, abort, err);
+                        if (ok && fix && t == (all + kKeys - 1) / kKeys) {
+                            arrive_if(leader, v_tail);   // V(t - 1) has landed: warp 2 may clear its tail
+                            ok = wait_warp(v_fixed, n_fixed++ & 1, abort, err);
                         }
                     }
+                    if (ok && t < end) ok = wait_warp(kv_full + 8 * sk, (st / S) & 1, abort, err);
+                    if (!ok) break;
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        if (t > it.tile0 && t - 1 < it.end[q]) {
+                            const int steps = (min(seen[q] - (t - 1) * kKeys, kKeys) + 15) / 16;
+                            const uint64_t vd = value_desc(v0);
+                            const uint32_t later = t - 1 > it.tile0 ? 1u : 0u;
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {   // P comes in two halves of the keys
+                                ok = ok && wait_warp(p_full + 16 * q + 8 * h, n_p[q] & 1, abort, err);
+                                fence_after();
+#pragma unroll
+                                for (int k = 4 * h; k < 4 * h + 4; ++k)   // 16 keys: 16 rows of 128 bytes, 8 columns of P
+                                    mma_ts(leader && ok && k < steps, t0 + 256 + 128 * q, t0 + 128 * q + 8 * k,
+                                           vd + k * (2048 >> 4), idesc_pv, k > 0 ? 1u : later);
+                            }
+                            ++n_p[q];
+                            if (!ok) break;
+                            if (t == it.end[q]) mma_commit_if(leader, o_full + 8 * q);
+                        }
+                        if (t < it.end[q]) {
+                            fence_after();
+                            const int n16 = (min(seen[q] - t * kKeys, kKeys) + 15) / 16;
+                            const uint32_t id = idesc | (static_cast<uint32_t>(2 * n16) << 17);
+                            const uint64_t ad = umma_desc(sbase + q * C::kTileBytes), bd = umma_desc(k0);
+#pragma unroll
+                            for (int k = 0; k < DP / 16; ++k) {   // 16 dims: 32 bytes along a row of 64
+                                const uint32_t off = ((k >> 2) * C::kHalfBytes + 32 * (k & 3)) >> 4;
+                                mma_ss(leader && k < k_steps, t0 + 128 * q, ad + off, bd + off, id, k > 0 ? 1u : 0u);
+                            }
+                            mma_commit_if(leader, s_full + 8 * q);
+                        }
+                    }
+                    if (!ok) break;
+                    if (t > it.tile0) mma_commit_if(leader, kv_empty + 8 * sv);
+                    if (t < end) {
+                        mma_commit_if(leader, kv_empty + 8 * sk);
+                        mma_commit_if(leader && t == end - 1, q_empty);
+                        st += 2;
+                    }
                 }
-                // teardown: every product issued has completed before the tensor memory is freed
+            }
+            // teardown: every product issued has completed before the tensor memory is freed
+            if (leader) {
                 mma_commit(done);
                 drain_wait(done, 0);
             }
@@ -543,8 +607,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             // ---------------- clears value rows past a sequence's last key
             uint32_t st = 0, n_fixed = 0;
             for (uint32_t n = 0;; ++n) {
-                bool ok = wait_bounded(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (!wait_warp(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err)) break;
                 const Item it = *item_slot(n);
                 __syncwarp();
                 if (lane == 0) arrive(item_empty + 8 * (n % kItemSlots));
@@ -556,9 +619,9 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 if (upto > it.kv && end == (all + kKeys - 1) / kKeys) {
                     const uint32_t j = st + 2 * (end - 1 - it.tile0) + 1, s = j % S;   // the stage of V(end - 1)
                     // (its own phase of kv_full: the stage is not released before v_fixed)
-                    ok = wait_bounded(v_tail, n_fixed++ & 1, abort, err) &&
-                         wait_bounded(kv_full + 8 * s, (j / S) & 1, abort, err);
-                    if (!__all_sync(0xffffffffu, ok)) break;
+                    if (!wait_warp(v_tail, n_fixed++ & 1, abort, err) ||
+                        !wait_warp(kv_full + 8 * s, (j / S) & 1, abort, err))
+                        break;
                     const int r0 = it.kv - (end - 1) * kKeys, rows = upto - it.kv;
                     for (int h = 0; h < C::kHalves; ++h)
                         for (int i = lane; i < rows * 8; i += 32)
@@ -580,12 +643,12 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const uint32_t t_s = tmem + quarter + 128 * q, t_o = tmem + quarter + 256 + 128 * q;
         const int token = q * p.tile_tokens + row / p.group, sub = row % p.group;
         const bool in_tile = row < p.tile_tokens * p.group;
-        const float2 c2 = make_float2(p.c, p.c);
+        const float c = p.c;
+        const float2 c2 = make_float2(c, c);
         uint32_t n_s = 0, n_o = 0;
         bool stop = false;
         for (uint32_t n = 0; !stop; ++n) {
-            bool ok = wait_bounded(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err);
-            if (!__all_sync(0xffffffffu, ok)) break;
+            if (!wait_warp(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err)) break;
             const Item it = *item_slot(n);
             __syncwarp();
             if (lane == 0) arrive(item_empty + 8 * (n % kItemSlots));
@@ -595,80 +658,100 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const bool any_live = __any_sync(0xffffffffu, live);
             float m = -INFINITY, l = 0.0f;
             for (int t = it.tile0; t < it.end[q]; ++t, ++n_s) {
-                ok = wait_bounded(s_full + 8 * q, n_s & 1, abort, err);
-                if (!__all_sync(0xffffffffu, ok)) {
+                if (!wait_warp(s_full + 8 * q, n_s & 1, abort, err)) {
                     stop = true;
                     break;
                 }
                 fence_after();
                 if (any_live) {
-                    float s[kKeys];
-#pragma unroll
-                    for (int i = 0; i < kKeys; i += 32) tmem_load32(t_s + i, s + i);
-                    tmem_wait_load();
-                    if (p.negate) {
-#pragma unroll
-                        for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
-                    }
+                    // two passes over S, 32 columns at a time with the next 32 on their way: the maximum, then P.  (Held in
+                    // registers, 128 scores a thread leave too few for the exponentials to overlap, and their unrolled code
+                    // misses the instruction cache.)
                     const int columns = limit - t * kKeys;
-                    if (!__all_sync(0xffffffffu, columns >= kKeys || !live)) {
+                    const bool masked = !__all_sync(0xffffffffu, columns >= kKeys || !live);
+                    float s[2][32];
+                    const auto fetch = [&](int i, float* d) { tmem_load32(t_s + 32 * i, d); };
+                    const auto prepare = [&](int i, float* d) {
+                        if (p.negate) {
 #pragma unroll
-                        for (int i = 0; i < kKeys; ++i) s[i] = i < columns ? s[i] : -INFINITY;
-                    }
-                    float top[4];
+                            for (int j = 0; j < 32; ++j) d[j] = -d[j];
+                        }
+                        if (masked) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) top[j] = fmaxf(s[j], s[4 + j]);
-#pragma unroll
-                    for (int i = 8; i < kKeys; i += 8)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) top[j] = fmaxf(top[j], fmaxf(s[i + j], s[i + 4 + j]));
-                    const float tile_max = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                    // a first maximum is taken as it is (nothing but zeros was summed); a later one when it rose enough
-                    const bool rise = live && m != -INFINITY && (tile_max - m) * p.c > 8.0f;
-                    if (__any_sync(0xffffffffu, rise)) {   // products up to t - 1 are done: S(t) came after them
-                        const float f = rise ? exp2_fast((m - tile_max) * p.c) : 1.0f;
-                        l *= f;
-                        if (rise) m = tile_max;
+                            for (int j = 0; j < 32; ++j) d[j] = 32 * i + j < columns ? d[j] : -INFINITY;
+                        }
+                    };
+                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    fetch(0, s[0]);
 #pragma unroll 1
-                        for (int i = 0; i < DP; i += 32) {
-                            float o[32];
-                            tmem_load32(t_o + i, o);
+                    for (int i = 0; i < 4; i += 2)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            tmem_wait_load();
+                            fetch((i + h + 1) & 3, s[h ^ 1]);   // (after the last: the first again, for the second pass)
+                            prepare(i + h, s[h]);
+#pragma unroll
+                            for (int j = 0; j < 32; j += 8)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) top[k] = max3(top[k], s[h][j + k], s[h][j + 4 + k]);
+                        }
+                    const float tile_max = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
+                    // a first maximum is taken as it is (nothing but zeros was summed), a later one when it rose enough; a
+                    // NaN score makes the row NaN
+                    const bool rise = live && m != -INFINITY && (tile_max - m) * c > 8.0f;
+                    const float f = rise ? exp2_fast((m - tile_max) * c) : 1.0f;
+                    if (rise || m == -INFINITY || tile_max != tile_max) m = tile_max;
+                    const float mc = m == -INFINITY ? 0.0f : -m * c;
+                    const float2 mc2 = make_float2(mc, mc);
+                    float2 sum[4] = {};
+                    if (__any_sync(0xffffffffu, rise)) {   // products up to t - 1 are done: S(t) came after them
+                        tmem_wait_load();
+#pragma unroll 1
+                        for (int d = 0; d < DP; d += 32) {
+                            tmem_load32(t_o + d, s[1]);
                             tmem_wait_load();
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] *= f;
-                            tmem_store32(t_o + i, o);
+                            for (int j = 0; j < 32; ++j) s[1][j] *= f;
+                            tmem_store32(t_o + d, s[1]);
+                        }
+                    }
+#pragma unroll 1
+                    for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            tmem_wait_load();
+                            if (i + h < 3) fetch(i + h + 1, s[h ^ 1]);
+                            prepare(i + h, s[h]);
+                            float2 e[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) e[j] = fma2(make_float2(s[h][2 * j], s[h][2 * j + 1]), c2, mc2);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j)
+                                e[j] = (j * 3) % 8 < kPolyPairs ? exp2_poly(e[j])
+                                                                : make_float2(exp2_fast(e[j].x), exp2_fast(e[j].y));
+                            uint32_t pk[16];   // the product's operand; the sum keeps fp32
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) pk[j] = pack_bf16(e[j].x, e[j].y);
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) sum[j & 3] = add2(sum[j & 3], e[j]);
+                            tmem_store16(t_s + 16 * (i + h), pk);   // over scores that were read
                         }
                         tmem_wait_store();
+                        fence_before();
+                        __syncwarp();
+                        arrive_if(lane == 0, p_full + 16 * q + 4 * i);
                     }
-                    if (m == -INFINITY) m = tile_max;
-                    const float mc = m == -INFINITY ? 0.0f : -m * p.c;
-                    const float2 mc2 = make_float2(mc, mc);
-                    float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-#pragma unroll
-                    for (int i = 0; i < kKeys; i += 32) {
-                        uint32_t pk[16];
-#pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float2 x = fma2(make_float2(s[i + j], s[i + j + 1]), c2, mc2);
-                            const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
-                            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
-                            pk[j >> 1] = pack_bf16(e.x, e.y);   // the product's operand; the sum keeps fp32
-                        }
-                        tmem_store16(t_s + (i >> 1), pk);
-                    }
-                    const float2 both = add2(sum[0], sum[1]);
-                    l += both.x + both.y;
-                    tmem_wait_store();
+                    const float2 both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                    l = __fmaf_rn(l, f, both.x + both.y);
+                } else {
+                    arrive_if(lane == 0, p_full + 16 * q);
+                    arrive_if(lane == 0, p_full + 16 * q + 8);
                 }
-                fence_before();
-                __syncwarp();
-                if (lane == 0) arrive(p_full + 8 * q);
             }
             if (stop) break;
             const bool some = it.end[q] > it.tile0;
             if (some) {
-                ok = wait_bounded(o_full + 8 * q, n_o++ & 1, abort, err);
-                if (!__all_sync(0xffffffffu, ok)) break;
+                if (!wait_warp(o_full + 8 * q, n_o++ & 1, abort, err)) break;
                 fence_after();
             }
             if (!any_live) continue;
@@ -677,38 +760,62 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const int64_t call_row = it.row0 + token;
             const int head = it.kv_head * p.group + sub;
             const bool part = it.part_row >= 0;
-            const int64_t part_row = static_cast<int64_t>(it.part_row) + token * p.group + sub;
+            const int tile_rows = p.tile_tokens * p.group;
+            const int live_rows = min(tile_rows, it.tokens * p.group - q * tile_rows);   // of this row tile
+            const int64_t part0 = static_cast<int64_t>(it.part_row) + q * tile_rows;     // the tile's first partial row
             if (live) {
                 const float lse = m * p.c + log2f(l);   // no key seen: -inf
                 if (part)
-                    p.w.part_lse[part_row] = lse;
+                    p.w.part_lse[part0 + row] = lse;
                 else if (p.a.rows.lse)
                     p.a.rows.lse[call_row * p.a.rows.n_q_heads + head] = lse * kLn2;
             }
-            __nv_bfloat16* out = p.a.rows.out + call_row * p.a.rows.out_row + head * p.a.rows.out_head;
-            float* part_o = p.w.part_o + part_row * DP;
+            // O / l through shared memory (16-byte pieces of a row at piece ^ (row & 7)), so that eight lanes write 128
+            // bytes of one row: a lane storing its own row touches 32 lines an instruction
+            uint8_t* mine = sm + C::kOffOut + (warp - 4) * kOutBytes;
+            const uint64_t out_row =
+                reinterpret_cast<uint64_t>(p.a.rows.out + call_row * p.a.rows.out_row + head * p.a.rows.out_head);
+            const int width = part ? 32 : 64;   // columns of 128 bytes
 #pragma unroll 1
-            for (int i = 0; i < DP; i += 32) {
+            for (int c0 = 0; c0 < D; c0 += width) {
                 float o[32];
-                if (some) {
-                    tmem_load32(t_o + i, o);
-                    tmem_wait_load();
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (half == 1 && part) break;
+                    if (some) {
+                        tmem_load32(t_o + c0 + 32 * half, o);
+                        tmem_wait_load();
+                    }
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) o[j] = some ? o[j] * r : 0.0f;
+                    if (part) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            *reinterpret_cast<float4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                                make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *reinterpret_cast<uint4*>(mine + lane * 128 + (((4 * half + j) ^ (lane & 7)) << 4)) =
+                                make_uint4(pack_bf16(o[8 * j], o[8 * j + 1]), pack_bf16(o[8 * j + 2], o[8 * j + 3]),
+                                           pack_bf16(o[8 * j + 4], o[8 * j + 5]), pack_bf16(o[8 * j + 6], o[8 * j + 7]));
+                    }
                 }
+                __syncwarp();
+                const int piece = lane & 7;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) o[j] = some ? o[j] * r : 0.0f;
-                if (!live) continue;
-                if (part) {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4*>(part_o + i + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        if (i + j < D)
-                            *reinterpret_cast<uint4*>(out + i + j) =
-                                make_uint4(pack_bf16(o[j], o[j + 1]), pack_bf16(o[j + 2], o[j + 3]),
-                                           pack_bf16(o[j + 4], o[j + 5]), pack_bf16(o[j + 6], o[j + 7]));
+                for (int i = 0; i < 8; ++i) {
+                    const int rr = 4 * i + (lane >> 3);
+                    const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * 128 + ((piece ^ (rr & 7)) << 4));
+                    const uint64_t base = __shfl_sync(0xffffffffu, out_row, rr);
+                    const int tile_row = 32 * (warp & 3) + rr;
+                    if (tile_row >= live_rows) continue;
+                    if (part)
+                        *reinterpret_cast<uint4*>(p.w.part_o + (part0 + tile_row) * DP + c0 + 4 * piece) = v;
+                    else if (c0 + 8 * piece < D)
+                        *reinterpret_cast<uint4*>(base + 2 * (c0 + 8 * piece)) = v;
                 }
+                __syncwarp();
             }
             fence_before();   // the next block's products may overwrite O once its P is handed over
         }

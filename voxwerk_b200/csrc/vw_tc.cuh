@@ -45,6 +45,11 @@ static __device__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int3
     }
     return true;
 }
+// the same for a whole warp: one answer for its 32 lanes
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile int32_t* abort, unsigned* err) {
+    if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, wait_bounded(bar, parity, abort, err));
+}
 // teardown flavour: bounded, no error reporting (an abort is already recorded)
 static __device__ void drain_wait(uint32_t bar, uint32_t parity) {
     const uint64_t t0 = now_ns();
@@ -95,6 +100,21 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
+// (by the lanes with `pred`, so that a warp's other code stays uniform)
+__device__ __forceinline__ void arrive_if(bool pred, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q mbarrier.arrive.shared::cta.b64 _, [%0];\n\t}" ::"r"(bar),
+        "r"(pred ? 1 : 0)
+        : "memory");
+}
+__device__ __forceinline__ void mma_commit_if(bool pred, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(pred ? 1 : 0)
+        : "memory");
+}
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
