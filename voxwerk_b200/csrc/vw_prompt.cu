@@ -59,8 +59,8 @@ struct TileCfg {
     static constexpr uint32_t kOffKv = 2 * kTileBytes;   // after the two Q tiles
     static constexpr uint32_t kOffOut = kOffKv + kStages * kTileBytes;   // 4 KB per softmax warp
     static constexpr uint32_t kOffBar = kOffOut + 8 * kOutBytes;
-    // kv_full[S] kv_empty[S] q_full q_empty s_full[2] p_full[2][2] o_full[2] v_tail v_fixed item_full[3] item_empty[3] done
-    static constexpr uint32_t kBars = 2 * kStages + 19;
+    // kv_full[S] kv_empty[S] q_full q_empty s_full[2] p_full[2] o_full[2] v_tail v_fixed item_full[3] item_empty[3] done
+    static constexpr uint32_t kBars = 2 * kStages + 17;
     static constexpr uint32_t kOffItems = kOffBar + 8 * kBars;
     static constexpr uint32_t kOffMisc = kOffItems + kItemSlots * 64;
     static constexpr uint32_t kBytes = kOffMisc + 16;
@@ -381,7 +381,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     const uint32_t sbase = s32(sm);
     const uint32_t kv_full = sbase + C::kOffBar, kv_empty = kv_full + 8 * S;
     const uint32_t q_full = kv_empty + 8 * S, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 16,
-                   o_full = p_full + 32, v_tail = o_full + 16, v_fixed = v_tail + 8, item_full = v_fixed + 8,
+                   o_full = p_full + 16, v_tail = o_full + 16, v_fixed = v_tail + 8, item_full = v_fixed + 8,
                    item_empty = item_full + 8 * kItemSlots, done = item_empty + 8 * kItemSlots;
     Item* items = reinterpret_cast<Item*>(sm + C::kOffItems);   // 64 bytes apart
     auto item_slot = [&](uint32_t n) { return reinterpret_cast<Item*>(reinterpret_cast<uint8_t*>(items) + 64 * (n % kItemSlots)); };
@@ -399,8 +399,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         init(q_empty, 1);
         for (int q = 0; q < 2; ++q) {
             init(s_full + 8 * q, 1);
-            init(p_full + 16 * q, 4);
-            init(p_full + 16 * q + 8, 4);
+            init(p_full + 8 * q, 4);
             init(o_full + 8 * q, 1);
         }
         init(v_tail, 1);
@@ -442,8 +441,9 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             Item it = sched.next(), following = it;
             for (; !stop; it = following) {
                 if (n_items >= kItemSlots &&
-                    !wait_warp(item_empty + 8 * (n_items % kItemSlots), (n_items / kItemSlots - 1) & 1, abort, err))
-                    break;
+                    !wait_bounded(item_empty + 8 * (n_items % kItemSlots), (n_items / kItemSlots - 1) & 1, abort, err))
+                    stop = true;
+                if (__any_sync(0xffffffffu, stop)) break;
                 if (lane == 0) {
                     *item_slot(n_items) = it;
                     arrive(item_full + 8 * (n_items % kItemSlots));
@@ -470,7 +470,8 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     return page;
                 };
                 int page = page_of(it.tile0);
-                if (n_q > 0 && !wait_warp(q_empty, (n_q - 1) & 1, abort, err)) break;
+                if (n_q > 0 && !wait_bounded(q_empty, (n_q - 1) & 1, abort, err)) stop = true;
+                if (__any_sync(0xffffffffu, stop)) break;
                 ++n_q;
                 if (lane == 0) {
                     const int tiles = it.end[1] > it.tile0 ? 2 : 1;   // row tile 1 sees at least row tile 0's keys
@@ -489,7 +490,8 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     #pragma unroll
                     for (int kv = 0; kv < 2; ++kv, ++st) {
                         const uint32_t s = st % S;
-                        if (st >= S && !wait_warp(kv_empty + 8 * s, (st / S - 1) & 1, abort, err)) {
+                        if (st >= S && !wait_bounded(kv_empty + 8 * s, (st / S - 1) & 1, abort, err)) stop = true;
+                        if (__any_sync(0xffffffffu, stop)) {
                             stop = true;
                             break;
                         }
@@ -559,20 +561,16 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
                     for (int q = 0; q < 2; ++q) {
                         if (t > it.tile0 && t - 1 < it.end[q]) {
+                            ok = wait_warp(p_full + 8 * q, n_p[q]++ & 1, abort, err);
+                            if (!ok) break;
+                            fence_after();
                             const int steps = (min(seen[q] - (t - 1) * kKeys, kKeys) + 15) / 16;
                             const uint64_t vd = value_desc(v0);
                             const uint32_t later = t - 1 > it.tile0 ? 1u : 0u;
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {   // P comes in two halves of the keys
-                                ok = ok && wait_warp(p_full + 16 * q + 8 * h, n_p[q] & 1, abort, err);
-                                fence_after();
-#pragma unroll
-                                for (int k = 4 * h; k < 4 * h + 4; ++k)   // 16 keys: 16 rows of 128 bytes, 8 columns of P
-                                    mma_ts(leader && ok && k < steps, t0 + 256 + 128 * q, t0 + 128 * q + 8 * k,
-                                           vd + k * (2048 >> 4), idesc_pv, k > 0 ? 1u : later);
-                            }
-                            ++n_p[q];
-                            if (!ok) break;
+                            for (int k = 0; k < kKeys / 16; ++k)   // 16 keys: 16 rows of 128 bytes, 8 columns of P
+                                mma_ts(leader && k < steps, t0 + 256 + 128 * q, t0 + 128 * q + 8 * k, vd + k * (2048 >> 4),
+                                       idesc_pv, k > 0 ? 1u : later);
                             if (t == it.end[q]) mma_commit_if(leader, o_full + 8 * q);
                         }
                         if (t < it.end[q]) {
@@ -643,8 +641,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const uint32_t t_s = tmem + quarter + 128 * q, t_o = tmem + quarter + 256 + 128 * q;
         const int token = q * p.tile_tokens + row / p.group, sub = row % p.group;
         const bool in_tile = row < p.tile_tokens * p.group;
-        const float c = p.c;
-        const float2 c2 = make_float2(c, c);
+        const float2 c2 = make_float2(p.c, p.c);
         uint32_t n_s = 0, n_o = 0;
         bool stop = false;
         for (uint32_t n = 0; !stop; ++n) {
@@ -664,89 +661,82 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
                 fence_after();
                 if (any_live) {
-                    // two passes over S, 32 columns at a time with the next 32 on their way: the maximum, then P.  (Held in
-                    // registers, 128 scores a thread leave too few for the exponentials to overlap, and their unrolled code
-                    // misses the instruction cache.)
+                    float s[kKeys];
+#pragma unroll
+                    for (int i = 0; i < kKeys; i += 32) tmem_load32(t_s + i, s + i);
+                    tmem_wait_load();
+                    if (p.negate) {
+#pragma unroll
+                        for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
+                    }
                     const int columns = limit - t * kKeys;
                     const bool masked = !__all_sync(0xffffffffu, columns >= kKeys || !live);
-                    float s[2][32];
-                    const auto fetch = [&](int i, float* d) { tmem_load32(t_s + 32 * i, d); };
-                    const auto prepare = [&](int i, float* d) {
-                        if (p.negate) {
+                    if (masked) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) d[j] = -d[j];
-                        }
-                        if (masked) {
+                        for (int i = 0; i < kKeys; ++i) s[i] = i < columns ? s[i] : -INFINITY;
+                    }
+                    float top[4];
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) d[j] = 32 * i + j < columns ? d[j] : -INFINITY;
-                        }
-                    };
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    fetch(0, s[0]);
+                    for (int j = 0; j < 4; ++j) top[j] = max3(s[j], s[4 + j], s[8 + j]);
+#pragma unroll
+                    for (int i = 12; i + 8 <= kKeys; i += 8)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
+                    static_assert((kKeys - 12) % 8 == 4, "the last four scores are left");
+                    const float tile_max = max3(max3(top[0], s[kKeys - 4], s[kKeys - 3]),
+                                                max3(top[1], s[kKeys - 2], s[kKeys - 1]), max3(top[2], top[3], top[3]));
+                    // a first maximum is taken as it is (nothing but zeros was summed); a later one when it rose enough
+                    const bool rise = live && m != -INFINITY && (tile_max - m) * p.c > 8.0f;
+                    if (__any_sync(0xffffffffu, rise)) {   // products up to t - 1 are done: S(t) came after them
+                        const float f = rise ? exp2_fast((m - tile_max) * p.c) : 1.0f;
+                        l *= f;
+                        if (rise) m = tile_max;
 #pragma unroll 1
-                    for (int i = 0; i < 4; i += 2)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
+                        for (int i = 0; i < DP; i += 32) {
+                            float o[32];
+                            tmem_load32(t_o + i, o);
                             tmem_wait_load();
-                            fetch((i + h + 1) & 3, s[h ^ 1]);   // (after the last: the first again, for the second pass)
-                            prepare(i + h, s[h]);
 #pragma unroll
-                            for (int j = 0; j < 32; j += 8)
-#pragma unroll
-                                for (int k = 0; k < 4; ++k) top[k] = max3(top[k], s[h][j + k], s[h][j + 4 + k]);
+                            for (int j = 0; j < 32; ++j) o[j] *= f;
+                            tmem_store32(t_o + i, o);
                         }
-                    const float tile_max = max3(max3(top[0], top[1], top[2]), top[3], top[3]);
-                    // a first maximum is taken as it is (nothing but zeros was summed), a later one when it rose enough; a
-                    // NaN score makes the row NaN
-                    const bool rise = live && m != -INFINITY && (tile_max - m) * c > 8.0f;
-                    const float f = rise ? exp2_fast((m - tile_max) * c) : 1.0f;
-                    if (rise || m == -INFINITY || tile_max != tile_max) m = tile_max;
-                    const float mc = m == -INFINITY ? 0.0f : -m * c;
+                        tmem_wait_store();
+                    }
+                    if (m == -INFINITY || tile_max != tile_max) m = tile_max;   // a NaN score makes the row NaN
+                    const float mc = m == -INFINITY ? 0.0f : -m * p.c;
                     const float2 mc2 = make_float2(mc, mc);
                     float2 sum[4] = {};
-                    if (__any_sync(0xffffffffu, rise)) {   // products up to t - 1 are done: S(t) came after them
-                        tmem_wait_load();
-#pragma unroll 1
-                        for (int d = 0; d < DP; d += 32) {
-                            tmem_load32(t_o + d, s[1]);
-                            tmem_wait_load();
+                    // P = 2^(c S - c m); `poly` pairs of every eight by the polynomial (a tile with masked scores: none)
+                    const auto probabilities = [&](auto poly) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) s[1][j] *= f;
-                            tmem_store32(t_o + d, s[1]);
-                        }
-                    }
-#pragma unroll 1
-                    for (int i = 0; i < 4; i += 2) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            tmem_wait_load();
-                            if (i + h < 3) fetch(i + h + 1, s[h ^ 1]);
-                            prepare(i + h, s[h]);
+                        for (int i = 0; i < kKeys; i += 32) {
                             float2 e[16];
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) e[j] = fma2(make_float2(s[h][2 * j], s[h][2 * j + 1]), c2, mc2);
+                            for (int j = 0; j < 16; ++j)
+                                e[j] = fma2(make_float2(s[i + 2 * j], s[i + 2 * j + 1]), c2, mc2);
 #pragma unroll
                             for (int j = 0; j < 16; ++j)
-                                e[j] = (j * 3) % 8 < kPolyPairs ? exp2_poly(e[j])
-                                                                : make_float2(exp2_fast(e[j].x), exp2_fast(e[j].y));
+                                e[j] = (j * 3) % 8 < decltype(poly)::value ? exp2_poly(e[j])
+                                                                           : make_float2(exp2_fast(e[j].x), exp2_fast(e[j].y));
                             uint32_t pk[16];   // the product's operand; the sum keeps fp32
 #pragma unroll
                             for (int j = 0; j < 16; ++j) pk[j] = pack_bf16(e[j].x, e[j].y);
 #pragma unroll
                             for (int j = 0; j < 16; ++j) sum[j & 3] = add2(sum[j & 3], e[j]);
-                            tmem_store16(t_s + 16 * (i + h), pk);   // over scores that were read
+                            tmem_store16(t_s + (i >> 1), pk);
                         }
-                        tmem_wait_store();
-                        fence_before();
-                        __syncwarp();
-                        arrive_if(lane == 0, p_full + 16 * q + 4 * i);
-                    }
+                    };
+                    if (masked)
+                        probabilities(std::integral_constant<int, 0>{});
+                    else
+                        probabilities(std::integral_constant<int, kPolyPairs>{});
                     const float2 both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-                    l = __fmaf_rn(l, f, both.x + both.y);
-                } else {
-                    arrive_if(lane == 0, p_full + 16 * q);
-                    arrive_if(lane == 0, p_full + 16 * q + 8);
+                    l += both.x + both.y;
+                    tmem_wait_store();
                 }
+                fence_before();
+                __syncwarp();
+                if (lane == 0) arrive(p_full + 8 * q);
             }
             if (stop) break;
             const bool some = it.end[q] > it.tile0;
