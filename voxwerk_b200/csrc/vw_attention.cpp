@@ -266,6 +266,9 @@ VW_EXPORT vw_status vw_decode_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (r == VW_OK)
         r = reserve_parts(h, st, [&](auto take) {
             w.tickets = reinterpret_cast<int32_t*>(h->d_attn_counts + kCountsHeader);
+            w.units_per_cta = reinterpret_cast<int64_t*>(take(8));
+            w.chunk = reinterpret_cast<int32_t*>(take(4));
+            w.unit_end = reinterpret_cast<int64_t*>(take(static_cast<int64_t>(p.batch.n_seqs) * 8));
             w.part_lse = reinterpret_cast<float*>(take(plan.part_rows * 4));
             w.part_o = reinterpret_cast<float*>(take(plan.part_rows * plan.dim * 4));
             if (p.prefix.n_groups > 0) carve_tiles(h, prefix_plan, take, &w.prefix);

@@ -120,6 +120,9 @@ struct DecodePlan {
 };
 struct DecodeWork {
     int32_t* tickets;           // [items] pieces done, 0 between calls
+    int64_t* units_per_cta;
+    int64_t* unit_end;          // [sequences] units up to and including each
+    int32_t* chunk;             // tiles of a unit
     float* part_lse;
     float* part_o;
     TileWork prefix;            // the prefixes' partial results

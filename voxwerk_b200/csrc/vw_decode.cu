@@ -10,7 +10,8 @@
 // S = Q K^T and O += P V by mma.sync m16n8k16 from shared memory (rows are the query heads; the tensor cores idle most
 // of the time either way, a tile of 32 KB takes an SM about 1400 cycles to fetch), with a running maximum and sum of
 // their own, raised only past 2^8.  At an item's end the four are joined in shared memory, a warp per row.  An item cut
-// by a CTA boundary leaves its pieces in the workspace, and the CTA that finishes last joins them in order.
+// by a CTA boundary leaves its pieces in the workspace, and the CTA that finishes last joins them in order; with
+// prefixes every item leaves its result there, and a join kernel weighs it with the prefix's.
 //
 // Every mbarrier wait is bounded.
 
@@ -31,7 +32,6 @@ constexpr int kThreads = 160;     // producer warp, four warps of 16 keys
 constexpr int kKeys = 64;         // keys per tile
 constexpr int kMaxRows = 16;      // query heads per item: the rows of an mma
 constexpr int kItemSlots = 2;
-constexpr int kMinUnits = 2;      // fewest tiles a CTA takes
 constexpr uint32_t kSmemBudget = 113 * 1024;   // two CTAs per SM
 
 template <int DP>
@@ -142,6 +142,10 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     unsigned* err = p.a.err;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    if (p.has_prefix) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the join, once all CTAs run
+    if (warp == 0 && lane == 0)
+        for (const CUtensorMap* m : {&map_q, &map_k, &map_v})
+            asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     if (threadIdx.x == 0) {
         auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
         for (int s = 0; s < S; ++s) {
@@ -166,27 +170,46 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         auto keys_of = [&](int s) {
             return checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, shift, err, kErrKvLens);
         };
-        auto tiles_of = [&](int keys) { return max((keys + kKeys - 1) / kKeys, 1); };   // an empty one is written too
-        int64_t total = 0;
-        for (int s = lane; s < n_seqs; s += 32) total += tiles_of(keys_of(s));
-        total = __shfl_sync(0xffffffffu, warp_scan(total, lane), 31) * per_seq;
-        const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(kMinUnits));
+        // A unit is `chunk` tiles of an item (an item without keys has one, to be written).  Few items: as many tiles as
+        // give every CTA one unit at most, so that none has the ends of two items; else one tile.
+        int64_t total_tiles = 0;
+        for (int s = lane; s < n_seqs; s += 32) total_tiles += max((keys_of(s) + kKeys - 1) / kKeys, 1);
+        total_tiles = __shfl_sync(0xffffffffu, warp_scan(total_tiles, lane), 31) * per_seq;
+        const int64_t spare = static_cast<int64_t>(gridDim.x) - p.plan.items;
+        const int chunk = 2 * spare >= gridDim.x ? static_cast<int>(max((total_tiles + spare - 1) / spare, int64_t{1})) : 1;
+        auto units_of = [&](int keys) { return max((keys + kKeys * chunk - 1) / (kKeys * chunk), 1); };
+        int64_t total = total_tiles;
+        if (chunk > 1) {
+            total = 0;
+            for (int s = lane; s < n_seqs; s += 32) total += units_of(keys_of(s));
+            total = __shfl_sync(0xffffffffu, warp_scan(total, lane), 31) * per_seq;
+        }
+        const int64_t per = (total + gridDim.x - 1) / gridDim.x;
         int64_t unit = min(per * blockIdx.x, total);
         const int64_t unit_end = min(unit + per, total);
         int64_t first = 0;   // the first unit of sequence `seq`
         int seq = 0;
-        for (int s0 = 0; unit < unit_end && s0 < n_seqs; s0 += 32) {
-            const int64_t u = s0 + lane < n_seqs ? static_cast<int64_t>(tiles_of(keys_of(s0 + lane))) * per_seq : 0;
+        if (p.has_prefix && blockIdx.x == 0 && lane == 0) {   // for the join
+            *p.w.units_per_cta = per;
+            *p.w.chunk = chunk;
+        }
+        const bool all = p.has_prefix && blockIdx.x == 0;
+        bool found = false;
+        for (int s0 = 0; (all || (unit < unit_end && !found)) && s0 < n_seqs; s0 += 32) {
+            const int s = s0 + lane;
+            const int64_t u = s < n_seqs ? static_cast<int64_t>(units_of(keys_of(s))) * per_seq : 0;
             const int64_t sum = warp_scan(u, lane);
+            if (all && s < n_seqs) p.w.unit_end[s] = first + sum;
             const unsigned m = __ballot_sync(0xffffffffu, first + sum > unit);
-            if (m) {
+            if (m && !found) {
+                found = true;
                 const int at = __ffs(m) - 1;
                 seq = s0 + at;
-                first += __shfl_sync(0xffffffffu, sum - u, at);
-                break;
+                if (!all) first += __shfl_sync(0xffffffffu, sum - u, at);   // (CTA 0 begins with sequence 0)
             }
-            first += __shfl_sync(0xffffffffu, sum, 31);
+            if (all || !found) first += __shfl_sync(0xffffffffu, sum, 31);
         }
+        if (all) first = 0;
         const int box_rows = min(cache.page_size, kKeys);
         // a lane's box of a tile: page box, keys or values, half of the head
         const int box = lane / (2 * C::kHalves), is_v = (lane / C::kHalves) & 1, half = lane % C::kHalves;
@@ -196,24 +219,27 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             DecodeItem it;
             it.valid = unit < unit_end;
             if (it.valid) {
-                int keys = keys_of(seq), tiles = tiles_of(keys);
-                while (unit >= first + static_cast<int64_t>(tiles) * per_seq) {
-                    first += static_cast<int64_t>(tiles) * per_seq;
+                int keys = keys_of(seq), units = units_of(keys);
+                while (unit >= first + static_cast<int64_t>(units) * per_seq) {
+                    first += static_cast<int64_t>(units) * per_seq;
                     keys = keys_of(++seq);
-                    tiles = tiles_of(keys);
+                    units = units_of(keys);
                 }
-                const int j = static_cast<int>((unit - first) / tiles);
-                const int64_t item_first = first + static_cast<int64_t>(j) * tiles;
+                const int j = static_cast<int>((unit - first) / units);
+                const int64_t item_first = first + static_cast<int64_t>(j) * units;
+                const int tiles = max((keys + kKeys - 1) / kKeys, 1);
+                const int u0 = static_cast<int>(unit - item_first);
+                const int u1 = static_cast<int>(min(unit_end - item_first, static_cast<int64_t>(units)));
                 it.seq = seq;
                 it.kv_head = j / p.plan.row_blocks;
                 it.row_block = j % p.plan.row_blocks;
                 it.keys = keys;
-                it.tile0 = static_cast<int>(unit - item_first);
-                it.tile1 = static_cast<int>(min(unit_end - item_first, static_cast<int64_t>(tiles)));
+                it.tile0 = u0 * chunk;
+                it.tile1 = min(u1 * chunk, tiles);
                 it.c0 = static_cast<int>(item_first / per);
-                it.c1 = static_cast<int>((item_first + tiles - 1) / per);
+                it.c1 = static_cast<int>((item_first + units - 1) / per);
                 it.index = seq * per_seq + j;
-                unit = item_first + it.tile1;
+                unit = item_first + u1;
             }
             const uint32_t slot = n_items % kItemSlots;
             if (n_items >= kItemSlots && !wait_bounded(item_empty + 8 * slot, (n_items / kItemSlots - 1) & 1, abort, err))
@@ -276,6 +302,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 drain_wait(item_full + 8 * (j % kItemSlots), (j / kItemSlots) & 1);
         }
         __syncwarp();
+        if (p.has_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 
@@ -285,7 +312,6 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     float* scratch_o = reinterpret_cast<float*>(sm + off_scratch);                 // [4][rows][DP]
     float2* scratch_ml = reinterpret_cast<float2*>(scratch_o + 4 * rows * DP);     // [4][rows]
     uint32_t st = 0;
-    bool waited = false;
     for (uint32_t n = 0;; ++n) {
         const uint32_t slot = n % kItemSlots;
         bool ok = wait_bounded(item_full + 8 * slot, (n / kItemSlots) & 1, abort, err);
@@ -407,20 +433,6 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         const int live_rows = min(rows, p.group - it.row_block * kMaxRows);
         const bool pieces = it.c0 != it.c1;
         const int head0 = it.kv_head * p.group + it.row_block * kMaxRows;
-        int group = -1;
-        if (p.has_prefix) {   // the prefixes' partial results are written
-            if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-            waited = true;
-            group = find_sequence(p.a.prefix.group_offsets, p.a.prefix.n_groups, it.seq, lane);
-        }
-        auto finish = [&](PartSum<DP>& sum, int r) {
-            if (group >= 0) {
-                const PieceSpan at = piece_span<true>(p.a, p.w.prefix, group, it.seq, head0 + r, p.tile_tokens);
-                if (at.c0 <= at.c1)
-                    sum.add(p.w.prefix.part_lse, p.w.prefix.part_o, at.base, kPartRows, at.c0, at.c1, lane);
-            }
-            sum.write(p.a, it.seq, head0 + r, lane);
-        };
         const int64_t part0 = static_cast<int64_t>(it.index) * rows;   // piece c at + c * rows
         for (int r = w; r < live_rows; r += 4) {
             PartSum<DP> sum;
@@ -432,8 +444,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 for (int d = 0; d < PartSum<DP>::kDims; ++d) x[d] = scratch_o[(i * rows + r) * DP + lane * PartSum<DP>::kDims + d];
                 add_raw(sum, ml.x, ml.y, x);
             }
-            if (!pieces) {
-                finish(sum, r);
+            if (!pieces && !p.has_prefix) {
+                sum.write(p.a, it.seq, head0 + r, lane);
             } else {
                 const int64_t at = part0 + static_cast<int64_t>(blockIdx.x) * rows + r;
                 const float inv = sum.l == 0.0f ? 0.0f : 1.0f / sum.l;
@@ -442,7 +454,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 if (lane == 0) p.w.part_lse[at] = sum.m + log2f(sum.l);
             }
         }
-        if (pieces) {   // the CTA that comes last joins them
+        if (pieces && !p.has_prefix) {   // the CTA that comes last joins them
             __threadfence();
             sync_consumers();
             if (threadIdx.x == 32) {
@@ -456,11 +468,40 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 for (int r = w; r < live_rows; r += 4) {
                     PartSum<DP> sum;
                     sum.add(p.w.part_lse, p.w.part_o, part0 + r, rows, it.c0, it.c1, lane);
-                    finish(sum, r);
+                    sum.write(p.a, it.seq, head0 + r, lane);
                 }
         }
         sync_consumers();   // the scratch may be written again
     }
+    // the join that follows reads the prefixes' results too: this kernel does not end before theirs
+    if (p.has_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// With prefixes: a row's own pieces and those of its group's prefix, one warp per (sequence, query head).
+template <int DP>
+__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ DecodeParams p) {
+    const AttnParams& a = p.a;
+    const int lane = threadIdx.x & 31, heads = a.rows.n_q_heads;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int s = static_cast<int>(i / heads), head = static_cast<int>(i % heads);
+    if (s >= a.batch.n_seqs) return;
+    const int g = find_sequence(a.prefix.group_offsets, a.prefix.n_groups, s, lane);
+    const int keys = checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, a.cache.page_shift, a.err, kErrKvLens);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int kv_head = head / p.group, sub = head % p.group, row_block = sub / kMaxRows;
+    const int chunk = *p.w.chunk, units = max((keys + kKeys * chunk - 1) / (kKeys * chunk), 1);
+    const int j = kv_head * p.plan.row_blocks + row_block;
+    const int64_t per = *p.w.units_per_cta, first = (s > 0 ? p.w.unit_end[s - 1] : 0) + static_cast<int64_t>(j) * units;
+    const int64_t item = static_cast<int64_t>(s) * a.cache.n_kv_heads * p.plan.row_blocks + j;
+    PartSum<DP> sum;
+    sum.add(p.w.part_lse, p.w.part_o, item * p.plan.rows + sub % kMaxRows, p.plan.rows, static_cast<int>(first / per),
+            static_cast<int>((first + units - 1) / per), lane);
+    if (g >= 0) {
+        const PieceSpan at = piece_span<true>(a, p.w.prefix, g, s, head, p.tile_tokens);
+        if (at.c0 <= at.c1)
+            sum.add(p.w.prefix.part_lse, p.w.prefix.part_o, at.base, kPartRows, at.c0, at.c1, lane);
+    }
+    sum.write(a, s, head, lane);
 }
 
 template <int DP>
@@ -491,7 +532,12 @@ cudaError_t launch_dim(DecodeParams& p, cudaStream_t stream) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = p.has_prefix ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, decode_kernel<DP>, q, k, v, p);
+    e = cudaLaunchKernelEx(&cfg, decode_kernel<DP>, q, k, v, p);
+    if (e != cudaSuccess || !p.has_prefix) return e;
+    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.a.batch.n_seqs) * p.a.rows.n_q_heads + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, decode_join_kernel<DP>, p);
 }
 
 }  // namespace
@@ -504,7 +550,7 @@ DecodePlan plan_decode(const AttnParams& a, int sms) {
     plan.dim = a.cache.head_dim <= 64 ? 64 : 128;
     plan.items = static_cast<int64_t>(a.batch.n_seqs) * a.cache.n_kv_heads * plan.row_blocks;
     const int64_t tiles = (static_cast<int64_t>(a.batch.max_pages) * a.cache.page_size + kKeys - 1) / kKeys;
-    plan.grid = static_cast<int>(std::min<int64_t>((plan.items * tiles + kMinUnits - 1) / kMinUnits, 2 * sms));
+    plan.grid = static_cast<int>(std::min<int64_t>(plan.items * tiles, 2 * sms));
     plan.part_rows = (plan.items + plan.grid) * plan.rows;
     return plan;
 }
