@@ -1,21 +1,23 @@
 // vw_prompt.cu -- attention of many rows over a paged key/value cache on the tensor cores (include/vwsampler.h):
 // vw_prompt_attention, and the shared prefixes of vw_decode_attention.
 //
-// out = softmax(scale Q K^T) V in one pass over the keys: a block of query rows keeps the running maximum m and sum l
-// of its scores in registers and its output O in tensor memory; a tile of 128 keys adds P V with P = exp2(c S - c m),
-// c = scale log2(e).  O and l are brought to a new maximum only when it has risen by more than 2^8 (P then stays below
-// 2^8, far inside bf16's and fp32's range, and the factor cancels in O / l), so O is hardly ever touched.
+// out = softmax(scale Q K^T) V in one pass over the keys: a block of query rows keeps a reference m and the sum l of its
+// probabilities in registers and its output O in tensor memory; a tile of 128 keys adds P V with P = exp2(c S - c m),
+// c = scale log2(e).  m is the maximum of the first keys a row sees.  It need not follow the running maximum: any m gives
+// the same O / l as long as nothing overflows, so m is raised, O and l brought to it and the tile done again only when
+// the tile's probabilities sum to more than 2^16.  That saves a pass over the scores in nearly every tile.
 //
 // A block is two tiles of up to 128 rows of one key head: the rows of a tile are (token, query head) pairs, so grouped
 // heads share every key and value read.  One CTA per SM, 12 warps:
-//   warp 0     schedules the blocks and loads by TMA: Q once per block, then K and V tiles (page boxes) into a ring;
-//   warp 1     one thread issues every tcgen05.mma: S = Q K^T (operands in shared memory) and O += P V (P from tensor
-//              memory); the two row tiles alternate, so one tile's products run while the other's softmax does;
+//   warp 0     schedules the blocks and loads by TMA: Q once per block, K and V tiles (page boxes) into two rings;
+//   warps 1, 3 issue the tcgen05.mma: S = Q K^T (operands in shared memory) and O += P V (P from tensor memory);
 //   warp 2     clears the rows past a sequence's last key in its last V tile (pages end inside a tile, and what lies
 //              there may be anything: 0 * NaN would reach every row);
-//   warps 4-7, 8-11   one warpgroup per row tile, one thread per row: S from tensor memory, maximum, exponentials, P
-//              back over S as bf16, and at the end O / l to the output.
-// Tensor memory (512 columns): S0 S1 (128 fp32 columns each, P over their first halves), O0 O1.
+//   warps 4-7, 8-11   one warpgroup per row tile, one thread per row: S from tensor memory into registers, exponentials,
+//              P back to tensor memory as bf16, and at the end O / l to the output.
+// Tensor memory (512 columns): one S (128 fp32 columns) that both row tiles use in turn, since the softmax warps read it
+// as soon as it is there; P0 P1 (64 each); O0 O1 (128 each).  So S of the next tile is computed while the softmax of this
+// one runs, and a row tile's time per key tile is its softmax alone.
 //
 // Schedule.  Blocks in order of decreasing key count from a ticket counter, so that the last ones are short.  Where
 // there are too few blocks for the SMs, the (block, tile) units are dealt evenly instead, a block's pieces leave
@@ -29,7 +31,6 @@
 #include <atomic>
 #include <cmath>
 #include <cstdint>
-#include <type_traits>
 
 #include "vw_attention.h"
 #include "vw_internal.h"
@@ -43,24 +44,27 @@ constexpr int kKeys = kTileKeys;  // keys per tile
 constexpr int kRows = kTileRows;  // rows per row tile
 constexpr int kWholeKeys = 512;   // sequences of at most this many keys are never split
 constexpr int kMinPromptUnits = 2, kMinPrefixUnits = 1;   // fewest units a CTA takes
-constexpr int kFeedRegs = 96, kSoftmaxRegs = 200;   // registers per thread of warps 0-3 and 4-11
-constexpr int kPolyPairs = 0;   // pairs of scores of every eight whose power of two is the polynomial
+constexpr int kFeedRegs = 72, kSoftmaxRegs = 208;   // registers per thread of warps 0-3 and 4-11
+// a tile whose probabilities sum to more is done again with its own maximum: far from what overflows in fp32 or bf16
+constexpr float kMaxTileSum = 65536.0f;
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;   // tensor memory columns: S; P0 P1, 64 each; O0 O1, 128 each
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr uint32_t kOutBytes = 32 * 128;   // a softmax warp's outputs on their way: 32 rows of 128 bytes
 constexpr int kItemSlots = 3;
-constexpr int kItemReaders = 10;  // MMA thread, warp 2, eight softmax warps
+constexpr int kItemReaders = 11;  // warps 1 to 11
 
 template <int DP>   // head_dim padded to 64 or 128 (the TMA fills the rest with zeros)
 struct TileCfg {
     static constexpr int kHalves = DP / 64;
     static constexpr uint32_t kHalfBytes = 128 * 128;   // 128 rows of 64 bf16, 128-byte swizzle
     static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
-    static constexpr int kStages = DP == 128 ? 4 : 8;
+    static constexpr int kStages = DP == 128 ? 2 : 4;   // of K, and of V
     static constexpr uint32_t kOffKv = 2 * kTileBytes;   // after the two Q tiles
-    static constexpr uint32_t kOffOut = kOffKv + kStages * kTileBytes;   // 4 KB per softmax warp
+    static constexpr uint32_t kOffOut = kOffKv + 2 * kStages * kTileBytes;   // 4 KB per softmax warp
     static constexpr uint32_t kOffBar = kOffOut + 8 * kOutBytes;
-    // kv_full[S] kv_empty[S] q_full q_empty s_full[2] p_full[2] o_full[2] v_tail v_fixed item_full[3] item_empty[3] done
-    static constexpr uint32_t kBars = 2 * kStages + 17;
+    // k_full[S] k_empty[S] v_full[S] v_empty[S] q_full q_empty s_full[2] s_free p_full[2] o_full[2] v_tail v_fixed
+    // item_full[3] item_empty[3] done[2]
+    static constexpr uint32_t kBars = 4 * kStages + 19;
     static constexpr uint32_t kOffItems = kOffBar + 8 * kBars;
     static constexpr uint32_t kOffMisc = kOffItems + kItemSlots * 64;
     static constexpr uint32_t kBytes = kOffMisc + 16;
@@ -268,16 +272,14 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float* f) {
           "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_store32(uint32_t addr, const float* f) {
-    const uint32_t* v = reinterpret_cast<const uint32_t*>(f);
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float* f) {
+    uint32_t* v = reinterpret_cast<uint32_t*>(f);
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
-        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-        "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-        "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+        "[%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(addr));
 }
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* v) {
     asm volatile(
@@ -301,27 +303,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "=f"(d.x), "=f"(d.y)
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
-}
-// 2^x of two values without the special-function unit: x = j + f with j the nearest integer (it lands in the low bits of
-// x + 1.5 * 2^23), 2^f by a polynomial of degree 5 on [-1/2, 1/2] with p(0) = 1 (a minimax fit of the relative error,
-// 1.9e-7 in fp32, as good as ex2.approx), and j added to the exponent.  Below 2^-126 it stays at 2^-126; a NaN gives
-// no NaN.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c);
-__device__ __forceinline__ float2 add2(float2 a, float2 b);
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    const auto both = [](float v) { return make_float2(v, v); };
-    x.x = fmaxf(x.x, -126.0f);
-    x.y = fmaxf(x.y, -126.0f);
-    const float2 t = add2(x, both(12582912.0f));
-    const float2 j = add2(t, both(-12582912.0f));
-    const float2 f = fma2(j, both(-1.0f), x);
-    float2 r = fma2(f, both(0.001326472731307149f), both(0.009671512991189957f));
-    r = fma2(r, f, both(0.05550733581185341f));
-    r = fma2(r, f, both(0.24022242426872253f));
-    r = fma2(r, f, both(0.6931470036506653f));
-    r = fma2(r, f, both(1.0f));
-    return make_float2(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(t.x) << 23)),
-                       __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(t.y) << 23)));
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if one is
     float d;
@@ -379,10 +360,11 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t sbase = s32(sm);
-    const uint32_t kv_full = sbase + C::kOffBar, kv_empty = kv_full + 8 * S;
-    const uint32_t q_full = kv_empty + 8 * S, q_empty = q_full + 8, s_full = q_empty + 8, p_full = s_full + 16,
-                   o_full = p_full + 16, v_tail = o_full + 16, v_fixed = v_tail + 8, item_full = v_fixed + 8,
-                   item_empty = item_full + 8 * kItemSlots, done = item_empty + 8 * kItemSlots;
+    const uint32_t k_full = sbase + C::kOffBar, k_empty = k_full + 8 * S, v_full = k_empty + 8 * S, v_empty = v_full + 8 * S;
+    const uint32_t q_full = v_empty + 8 * S, q_empty = q_full + 8, s_full = q_empty + 8, s_free = s_full + 16,
+                   p_full = s_free + 8, o_full = p_full + 16, v_tail = o_full + 16, v_fixed = v_tail + 8,
+                   item_full = v_fixed + 8, item_empty = item_full + 8 * kItemSlots, done = item_empty + 8 * kItemSlots;
+    const uint32_t k_smem = sbase + C::kOffKv, v_smem = k_smem + S * C::kTileBytes;
     Item* items = reinterpret_cast<Item*>(sm + C::kOffItems);   // 64 bytes apart
     auto item_slot = [&](uint32_t n) { return reinterpret_cast<Item*>(reinterpret_cast<uint8_t*>(items) + 64 * (n % kItemSlots)); };
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + C::kOffMisc);
@@ -394,7 +376,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     if (kPrefix) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
-        for (int s = 0; s < 2 * S; ++s) init(kv_full + 8 * s, 1);
+        for (int s = 0; s < 4 * S; ++s) init(k_full + 8 * s, 1);
         init(q_full, 1);
         init(q_empty, 1);
         for (int q = 0; q < 2; ++q) {
@@ -402,6 +384,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             init(p_full + 8 * q, 4);
             init(o_full + 8 * q, 1);
         }
+        init(s_free, 4);
         init(v_tail, 1);
         init(v_fixed, 1);
         for (int s = 0; s < kItemSlots; ++s) {
@@ -409,6 +392,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             init(item_empty + 8 * s, kItemReaders);
         }
         init(done, 1);
+        init(done + 8, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *abort = 0;
     }
@@ -436,14 +420,13 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const int32_t* tables = kPrefix ? p.a.prefix.page_table : p.a.batch.page_table;
             const int64_t table_stride = kPrefix ? p.a.prefix.page_table_stride : p.a.batch.page_table_stride;
             Scheduler<kPrefix> sched(p, lane);
-            uint32_t n_items = 0, n_q = 0, st = 0;
+            uint32_t n_items = 0, n_q = 0, st = 0, loaded_k = 0, loaded_v = 0;
             bool stop = false;
             Item it = sched.next(), following = it;
             for (; !stop; it = following) {
                 if (n_items >= kItemSlots &&
-                    !wait_bounded(item_empty + 8 * (n_items % kItemSlots), (n_items / kItemSlots - 1) & 1, abort, err))
-                    stop = true;
-                if (__any_sync(0xffffffffu, stop)) break;
+                    !wait_warp(item_empty + 8 * (n_items % kItemSlots), (n_items / kItemSlots - 1) & 1, abort, err))
+                    break;
                 if (lane == 0) {
                     *item_slot(n_items) = it;
                     arrive(item_full + 8 * (n_items % kItemSlots));
@@ -470,8 +453,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     return page;
                 };
                 int page = page_of(it.tile0);
-                if (n_q > 0 && !wait_bounded(q_empty, (n_q - 1) & 1, abort, err)) stop = true;
-                if (__any_sync(0xffffffffu, stop)) break;
+                if (n_q > 0 && !wait_warp(q_empty, (n_q - 1) & 1, abort, err)) break;
                 ++n_q;
                 if (lane == 0) {
                     const int tiles = it.end[1] > it.tile0 ? 2 : 1;   // row tile 1 sees at least row tile 0's keys
@@ -483,30 +465,31 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                             tma_load_3d(sbase + q * C::kTileBytes + h * C::kHalfBytes, &map_q, 64 * h, it.kv_head * p.group,
                                         it.row0 + q * p.tile_tokens, q_full);
                 }
-                for (int t = it.tile0; t < end && !stop; ++t) {
+                for (int t = it.tile0; t < end && !stop; ++t, ++st) {
                     const int next = page_of(t + 1);
-                    const uint32_t mine = __ballot_sync(0xffffffffu, page >= 0);
-                    const uint32_t bytes = __popc(mine) * box_rows * 128 * C::kHalves;
-    #pragma unroll
-                    for (int kv = 0; kv < 2; ++kv, ++st) {
-                        const uint32_t s = st % S;
-                        if (st >= S && !wait_bounded(kv_empty + 8 * s, (st / S - 1) & 1, abort, err)) stop = true;
-                        if (__any_sync(0xffffffffu, stop)) {
+                    const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, page >= 0)) * box_rows * 128 * C::kHalves;
+                    const uint32_t s = st % S;
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const uint32_t full = (kv ? v_full : k_full) + 8 * s, empty = (kv ? v_empty : k_empty) + 8 * s;
+                        if (st >= S && !wait_warp(empty, (st / S - 1) & 1, abort, err)) {
                             stop = true;
                             break;
                         }
                         if (lane == 0)
-                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(kv_full + 8 * s),
-                                         "r"(bytes)
+                            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "r"(bytes)
                                          : "memory");
                         __syncwarp();
                         if (page >= 0) {
                             const int token = (t * kKeys) & (cache.page_size - 1);
-    #pragma unroll
+#pragma unroll
                             for (int h = 0; h < C::kHalves; ++h)
-                                tma_load_4d(sbase + C::kOffKv + s * C::kTileBytes + h * C::kHalfBytes + lane * box_rows * 128,
-                                            kv ? &map_v : &map_k, 64 * h, token, it.kv_head, page, kv_full + 8 * s);
+                                tma_load_4d((kv ? v_smem : k_smem) + s * C::kTileBytes + h * C::kHalfBytes +
+                                                lane * box_rows * 128,
+                                            kv ? &map_v : &map_k, 64 * h, token, it.kv_head, page, full);
                         }
+                        if (kv) loaded_v = st + 1;
+                        else loaded_k = st + 1;
                     }
                     page = next;
                     // the next block is taken near the end of this one (early tickets would deal the blocks out as by turns)
@@ -516,19 +499,20 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             // teardown: the copies in flight land before the CTA may exit
             if (lane == 0) {
                 if (n_q > 0) drain_wait(q_full, (n_q - 1) & 1);
-                for (uint32_t j = st > S ? st - S : 0; j < st; ++j) drain_wait(kv_full + 8 * (j % S), (j / S) & 1);
+                for (uint32_t j = loaded_k > S ? loaded_k - S : 0; j < loaded_k; ++j) drain_wait(k_full + 8 * (j % S), (j / S) & 1);
+                for (uint32_t j = loaded_v > S ? loaded_v - S : 0; j < loaded_v; ++j) drain_wait(v_full + 8 * (j % S), (j / S) & 1);
             }
             __syncwarp();
-        } else if (warp == 1) {
-            // ---------------- matrix products: one thread issues them, the whole warp walks the loop, so that descriptors
-            // and addresses stay in uniform registers (computed in a divergent thread they cost ten cycles apiece to move
-            // there: 4700 cycles a tile pair, against 2048 for its products)
-            const bool leader = lane == 0;
+        } else if (warp & 1) {
+            // ---------------- matrix products: warp 1 issues S = Q K^T, warp 3 O += P V, one thread of each.  The whole warp
+            // walks the loop, so that descriptors and addresses stay in uniform registers (computed in a divergent thread
+            // they cost ten cycles apiece to move there, and the issue takes longer than the products).
+            const bool leader = lane == 0, scores = warp == 1;
             const int k_steps = (p.a.cache.head_dim + 15) / 16;       // of Q K^T
             const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((kRows >> 4) << 24);   // fp32 += bf16 x bf16
             const uint32_t idesc_pv = idesc | (1u << 16) | (static_cast<uint32_t>(2 * k_steps) << 17);   // V is N-major
             const uint32_t t0 = __shfl_sync(0xffffffffu, tmem, 0);
-            uint32_t st = 0, n_q = 0, n_p[2] = {0, 0}, n_fixed = 0;
+            uint32_t st = 0, n_q = 0, n_s = 0, n_p[2] = {0, 0}, n_fixed = 0;
             bool ok = true;
             for (uint32_t n = 0; ok; ++n) {
                 ok = wait_warp(item_full + 8 * (n % kItemSlots), (n / kItemSlots) & 1, abort, err);
@@ -538,67 +522,68 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 if (!it.valid) break;
                 const int end = max(it.end[0], it.end[1]);
                 if (end <= it.tile0) continue;
-                int seen[2];   // keys the tile's last row sees
+                int seen[2];   // keys the row tile's last row sees
 #pragma unroll
                 for (int q = 0; q < 2; ++q)
                     seen[q] = kPrefix ? it.kv : min(max(it.pos0 + min(it.tokens, (q + 1) * p.tile_tokens), 0), it.kv);
-                const int all = max(seen[0], seen[1]);
-                const bool fix = ((all + 15) & ~15) > it.kv;   // the last tile's value rows past it.kv are cleared
-                ok = wait_warp(q_full, n_q++ & 1, abort, err);
-                for (int t = it.tile0; t <= end && ok; ++t) {
-                    // tile t: S(t) after P V(t - 1), so that P's columns are free for S
-                    const uint32_t sk = st % S, sv = (st + S - 1) % S;   // stages of K(t) and V(t - 1)
-                    const uint32_t k0 = sbase + C::kOffKv + sk * C::kTileBytes, v0 = sbase + C::kOffKv + sv * C::kTileBytes;
-                    if (t > it.tile0) {
-                        ok = wait_warp(kv_full + 8 * sv, ((st - 1) / S) & 1, abort, err);
-                        if (ok && fix && t == (all + kKeys - 1) / kKeys) {
-                            arrive_if(leader, v_tail);   // V(t - 1) has landed: warp 2 may clear its tail
+                if (scores) {
+                    ok = wait_warp(q_full, n_q++ & 1, abort, err);
+                    for (int t = it.tile0; t < end && ok; ++t, ++st) {
+                        const uint32_t s = st % S;
+                        ok = wait_warp(k_full + 8 * s, (st / S) & 1, abort, err);
+                        const uint64_t bd = umma_desc(k_smem + s * C::kTileBytes);
+#pragma unroll
+                        for (int q = 0; q < 2; ++q)
+                            if (t < it.end[q]) {
+                                // the softmax warps have read the S before this one
+                                if (n_s > 0) ok = ok && wait_warp(s_free, (n_s - 1) & 1, abort, err);
+                                ++n_s;
+                                fence_after();
+                                const int n16 = (min(seen[q] - t * kKeys, kKeys) + 15) / 16;
+                                const uint32_t id = idesc | (static_cast<uint32_t>(2 * n16) << 17);
+                                const uint64_t ad = umma_desc(sbase + q * C::kTileBytes);
+#pragma unroll
+                                for (int k = 0; k < DP / 16; ++k) {   // 16 dims: 32 bytes along a row of 64
+                                    const uint32_t off = ((k >> 2) * C::kHalfBytes + 32 * (k & 3)) >> 4;
+                                    mma_ss(leader && ok && k < k_steps, t0 + kColS, ad + off, bd + off, id, k > 0 ? 1u : 0u);
+                                }
+                                mma_commit_if(leader && ok, s_full + 8 * q);
+                            }
+                        mma_commit_if(leader && ok, k_empty + 8 * s);
+                        mma_commit_if(leader && ok && t == end - 1, q_empty);
+                    }
+                } else {
+                    const int all = max(seen[0], seen[1]);
+                    const bool fix = ((all + 15) & ~15) > it.kv;   // the last tile's value rows past it.kv are cleared
+                    for (int t = it.tile0; t < end && ok; ++t, ++st) {
+                        const uint32_t s = st % S;
+                        ok = wait_warp(v_full + 8 * s, (st / S) & 1, abort, err);
+                        if (ok && fix && t == (all - 1) / kKeys) {
+                            arrive_if(leader, v_tail);   // V(t) has landed: warp 2 may clear its tail
                             ok = wait_warp(v_fixed, n_fixed++ & 1, abort, err);
                         }
-                    }
-                    if (ok && t < end) ok = wait_warp(kv_full + 8 * sk, (st / S) & 1, abort, err);
-                    if (!ok) break;
+                        const uint64_t vd = value_desc(v_smem + s * C::kTileBytes);
+                        const uint32_t later = t > it.tile0 ? 1u : 0u;
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        if (t > it.tile0 && t - 1 < it.end[q]) {
-                            ok = wait_warp(p_full + 8 * q, n_p[q]++ & 1, abort, err);
-                            if (!ok) break;
-                            fence_after();
-                            const int steps = (min(seen[q] - (t - 1) * kKeys, kKeys) + 15) / 16;
-                            const uint64_t vd = value_desc(v0);
-                            const uint32_t later = t - 1 > it.tile0 ? 1u : 0u;
+                        for (int q = 0; q < 2; ++q)
+                            if (t < it.end[q]) {
+                                ok = ok && wait_warp(p_full + 8 * q, n_p[q]++ & 1, abort, err);
+                                fence_after();
+                                const int steps = (min(seen[q] - t * kKeys, kKeys) + 15) / 16;
 #pragma unroll
-                            for (int k = 0; k < kKeys / 16; ++k)   // 16 keys: 16 rows of 128 bytes, 8 columns of P
-                                mma_ts(leader && k < steps, t0 + 256 + 128 * q, t0 + 128 * q + 8 * k, vd + k * (2048 >> 4),
-                                       idesc_pv, k > 0 ? 1u : later);
-                            if (t == it.end[q]) mma_commit_if(leader, o_full + 8 * q);
-                        }
-                        if (t < it.end[q]) {
-                            fence_after();
-                            const int n16 = (min(seen[q] - t * kKeys, kKeys) + 15) / 16;
-                            const uint32_t id = idesc | (static_cast<uint32_t>(2 * n16) << 17);
-                            const uint64_t ad = umma_desc(sbase + q * C::kTileBytes), bd = umma_desc(k0);
-#pragma unroll
-                            for (int k = 0; k < DP / 16; ++k) {   // 16 dims: 32 bytes along a row of 64
-                                const uint32_t off = ((k >> 2) * C::kHalfBytes + 32 * (k & 3)) >> 4;
-                                mma_ss(leader && k < k_steps, t0 + 128 * q, ad + off, bd + off, id, k > 0 ? 1u : 0u);
+                                for (int k = 0; k < kKeys / 16; ++k)   // 16 keys: 16 rows of 128 bytes, 8 columns of P
+                                    mma_ts(leader && ok && k < steps, t0 + kColO + 128 * q, t0 + kColP + 64 * q + 8 * k,
+                                           vd + k * (2048 >> 4), idesc_pv, k > 0 ? 1u : later);
+                                mma_commit_if(leader && ok, o_full + 8 * q);
                             }
-                            mma_commit_if(leader, s_full + 8 * q);
-                        }
-                    }
-                    if (!ok) break;
-                    if (t > it.tile0) mma_commit_if(leader, kv_empty + 8 * sv);
-                    if (t < end) {
-                        mma_commit_if(leader, kv_empty + 8 * sk);
-                        mma_commit_if(leader && t == end - 1, q_empty);
-                        st += 2;
+                        mma_commit_if(leader && ok, v_empty + 8 * s);
                     }
                 }
             }
             // teardown: every product issued has completed before the tensor memory is freed
             if (leader) {
-                mma_commit(done);
-                drain_wait(done, 0);
+                mma_commit(done + 8 * (warp >> 1));
+                drain_wait(done + 8 * (warp >> 1), 0);
             }
             __syncwarp();
         } else if (warp == 2) {
@@ -615,21 +600,20 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const int all = kPrefix ? it.kv : min(max(it.pos0 + it.tokens, 0), it.kv);
                 const int upto = (all + 15) & ~15;
                 if (upto > it.kv && end == (all + kKeys - 1) / kKeys) {
-                    const uint32_t j = st + 2 * (end - 1 - it.tile0) + 1, s = j % S;   // the stage of V(end - 1)
-                    // (its own phase of kv_full: the stage is not released before v_fixed)
-                    if (!wait_warp(v_tail, n_fixed++ & 1, abort, err) ||
-                        !wait_warp(kv_full + 8 * s, (j / S) & 1, abort, err))
+                    const uint32_t j = st + (end - 1 - it.tile0), s = j % S;   // the stage of V(end - 1)
+                    // (its own phase of v_full: the stage is not released before v_fixed)
+                    if (!wait_warp(v_tail, n_fixed++ & 1, abort, err) || !wait_warp(v_full + 8 * s, (j / S) & 1, abort, err))
                         break;
                     const int r0 = it.kv - (end - 1) * kKeys, rows = upto - it.kv;
                     for (int h = 0; h < C::kHalves; ++h)
                         for (int i = lane; i < rows * 8; i += 32)
-                            *reinterpret_cast<uint4*>(sm + C::kOffKv + s * C::kTileBytes + h * C::kHalfBytes + r0 * 128 +
+                            *reinterpret_cast<uint4*>(sm + (v_smem - sbase) + s * C::kTileBytes + h * C::kHalfBytes + r0 * 128 +
                                                       16 * i) = make_uint4(0, 0, 0, 0);
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // visible to the products
                     __syncwarp();
                     if (lane == 0) arrive(v_fixed);
                 }
-                st += 2 * (end - it.tile0);
+                st += end - it.tile0;
             }
         }
     } else {
@@ -638,10 +622,12 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const int q = (warp - 4) >> 2;
         const int row = 32 * (warp & 3) + lane;
         const uint32_t quarter = static_cast<uint32_t>(32 * (warp & 3)) << 16;
-        const uint32_t t_s = tmem + quarter + 128 * q, t_o = tmem + quarter + 256 + 128 * q;
+        const uint32_t t_s = tmem + quarter + kColS, t_p = tmem + quarter + kColP + 64 * q,
+                       t_o = tmem + quarter + kColO + 128 * q;
         const int token = q * p.tile_tokens + row / p.group, sub = row % p.group;
         const bool in_tile = row < p.tile_tokens * p.group;
-        const float2 c2 = make_float2(p.c, p.c);
+        const float c = p.c;
+        const float2 c2 = make_float2(c, c);
         uint32_t n_s = 0, n_o = 0;
         bool stop = false;
         for (uint32_t n = 0; !stop; ++n) {
@@ -650,6 +636,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             __syncwarp();
             if (lane == 0) arrive(item_empty + 8 * (n % kItemSlots));
             if (!it.valid) break;
+            bool ok = true;
             const bool live = in_tile && token < it.tokens;
             const int limit = !live ? 0 : kPrefix ? it.kv : min(it.pos0 + token + 1, it.kv);   // keys this row sees
             const bool any_live = __any_sync(0xffffffffu, live);
@@ -660,83 +647,99 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     break;
                 }
                 fence_after();
+                float s[kKeys];
                 if (any_live) {
-                    float s[kKeys];
 #pragma unroll
                     for (int i = 0; i < kKeys; i += 32) tmem_load32(t_s + i, s + i);
                     tmem_wait_load();
+                }
+                fence_before();
+                __syncwarp();
+                arrive_if(lane == 0, s_free);   // the next S may be written
+                if (any_live) {
                     if (p.negate) {
 #pragma unroll
                         for (int i = 0; i < kKeys; ++i) s[i] = -s[i];
                     }
                     const int columns = limit - t * kKeys;
-                    const bool masked = !__all_sync(0xffffffffu, columns >= kKeys || !live);
-                    if (masked) {
+                    if (!__all_sync(0xffffffffu, columns >= kKeys || !live)) {
 #pragma unroll
                         for (int i = 0; i < kKeys; ++i) s[i] = i < columns ? s[i] : -INFINITY;
                     }
-                    float top[4];
+                    const auto row_max = [&] {   // NaN if a score is
+                        float top[4];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) top[j] = max3(s[j], s[4 + j], s[8 + j]);
+                        for (int j = 0; j < 4; ++j) top[j] = max3(s[j], s[4 + j], s[8 + j]);
 #pragma unroll
-                    for (int i = 12; i + 8 <= kKeys; i += 8)
+                        for (int i = 12; i + 8 <= kKeys; i += 8)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
-                    static_assert((kKeys - 12) % 8 == 4, "the last four scores are left");
-                    const float tile_max = max3(max3(top[0], s[kKeys - 4], s[kKeys - 3]),
-                                                max3(top[1], s[kKeys - 2], s[kKeys - 1]), max3(top[2], top[3], top[3]));
-                    // a first maximum is taken as it is (nothing but zeros was summed); a later one when it rose enough
-                    const bool rise = live && m != -INFINITY && (tile_max - m) * p.c > 8.0f;
-                    if (__any_sync(0xffffffffu, rise)) {   // products up to t - 1 are done: S(t) came after them
-                        const float f = rise ? exp2_fast((m - tile_max) * p.c) : 1.0f;
-                        l *= f;
-                        if (rise) m = tile_max;
-#pragma unroll 1
-                        for (int i = 0; i < DP; i += 32) {
-                            float o[32];
-                            tmem_load32(t_o + i, o);
-                            tmem_wait_load();
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) o[j] *= f;
-                            tmem_store32(t_o + i, o);
-                        }
-                        tmem_wait_store();
+                            for (int j = 0; j < 4; ++j) top[j] = max3(top[j], s[i + j], s[i + 4 + j]);
+                        static_assert((kKeys - 12) % 8 == 4, "the last four scores are left");
+                        return max3(max3(top[0], s[kKeys - 4], s[kKeys - 3]), max3(top[1], s[kKeys - 2], s[kKeys - 1]),
+                                    max3(top[2], top[3], top[3]));
+                    };
+                    // The first keys a row sees set m to their maximum; later ones are taken relative to it as it is, and m
+                    // is raised (and the tile done again) only when their sum shows that they are far above it.
+                    if (__any_sync(0xffffffffu, m == -INFINITY)) {
+                        const float top = row_max();
+                        if (m == -INFINITY) m = top;
                     }
-                    if (m == -INFINITY || tile_max != tile_max) m = tile_max;   // a NaN score makes the row NaN
-                    const float mc = m == -INFINITY ? 0.0f : -m * p.c;
-                    const float2 mc2 = make_float2(mc, mc);
-                    float2 sum[4] = {};
-                    // P = 2^(c S - c m); `poly` pairs of every eight by the polynomial (a tile with masked scores: none)
-                    const auto probabilities = [&](auto poly) {
+                    // P V(t - 1) is done: P may be written, and O brought to a new maximum
+                    if (t > it.tile0) ok = spin_warp(o_full + 8 * q, n_o++ & 1, abort, err);
+                    fence_after();
+                    float tile_sum;
+                    for (bool again = false;; again = true) {
+                        const float mc = m == -INFINITY ? 0.0f : -m * c;
+                        const float2 mc2 = make_float2(mc, mc);
+                        float2 sum[4] = {};
 #pragma unroll
                         for (int i = 0; i < kKeys; i += 32) {
-                            float2 e[16];
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                e[j] = fma2(make_float2(s[i + 2 * j], s[i + 2 * j + 1]), c2, mc2);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                e[j] = (j * 3) % 8 < decltype(poly)::value ? exp2_poly(e[j])
-                                                                           : make_float2(exp2_fast(e[j].x), exp2_fast(e[j].y));
                             uint32_t pk[16];   // the product's operand; the sum keeps fp32
 #pragma unroll
-                            for (int j = 0; j < 16; ++j) pk[j] = pack_bf16(e[j].x, e[j].y);
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) sum[j & 3] = add2(sum[j & 3], e[j]);
-                            tmem_store16(t_s + (i >> 1), pk);
+                            for (int j = 0; j < 16; ++j) {
+                                const float2 x = fma2(make_float2(s[i + 2 * j], s[i + 2 * j + 1]), c2, mc2);
+                                const float2 e = make_float2(exp2_fast(x.x), exp2_fast(x.y));
+                                sum[j & 3] = add2(sum[j & 3], e);
+                                pk[j] = pack_bf16(e.x, e.y);
+                            }
+                            tmem_store16(t_p + (i >> 1), pk);
                         }
-                    };
-                    if (masked)
-                        probabilities(std::integral_constant<int, 0>{});
-                    else
-                        probabilities(std::integral_constant<int, kPolyPairs>{});
-                    const float2 both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
-                    l += both.x + both.y;
+                        const float2 both = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                        tile_sum = both.x + both.y;
+                        const bool rise = live && !(tile_sum <= kMaxTileSum);   // (or not a number)
+                        if (again || !__any_sync(0xffffffffu, rise)) break;
+                        float f = 1.0f;
+                        if (rise) {
+                            const float top = row_max();
+                            f = exp2_fast((m - top) * c);
+                            m = top;
+                        }
+                        l *= f;
+                        if (t > it.tile0) {
+#pragma unroll 1
+                            for (int d = 0; d < DP; d += 16) {
+                                float o[16];
+                                tmem_load16(t_o + d, o);
+                                tmem_wait_load();
+#pragma unroll
+                                for (int j = 0; j < 16; ++j) o[j] *= f;
+                                tmem_store16(t_o + d, reinterpret_cast<const uint32_t*>(o));
+                            }
+                        }
+                    }
+                    l += tile_sum;
                     tmem_wait_store();
+                } else if (t > it.tile0) {
+                    ok = wait_warp(o_full + 8 * q, n_o++ & 1, abort, err);
+                    fence_after();
+                }
+                if (!ok) {
+                    stop = true;
+                    break;
                 }
                 fence_before();
                 __syncwarp();
-                if (lane == 0) arrive(p_full + 8 * q);
+                arrive_if(lane == 0, p_full + 8 * q);
             }
             if (stop) break;
             const bool some = it.end[q] > it.tile0;

@@ -50,6 +50,20 @@ __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatil
     if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
     return __all_sync(0xffffffffu, wait_bounded(bar, parity, abort, err));
 }
+// the same without a call (where registers are full, a call would spill them)
+__device__ __forceinline__ bool spin_warp(uint32_t bar, uint32_t parity, volatile int32_t* abort, unsigned* err) {
+    if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
+    const uint64_t t0 = now_ns();
+    for (;;) {
+        if (__all_sync(0xffffffffu, try_wait(bar, parity))) return true;
+        const bool late = now_ns() - t0 > kWaitLimitNs;
+        if (__any_sync(0xffffffffu, late || *abort)) {
+            if (late) atomicOr(err, kErrTimeout);
+            *abort = 1;
+            return false;
+        }
+    }
+}
 // teardown flavour: bounded, no error reporting (an abort is already recorded)
 static __device__ void drain_wait(uint32_t bar, uint32_t parity) {
     const uint64_t t0 = now_ns();
