@@ -763,50 +763,41 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 else if (p.a.rows.lse)
                     p.a.rows.lse[call_row * p.a.rows.n_q_heads + head] = lse * kLn2;
             }
-            // O / l through shared memory (16-byte pieces of a row at piece ^ (row & 7)), so that eight lanes write 128
-            // bytes of one row: a lane storing its own row touches 32 lines an instruction
+            // O / l through shared memory, 32 columns at a time (16-byte piece j of row r at j ^ (r & 7)), so that the lanes
+            // write 64 (bf16) or 128 (partial fp32) bytes of one row together: a lane storing its own row touches 32 lines
+            // an instruction.  Short loops: this runs once a block, and its instructions come from far away.
             uint8_t* mine = sm + C::kOffOut + (warp - 4) * kOutBytes;
-            const uint64_t out_row =
-                reinterpret_cast<uint64_t>(p.a.rows.out + call_row * p.a.rows.out_row + head * p.a.rows.out_head);
-            const int width = part ? 32 : 64;   // columns of 128 bytes
+            const uint64_t to = part ? reinterpret_cast<uint64_t>(p.w.part_o + (part0 + row) * DP)
+                                     : reinterpret_cast<uint64_t>(p.a.rows.out + call_row * p.a.rows.out_row +
+                                                                  head * p.a.rows.out_head);
+            const int shift = part ? 3 : 2;   // log2 of the lanes that share a row
+            const int piece = lane & ((1 << shift) - 1);
 #pragma unroll 1
-            for (int c0 = 0; c0 < D; c0 += width) {
+            for (int c0 = 0; c0 < D; c0 += 32) {
                 float o[32];
+                tmem_load32(t_o + c0, o);
+                tmem_wait_load();
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (half == 1 && part) break;
-                    if (some) {
-                        tmem_load32(t_o + c0 + 32 * half, o);
-                        tmem_wait_load();
-                    }
+                for (int j = 0; j < 32; ++j) o[j] = some ? o[j] * r : 0.0f;
+                if (part) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) o[j] = some ? o[j] * r : 0.0f;
-                    if (part) {
+                    for (int j = 0; j < 8; ++j)
+                        *reinterpret_cast<float4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                            make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                } else {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            *reinterpret_cast<float4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                                make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            *reinterpret_cast<uint4*>(mine + lane * 128 + (((4 * half + j) ^ (lane & 7)) << 4)) =
-                                make_uint4(pack_bf16(o[8 * j], o[8 * j + 1]), pack_bf16(o[8 * j + 2], o[8 * j + 3]),
-                                           pack_bf16(o[8 * j + 4], o[8 * j + 5]), pack_bf16(o[8 * j + 6], o[8 * j + 7]));
-                    }
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<uint4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+                            make_uint4(pack_bf16(o[8 * j], o[8 * j + 1]), pack_bf16(o[8 * j + 2], o[8 * j + 3]),
+                                       pack_bf16(o[8 * j + 4], o[8 * j + 5]), pack_bf16(o[8 * j + 6], o[8 * j + 7]));
                 }
                 __syncwarp();
-                const int piece = lane & 7;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int rr = 4 * i + (lane >> 3);
+                const bool inside = part || c0 + 8 * piece < D;
+#pragma unroll 1
+                for (int rr = lane >> shift; rr < 32; rr += 32 >> shift) {
                     const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * 128 + ((piece ^ (rr & 7)) << 4));
-                    const uint64_t base = __shfl_sync(0xffffffffu, out_row, rr);
-                    const int tile_row = 32 * (warp & 3) + rr;
-                    if (tile_row >= live_rows) continue;
-                    if (part)
-                        *reinterpret_cast<uint4*>(p.w.part_o + (part0 + tile_row) * DP + c0 + 4 * piece) = v;
-                    else if (c0 + 8 * piece < D)
-                        *reinterpret_cast<uint4*>(base + 2 * (c0 + 8 * piece)) = v;
+                    const uint64_t at = __shfl_sync(0xffffffffu, to, rr) + (part ? 4 : 2) * c0 + 16 * piece;
+                    if (inside && 32 * (warp & 3) + rr < live_rows) *reinterpret_cast<uint4*>(at) = v;
                 }
                 __syncwarp();
             }
