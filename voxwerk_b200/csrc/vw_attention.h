@@ -111,7 +111,7 @@ cudaError_t launch_prompt_attention(const AttnParams& p, const TilePlan& plan, c
 
 // ---- the decode kernel (vw_decode.cu)
 struct DecodePlan {
-    int32_t grid;
+    int32_t grid, sms;
     int32_t rows;               // query heads an item takes: min(group, 16)
     int32_t row_blocks;         // items per key head
     int32_t dim;
@@ -208,6 +208,11 @@ __device__ __forceinline__ int64_t seq_units(const Seq& q, int block_tokens, int
     return u * kv_heads;
 }
 
+// a / b, by 32-bit division where both fit (the 64-bit one takes some hundred instructions)
+__device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
 __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusive
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -215,6 +220,31 @@ __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusi
         if (lane >= o) x += y;
     }
     return x;
+}
+
+// SMs for the prefixes' tile kernel; the decode kernel, launched behind it, takes the others at once (all when this is
+// all, after the prefixes).  It is bound by HBM and reaches that rate with some 80 of 148 SMs, the prefixes by the SMs, so
+// the two overlap well.  Of 32 counts the one whose later end comes first, by what was measured of each: 12 us and then
+// 1.6 us a unit for a prefix CTA (17 us and 2.45 us where blocks have two row tiles); 8 us, then 64-key tiles at 6.5 TB/s
+// or 0.5 us each on an SM, for the sequences' own keys.  Every CTA of both kernels comes to the same count.
+__device__ __forceinline__ int prefix_ctas(const AttnParams& a, int64_t units, int sms, int lane) {
+    const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
+    int tiles = 0;
+    for (int s = lane; s < a.batch.n_seqs; s += 32)
+        tiles += ceil_div(checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, a.cache.page_shift, a.err,
+                                      kErrKvLens), 64);
+    const float own_tiles = static_cast<float>(__reduce_add_sync(0xffffffffu, tiles)) *
+                            (a.cache.n_kv_heads * ((group + 15) / 16));
+    const int mine = (sms * (lane + 1)) >> 5;
+    const bool two = a.batch.n_seqs * group > kTileRows;
+    const float prefix_us = (two ? 17.0f : 12.0f) + static_cast<float>(units) * (two ? 2.45f : 1.6f) / static_cast<float>(mine);
+    const float hbm_us = own_tiles * (256.0f * a.cache.head_dim) / 6.5e6f;
+    const int rest = mine < sms ? sms - mine : sms;
+    const float own_us = 8.0f + fmaxf(hbm_us, own_tiles * 0.5f / static_cast<float>(rest));
+    const float us = mine == 0 ? 1e30f : mine < sms ? fmaxf(prefix_us, own_us) : prefix_us + own_us;
+    const unsigned best = __reduce_min_sync(0xffffffffu, __float_as_uint(us));   // (positive floats order as integers)
+    const unsigned m = __ballot_sync(0xffffffffu, __float_as_uint(us) == best);
+    return (sms * (32 - __clz(m))) >> 5;
 }
 
 // Where the pieces of one row's block are: piece c (of CTA c) at partial row base + c * kPartRows, c0 <= c <= c1; c0 > c1
@@ -239,8 +269,8 @@ __device__ PieceSpan piece_span(const AttnParams& a, const TileWork& w, int s, i
         for (int j = 0; j < i; ++j) first += static_cast<int64_t>(kv_heads) * block_units<kPrefix>(q, j, block_tokens);
     first += static_cast<int64_t>(kv_head) * cost;
     const int64_t per = *w.units_per_cta;
-    at.c0 = static_cast<int>(first / per);
-    at.c1 = static_cast<int>((first + cost - 1) / per);
+    at.c0 = static_cast<int>(divide(first, per));
+    at.c1 = static_cast<int>(divide(first + cost - 1, per));
     const int tokens = min(block_tokens, q.n - i * block_tokens);
     at.base = static_cast<int64_t>(q.row0) * heads + static_cast<int64_t>(i) * kv_heads * block_tokens * group +
               static_cast<int64_t>(kv_head) * tokens * group + (row - q.row0 - i * block_tokens) * group + head % group;

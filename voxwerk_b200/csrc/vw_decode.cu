@@ -72,7 +72,7 @@ struct DecodeParams {
     AttnParams a;
     DecodePlan plan;
     DecodeWork w;
-    int32_t group, tile_tokens, stages, negate, boxes, has_prefix;
+    int32_t group, tile_tokens, stages, negate, boxes, has_prefix, sms;
     float c;
 };
 
@@ -172,19 +172,29 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         };
         // A unit is `chunk` tiles of an item (an item without keys has one, to be written).  Few items: as many tiles as
         // give every CTA one unit at most, so that none has the ends of two items; else one tile.
-        int64_t total_tiles = 0;
-        for (int s = lane; s < n_seqs; s += 32) total_tiles += max((keys_of(s) + kKeys - 1) / kKeys, 1);
-        total_tiles = __shfl_sync(0xffffffffu, warp_scan(total_tiles, lane), 31) * per_seq;
-        const int64_t spare = static_cast<int64_t>(gridDim.x) - p.plan.items;
-        const int chunk = 2 * spare >= gridDim.x ? static_cast<int>(max((total_tiles + spare - 1) / spare, int64_t{1})) : 1;
+        // (the sequences' tiles together fit 32 bits: 2^31 of them would be 2^37 keys)
+        int sum_tiles = 0;
+        for (int s = lane; s < n_seqs; s += 32) sum_tiles += max((keys_of(s) + kKeys - 1) / kKeys, 1);
+        const int64_t total_tiles = static_cast<int64_t>(__reduce_add_sync(0xffffffffu, sum_tiles)) * per_seq;
+        int ctas = gridDim.x;
+        if (p.has_prefix) {   // the prefixes' SMs are not there yet: the CTAs that come to them later have no units
+            int64_t units = 0;
+            for (int g = lane; g < a.prefix.n_groups; g += 32)
+                units += seq_units<true>(load_seq<true>(a, g), 2 * p.tile_tokens, cache.n_kv_heads);
+            units = __shfl_sync(0xffffffffu, warp_scan(units, lane), 31);
+            const int taken = prefix_ctas(a, units, p.sms, lane);
+            if (taken < p.sms) ctas = min(ctas, 2 * (p.sms - taken));
+        }
+        const int64_t spare = static_cast<int64_t>(ctas) - p.plan.items;
+        const int chunk = 2 * spare >= ctas ? static_cast<int>(max(divide(total_tiles + spare - 1, spare), int64_t{1})) : 1;
         auto units_of = [&](int keys) { return max((keys + kKeys * chunk - 1) / (kKeys * chunk), 1); };
         int64_t total = total_tiles;
         if (chunk > 1) {
-            total = 0;
-            for (int s = lane; s < n_seqs; s += 32) total += units_of(keys_of(s));
-            total = __shfl_sync(0xffffffffu, warp_scan(total, lane), 31) * per_seq;
+            int sum = 0;
+            for (int s = lane; s < n_seqs; s += 32) sum += units_of(keys_of(s));
+            total = static_cast<int64_t>(__reduce_add_sync(0xffffffffu, sum)) * per_seq;
         }
-        const int64_t per = (total + gridDim.x - 1) / gridDim.x;
+        const int64_t per = divide(total + ctas - 1, ctas);
         int64_t unit = min(per * blockIdx.x, total);
         const int64_t unit_end = min(unit + per, total);
         int64_t first = 0;   // the first unit of sequence `seq`
@@ -225,7 +235,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     keys = keys_of(++seq);
                     units = units_of(keys);
                 }
-                const int j = static_cast<int>((unit - first) / units);
+                const int j = static_cast<int>(divide(unit - first, units));
                 const int64_t item_first = first + static_cast<int64_t>(j) * units;
                 const int tiles = max((keys + kKeys - 1) / kKeys, 1);
                 const int u0 = static_cast<int>(unit - item_first);
@@ -236,8 +246,8 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 it.keys = keys;
                 it.tile0 = u0 * chunk;
                 it.tile1 = min(u1 * chunk, tiles);
-                it.c0 = static_cast<int>(item_first / per);
-                it.c1 = static_cast<int>((item_first + units - 1) / per);
+                it.c0 = static_cast<int>(divide(item_first, per));
+                it.c1 = static_cast<int>(divide(item_first + units - 1, per));
                 it.index = seq * per_seq + j;
                 unit = item_first + u1;
             }
@@ -494,8 +504,8 @@ __global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant_
     const int64_t per = *p.w.units_per_cta, first = (s > 0 ? p.w.unit_end[s - 1] : 0) + static_cast<int64_t>(j) * units;
     const int64_t item = static_cast<int64_t>(s) * a.cache.n_kv_heads * p.plan.row_blocks + j;
     PartSum<DP> sum;
-    sum.add(p.w.part_lse, p.w.part_o, item * p.plan.rows + sub % kMaxRows, p.plan.rows, static_cast<int>(first / per),
-            static_cast<int>((first + units - 1) / per), lane);
+    sum.add(p.w.part_lse, p.w.part_o, item * p.plan.rows + sub % kMaxRows, p.plan.rows, static_cast<int>(divide(first, per)),
+            static_cast<int>(divide(first + units - 1, per)), lane);
     if (g >= 0) {
         const PieceSpan at = piece_span<true>(a, p.w.prefix, g, s, head, p.tile_tokens);
         if (at.c0 <= at.c1)
@@ -545,6 +555,7 @@ cudaError_t launch_dim(DecodeParams& p, cudaStream_t stream) {
 DecodePlan plan_decode(const AttnParams& a, int sms) {
     const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
     DecodePlan plan{};
+    plan.sms = sms;
     plan.rows = std::min(group, kMaxRows);
     plan.row_blocks = (group + kMaxRows - 1) / kMaxRows;
     plan.dim = a.cache.head_dim <= 64 ? 64 : 128;
@@ -558,7 +569,7 @@ DecodePlan plan_decode(const AttnParams& a, int sms) {
 cudaError_t launch_decode_attention(const AttnParams& a, const DecodePlan& plan, const DecodeWork& w, cudaStream_t stream) {
     const Geometry g = geometry(a);
     DecodeParams p{a, plan, w, g.group, g.tile_tokens, 0, a.rows.scale < 0.0f,
-                   a.cache.page_size >= kKeys ? 1 : kKeys / a.cache.page_size, a.prefix.n_groups > 0,
+                   a.cache.page_size >= kKeys ? 1 : kKeys / a.cache.page_size, a.prefix.n_groups > 0, plan.sms,
                    exp2_scale(a.rows.scale)};
     return plan.dim == 64 ? launch_dim<64>(p, stream) : launch_dim<128>(p, stream);
 }

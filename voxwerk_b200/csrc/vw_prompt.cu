@@ -138,34 +138,37 @@ struct Scheduler {
         block_tokens = 2 * p.tile_tokens;
         kv_heads = p.a.cache.n_kv_heads;
         if (p.split) {
-            int64_t total = 0;
+            const auto units_of = [&](int s) {
+                return s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p.a, s), block_tokens, kv_heads) : 0;
+            };
+            int64_t total = 0, u = 0, sum = 0;
             for (int s0 = 0; s0 < n_seqs; s0 += 32) {
                 const int s = s0 + lane;
-                int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p.a, s), block_tokens, kv_heads) : 0;
-                u = warp_scan(u, lane);
-                if (blockIdx.x == 0 && s < n_seqs) p.w.unit_end[s] = total + u;   // for the kernels that join
-                total += __shfl_sync(0xffffffffu, u, 31);
+                u = units_of(s);
+                sum = warp_scan(u, lane);
+                if (blockIdx.x == 0 && s < n_seqs) p.w.unit_end[s] = total + sum;   // for the kernels that join
+                total += __shfl_sync(0xffffffffu, sum, 31);
             }
-            const int64_t per = max((total + gridDim.x - 1) / gridDim.x, static_cast<int64_t>(p.min_units));
+            const int ctas = kPrefix ? prefix_ctas(p.a, total, gridDim.x, lane) : gridDim.x;
+            const int64_t per = max(divide(total + ctas - 1, ctas), static_cast<int64_t>(p.min_units));
             if (blockIdx.x == 0 && lane == 0) *p.w.units_per_cta = per;
             unit = min(per * blockIdx.x, total);
             unit_end = min(unit + per, total);
             seq = 0;
             seq_first = 0;
-            if (unit < unit_end) {   // the sequence that holds `unit`
-                for (int s0 = 0; s0 < n_seqs; s0 += 32) {
-                    const int s = s0 + lane;
-                    const int64_t u = s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p.a, s), block_tokens, kv_heads) : 0;
-                    const int64_t sum = warp_scan(u, lane);
-                    const unsigned m = __ballot_sync(0xffffffffu, seq_first + sum > unit);
-                    if (m) {
-                        const int at = __ffs(m) - 1;
-                        seq = s0 + at;
-                        seq_first += __shfl_sync(0xffffffffu, sum - u, at);
-                        break;
-                    }
-                    seq_first += __shfl_sync(0xffffffffu, sum, 31);
+            for (int s0 = 0; unit < unit_end && s0 < n_seqs; s0 += 32) {   // the sequence that holds `unit`
+                if (n_seqs > 32) {   // (else the values above)
+                    u = units_of(s0 + lane);
+                    sum = warp_scan(u, lane);
                 }
+                const unsigned m = __ballot_sync(0xffffffffu, seq_first + sum > unit);
+                if (m) {
+                    const int at = __ffs(m) - 1;
+                    seq = s0 + at;
+                    seq_first += __shfl_sync(0xffffffffu, sum - u, at);
+                    break;
+                }
+                seq_first += __shfl_sync(0xffffffffu, sum, 31);
             }
         } else {
             ticket = blockIdx.x;
@@ -235,7 +238,7 @@ struct Scheduler {
         int i = 0, cost;
         if (kPrefix) {
             cost = block_units<kPrefix>(q, 0, block_tokens);
-            i = static_cast<int>((unit - first) / (static_cast<int64_t>(cost) * kv_heads));
+            i = static_cast<int>(divide(unit - first, static_cast<int64_t>(cost) * kv_heads));
             first += static_cast<int64_t>(i) * cost * kv_heads;
         } else {
             for (;; ++i) {
@@ -244,7 +247,7 @@ struct Scheduler {
                 first += static_cast<int64_t>(cost) * kv_heads;
             }
         }
-        const int kv_head = static_cast<int>((unit - first) / cost);
+        const int kv_head = static_cast<int>(divide(unit - first, cost));
         first += static_cast<int64_t>(kv_head) * cost;
         const int t0 = static_cast<int>(unit - first);
         const int t1 = static_cast<int>(min(unit_end - first, static_cast<int64_t>(cost)));
