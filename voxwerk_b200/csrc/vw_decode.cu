@@ -32,6 +32,7 @@ constexpr int kThreads = 160;     // producer warp, four warps of 16 keys
 constexpr int kKeys = 64;         // keys per tile
 constexpr int kMaxRows = 16;      // query heads per item: the rows of an mma
 constexpr int kItemSlots = 2;
+constexpr float kLn2 = 0.693147180559945309f;
 constexpr uint32_t kSmemBudget = 113 * 1024;   // two CTAs per SM
 
 template <int DP>
@@ -110,16 +111,6 @@ __device__ __forceinline__ bool any_failed(bool ok) {
         : "r"(ok ? 0 : 1)
         : "memory");
     return r != 0;
-}
-
-// One row's sums of one warp: m, l and O (not divided), as PartSum keeps them
-template <int DIM>
-__device__ __forceinline__ void add_raw(PartSum<DIM>& s, float m, float l, const float* o) {
-    s.raise(m);
-    const float f = s.m == -INFINITY ? 0.0f : exp2f(m - s.m);
-    s.l = __fmaf_rn(f, l, s.l);
-#pragma unroll
-    for (int d = 0; d < PartSum<DIM>::kDims; ++d) s.o[d] = __fmaf_rn(f, o[d], s.o[d]);
 }
 
 template <int DP>
@@ -444,24 +435,38 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         const bool pieces = it.c0 != it.c1;
         const int head0 = it.kv_head * p.group + it.row_block * kMaxRows;
         const int64_t part0 = static_cast<int64_t>(it.index) * rows;   // piece c at + c * rows
-        for (int r = w; r < live_rows; r += 4) {
-            PartSum<DP> sum;
+        for (int i = threadIdx.x - 32; i < live_rows * (DP / 2); i += 128) {   // a thread: two dims of a row
+            const int r = i / (DP / 2), d = 2 * (i % (DP / 2));
+            float2 ml[4];
+            float top = -INFINITY, sum = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 ml = scratch_ml[i * rows + r];
-                float x[PartSum<DP>::kDims];
-#pragma unroll
-                for (int d = 0; d < PartSum<DP>::kDims; ++d) x[d] = scratch_o[(i * rows + r) * DP + lane * PartSum<DP>::kDims + d];
-                add_raw(sum, ml.x, ml.y, x);
+            for (int k = 0; k < 4; ++k) {
+                ml[k] = scratch_ml[k * rows + r];
+                top = fmaxf(top, ml[k].x);
             }
+            float2 x = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // (no key: weight 0; a NaN reference or sum makes the row NaN)
+                const float f = ml[k].x == -INFINITY ? 0.0f : exp2_fast(ml[k].x - top);
+                const float2 y = *reinterpret_cast<const float2*>(scratch_o + (k * rows + r) * DP + d);
+                sum = __fmaf_rn(f, ml[k].y, sum);
+                x.x = __fmaf_rn(f, y.x, x.x);
+                x.y = __fmaf_rn(f, y.y, x.y);
+            }
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            const float lse = top + log2f(sum);   // no key: -inf
             if (!pieces && !p.has_prefix) {
-                sum.write(p.a, it.seq, head0 + r, lane);
+                if (d < p.a.cache.head_dim)
+                    *reinterpret_cast<__nv_bfloat162*>(p.a.rows.out + it.seq * p.a.rows.out_row +
+                                                       (head0 + r) * p.a.rows.out_head + d) =
+                        __floats2bfloat162_rn(x.x * inv, x.y * inv);
+                if (d == 0 && p.a.rows.lse)
+                    p.a.rows.lse[static_cast<int64_t>(it.seq) * p.a.rows.n_q_heads + head0 + r] = lse * kLn2;
             } else {
                 const int64_t at = part0 + static_cast<int64_t>(blockIdx.x) * rows + r;
-                const float inv = sum.l == 0.0f ? 0.0f : 1.0f / sum.l;
-#pragma unroll
-                for (int d = 0; d < PartSum<DP>::kDims; ++d) p.w.part_o[at * DP + lane * PartSum<DP>::kDims + d] = sum.o[d] * inv;
-                if (lane == 0) p.w.part_lse[at] = sum.m + log2f(sum.l);
+                *reinterpret_cast<float2*>(p.w.part_o + at * DP + d) = make_float2(x.x * inv, x.y * inv);
+                if (d == 0) p.w.part_lse[at] = lse;
             }
         }
         if (pieces && !p.has_prefix) {   // the CTA that comes last joins them
@@ -481,8 +486,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                     sum.write(p.a, it.seq, head0 + r, lane);
                 }
         }
-        sync_consumers();   // the scratch may be written again
-    }
+    }   // (the next item's first barrier comes before its writes to the scratch)
     // the join that follows reads the prefixes' results too: this kernel does not end before theirs
     if (p.has_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
