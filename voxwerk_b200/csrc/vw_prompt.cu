@@ -49,7 +49,6 @@ constexpr int kFeedRegs = 72, kSoftmaxRegs = 208;   // registers per thread of w
 constexpr float kMaxTileSum = 65536.0f;
 constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;   // tensor memory columns: S; P0 P1, 64 each; O0 O1, 128 each
 constexpr float kLn2 = 0.693147180559945309f;
-constexpr uint32_t kOutBytes = 32 * 128;   // a softmax warp's outputs on their way: 32 rows of 128 bytes
 constexpr int kItemSlots = 3;
 constexpr int kItemReaders = 11;  // warps 1 to 11
 
@@ -60,8 +59,7 @@ struct TileCfg {
     static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
     static constexpr int kStages = DP == 128 ? 2 : 4;   // of K, and of V
     static constexpr uint32_t kOffKv = 2 * kTileBytes;   // after the two Q tiles
-    static constexpr uint32_t kOffOut = kOffKv + 2 * kStages * kTileBytes;   // 4 KB per softmax warp
-    static constexpr uint32_t kOffBar = kOffOut + 8 * kOutBytes;
+    static constexpr uint32_t kOffBar = kOffKv + 2 * kStages * kTileBytes;
     // k_full[S] k_empty[S] v_full[S] v_empty[S] q_full q_empty s_full[2] s_free p_full[2] o_full[2] v_tail v_fixed
     // item_full[3] item_empty[3] done[2]
     static constexpr uint32_t kBars = 4 * kStages + 19;
@@ -89,6 +87,7 @@ struct TileParams {
     int32_t min_units;           // fewest units a CTA takes (split)
     float c;                     // |scale| log2(e), not 0
     int32_t negate;              // scale < 0
+    int32_t wide_out;            // output rows start on 32-byte boundaries
     TileWork w;
 };
 
@@ -352,6 +351,12 @@ __device__ __forceinline__ void mma_ts(bool pred, uint32_t d, uint32_t a, uint64
         "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(pred ? 1 : 0)
         : "memory");
+}
+
+__device__ __forceinline__ void store_sector(void* to, const uint32_t* v) {   // 32 bytes, 32-byte aligned
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                 "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 template <int DP, bool kPrefix>
@@ -757,7 +762,6 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const int head = it.kv_head * p.group + sub;
             const bool part = it.part_row >= 0;
             const int tile_rows = p.tile_tokens * p.group;
-            const int live_rows = min(tile_rows, it.tokens * p.group - q * tile_rows);   // of this row tile
             const int64_t part0 = static_cast<int64_t>(it.part_row) + q * tile_rows;     // the tile's first partial row
             if (live) {
                 const float lse = m * p.c + log2f(l);   // no key seen: -inf
@@ -766,15 +770,11 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 else if (p.a.rows.lse)
                     p.a.rows.lse[call_row * p.a.rows.n_q_heads + head] = lse * kLn2;
             }
-            // O / l through shared memory, 32 columns at a time (16-byte piece j of row r at j ^ (r & 7)), so that the lanes
-            // write 64 (bf16) or 128 (partial fp32) bytes of one row together: a lane storing its own row touches 32 lines
-            // an instruction.  Short loops: this runs once a block, and its instructions come from far away.
-            uint8_t* mine = sm + C::kOffOut + (warp - 4) * kOutBytes;
-            const uint64_t to = part ? reinterpret_cast<uint64_t>(p.w.part_o + (part0 + row) * DP)
-                                     : reinterpret_cast<uint64_t>(p.a.rows.out + call_row * p.a.rows.out_row +
-                                                                  head * p.a.rows.out_head);
-            const int shift = part ? 3 : 2;   // log2 of the lanes that share a row
-            const int piece = lane & ((1 << shift) - 1);
+            // O / l to the row, a lane its own, whole 32-byte sectors where the rows' alignment allows (through shared
+            // memory, so that lanes share lines, it takes longer: the loop is bound by its latencies, not by the stores)
+            __nv_bfloat16* out = p.a.rows.out + call_row * p.a.rows.out_row + head * p.a.rows.out_head;
+            float* to_part = p.w.part_o + (part0 + row) * DP;
+            const bool wide = p.wide_out;
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
                 float o[32];
@@ -782,25 +782,28 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 tmem_wait_load();
 #pragma unroll
                 for (int j = 0; j < 32; ++j) o[j] = some ? o[j] * r : 0.0f;
-                if (part) {
+                if (!live) {
+                } else if (part) {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        *reinterpret_cast<float4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                            make_float4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    for (int j = 0; j < 32; j += 8)
+                        store_sector(to_part + c0 + j, reinterpret_cast<const uint32_t*>(o + j));
                 } else {
+                    uint32_t v[16];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        *reinterpret_cast<uint4*>(mine + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-                            make_uint4(pack_bf16(o[8 * j], o[8 * j + 1]), pack_bf16(o[8 * j + 2], o[8 * j + 3]),
-                                       pack_bf16(o[8 * j + 4], o[8 * j + 5]), pack_bf16(o[8 * j + 6], o[8 * j + 7]));
-                }
-                __syncwarp();
-                const bool inside = part || c0 + 8 * piece < D;
-#pragma unroll 1
-                for (int rr = lane >> shift; rr < 32; rr += 32 >> shift) {
-                    const uint4 v = *reinterpret_cast<const uint4*>(mine + rr * 128 + ((piece ^ (rr & 7)) << 4));
-                    const uint64_t at = __shfl_sync(0xffffffffu, to, rr) + (part ? 4 : 2) * c0 + 16 * piece;
-                    if (inside && 32 * (warp & 3) + rr < live_rows) *reinterpret_cast<uint4*>(at) = v;
+                    for (int j = 0; j < 16; ++j) v[j] = pack_bf16(o[2 * j], o[2 * j + 1]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int col = c0 + 16 * j;
+                        if (wide && col + 16 <= D) {
+                            store_sector(out + col, v + 8 * j);
+                        } else {
+                            if (col < D)
+                                *reinterpret_cast<uint4*>(out + col) = make_uint4(v[8 * j], v[8 * j + 1], v[8 * j + 2], v[8 * j + 3]);
+                            if (col + 8 < D)
+                                *reinterpret_cast<uint4*>(out + col + 8) =
+                                    make_uint4(v[8 * j + 4], v[8 * j + 5], v[8 * j + 6], v[8 * j + 7]);
+                        }
+                    }
                 }
                 __syncwarp();
             }
@@ -867,6 +870,10 @@ cudaError_t launch_tiles(const TileParams& p, const Geometry& g, int grid, cudaS
     return cudaGetLastError();
 }
 
+bool wide_rows(const AttnParams& a) {
+    return reinterpret_cast<uintptr_t>(a.rows.out) % 32 == 0 && a.rows.out_row % 16 == 0 && a.rows.out_head % 16 == 0;
+}
+
 }  // namespace
 
 // Whole blocks by ticket when there are at least two for each SM, or when no sequence can have more keys than
@@ -901,13 +908,13 @@ TilePlan plan_prefix(const AttnParams& a, int sms) {
 
 cudaError_t launch_prefix_attention(const AttnParams& a, const TilePlan& plan, const TileWork& w, cudaStream_t stream) {
     const Geometry g = geometry(a);
-    TileParams p{a, g.group, g.tile_tokens, 1, kMinPrefixUnits, exp2_scale(a.rows.scale), a.rows.scale < 0.0f, w};
+    TileParams p{a, g.group, g.tile_tokens, 1, kMinPrefixUnits, exp2_scale(a.rows.scale), a.rows.scale < 0.0f, wide_rows(a), w};
     return plan.dim == 64 ? launch_tiles<64, true>(p, g, plan.grid, stream) : launch_tiles<128, true>(p, g, plan.grid, stream);
 }
 
 cudaError_t launch_prompt_attention(const AttnParams& a, const TilePlan& plan, const TileWork& w, cudaStream_t stream) {
     const Geometry g = geometry(a);
-    TileParams p{a, g.group, g.tile_tokens, plan.split, kMinPromptUnits, exp2_scale(a.rows.scale), a.rows.scale < 0.0f, w};
+    TileParams p{a, g.group, g.tile_tokens, plan.split, kMinPromptUnits, exp2_scale(a.rows.scale), a.rows.scale < 0.0f, wide_rows(a), w};
     cudaError_t e = plan.dim == 64 ? launch_tiles<64, false>(p, g, plan.grid, stream)
                                    : launch_tiles<128, false>(p, g, plan.grid, stream);
     if (e != cudaSuccess || !plan.split) return e;
