@@ -192,7 +192,7 @@ VW_EXPORT vw_status vw_rope_append(vw_handle* h, const vw_kv_cache* cache, const
     p.batch = batch_dev(*batch);
     p.err = h->d_err;
     cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess) e = vw::launch_rope_append(p, st);
+    if (e == cudaSuccess) e = vw::launch_rope_append(p, h->sm_count, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "rope append");
     if (!stream) return read_device_error(h, st);
     return VW_OK;

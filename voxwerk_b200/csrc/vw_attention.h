@@ -64,7 +64,7 @@ struct RopeParams {
     KvBatchDev batch;
     unsigned* err;
 };
-cudaError_t launch_rope_append(const RopeParams& p, cudaStream_t stream);
+cudaError_t launch_rope_append(const RopeParams& p, int sms, cudaStream_t stream);
 
 struct AttnParams {
     AttnRowsDev rows;

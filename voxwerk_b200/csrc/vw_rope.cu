@@ -7,10 +7,12 @@
 // (i, i + half) or, interleaved, (2 i, 2 i + 1).  All in fp32, rounded to bf16 once, when written.  Queries go to
 // q_out, keys and values into the page that holds the row's key index.
 //
-// Bound: HBM (one read of q, k, v, one write of q_out and the cache rows); a handful of rows: latency.  So one pass: a
-// lane holds the two chunks of CH elements that hold its pairs' both halves, a group of GS lanes holds one head, and
-// the norm's sum is the only exchange between lanes.  The loads of a block's rows are issued before the row's sequence
-// is looked up, so the lookup's latency (sequence, page, table row) overlaps theirs.
+// Bound: HBM (one read of q, k, v, one write of q_out and the cache rows); a handful of rows: latency.  So one pass, a
+// warp to a row (several where rows are few): a lane holds the two chunks of CH elements that hold its pairs' both
+// halves, a group of GS lanes holds one head, and the norm's sum is the only exchange between lanes.  A lane meets the
+// same dims in every head of a row, so its part of the cos / sin row is read once, and the weights once for queries and
+// once for keys.  The first heads' loads are issued before the row's place is looked up (a chain of four dependent
+// loads: sequence, its length, its page, table row), four at a time after that.
 
 #include <cuda_runtime.h>
 
@@ -22,7 +24,9 @@
 namespace vw {
 namespace {
 
-constexpr int kMaxRowsPerBlock = 32;
+constexpr int kThreads = 256;
+constexpr int kBatch = 4;             // heads a lane has on their way
+constexpr int kWarpsPerSm = 16;       // what the registers leave room for
 
 struct RowPlace {
     int64_t slot;   // element offset of the row's (page, token) in the cache, or -1: the row is left alone
@@ -61,43 +65,43 @@ __device__ RowPlace place_row(const RopeParams& p, int row, int lane) {
     return r;
 }
 
-template <int CH>
-__device__ __forceinline__ void load_chunk(const __nv_bfloat16* s, float* x) {
-    if constexpr (CH == 8) {
-        const uint4 u = __ldcs(reinterpret_cast<const uint4*>(s));
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+// CH elements as they were loaded
+template <typename T, int CH>
+struct Chunk {
+    static constexpr int kBytes = CH * static_cast<int>(sizeof(T));
+    uint32_t w[kBytes < 4 ? 1 : kBytes / 4];
+
+    __device__ __forceinline__ void load(const T* s) {
+        if constexpr (kBytes >= 16) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    } else if constexpr (CH == 4) {
-        const uint2 u = __ldcs(reinterpret_cast<const uint2*>(s));
-        const uint32_t w[2] = {u.x, u.y};
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    } else {
-        x[0] = __bfloat162float(*s);
-    }
-}
-template <int CH>
-__device__ __forceinline__ void load_chunk(const float* s, float* x) {
-    if constexpr (CH == 1) {
-        x[0] = *s;
-    } else {
-#pragma unroll
-        for (int i = 0; i < CH; i += 4) {
-            const float4 f = __ldcs(reinterpret_cast<const float4*>(s + i));
-            x[i] = f.x;
-            x[i + 1] = f.y;
-            x[i + 2] = f.z;
-            x[i + 3] = f.w;
+            for (int i = 0; i < kBytes / 16; ++i) {
+                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(s) + i);
+                w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+            }
+        } else if constexpr (kBytes == 8) {
+            const uint2 u = __ldcs(reinterpret_cast<const uint2*>(s));
+            w[0] = u.x, w[1] = u.y;
+        } else if constexpr (kBytes == 4) {
+            w[0] = *reinterpret_cast<const uint32_t*>(s);
+        } else {
+            w[0] = *reinterpret_cast<const uint16_t*>(s);
         }
     }
-}
+    __device__ __forceinline__ void widen(float* x) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < CH; ++i) x[i] = __uint_as_float(w[i]);
+        } else if constexpr (CH == 1) {
+            x[0] = __uint_as_float(w[0] << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < CH / 2; ++i) {
+                x[2 * i] = __uint_as_float(w[i] << 16);
+                x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        }
+    }
+};
 // fp32 table or weight values; they are shared by many rows, so they stay cached
 template <int N>
 __device__ __forceinline__ void load_f32(const float* s, float* x) {
@@ -149,123 +153,129 @@ __device__ __forceinline__ void slot_dims(int j, int half, int& a, int& b, bool&
     }
 }
 
-// x[0..CH) and x[CH..2 CH): the slot's chunks
+// The row of the tables a slot turns by, and x[0..CH) and x[CH..2 CH), the slot's chunks, turned
 template <int CH, bool kInterleaved>
-__device__ __forceinline__ void turn(const RopeParams& p, int pos, int a, float* x) {
-    const float* c = p.cos_table + static_cast<int64_t>(pos) * p.half;
-    const float* s = p.sin_table + static_cast<int64_t>(pos) * p.half;
+struct Turn {
     float cs[CH], sn[CH];
-    if constexpr (kInterleaved && CH > 1) {   // chunk elements (2 e, 2 e + 1) are pair a / 2 + e of the head
-        load_f32<CH>(c + a / 2, cs);
-        load_f32<CH>(s + a / 2, sn);
+
+    __device__ __forceinline__ void load(const RopeParams& p, int pos, int a) {
+        // interleaved chunks: elements (2 e, 2 e + 1) of a slot are pair a / 2 + e of the head
+        const int64_t at = static_cast<int64_t>(pos) * p.half + (kInterleaved ? a / 2 : a);
+        load_f32<CH>(p.cos_table + at, cs);
+        load_f32<CH>(p.sin_table + at, sn);
+    }
+    __device__ __forceinline__ void apply(float* x) const {
 #pragma unroll
         for (int e = 0; e < CH; ++e) {
-            const float u = x[2 * e], v = x[2 * e + 1];
-            x[2 * e] = u * cs[e] - v * sn[e];
-            x[2 * e + 1] = v * cs[e] + u * sn[e];
-        }
-    } else {
-        const int i = kInterleaved ? a / 2 : a;
-        load_f32<CH>(c + i, cs);
-        load_f32<CH>(s + i, sn);
-#pragma unroll
-        for (int e = 0; e < CH; ++e) {
-            const float u = x[e], v = x[CH + e];
-            x[e] = u * cs[e] - v * sn[e];
-            x[CH + e] = v * cs[e] + u * sn[e];
+            float& first = kInterleaved && CH > 1 ? x[2 * e] : x[e];
+            float& second = kInterleaved && CH > 1 ? x[2 * e + 1] : x[CH + e];
+            const float u = first, v = second;
+            first = u * cs[e] - v * sn[e];
+            second = v * cs[e] + u * sn[e];
         }
     }
-}
+};
 
-// NP pair slots per lane (1 unless a head has more slots than a warp has lanes)
+// NP pair slots per lane (1 unless a head has more slots than a warp has lanes); teams of 2^team_shift warps to a row,
+// 2^group_shift lanes to a head
 template <typename T, int CH, bool kInterleaved, int NP>
-__global__ void __launch_bounds__(512) rope_append_kernel(const RopeParams p, int rows_per_block, int group_shift) {
-    __shared__ RowPlace places[kMaxRowsPerBlock];
-    const int heads = p.n_q_heads + 2 * p.cache.n_kv_heads;
-    const int D = p.cache.head_dim, slots = D / (2 * CH);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int row0 = blockIdx.x * rows_per_block;
-    const int rows = min(rows_per_block, p.batch.n_rows - row0);
-    const int groups = blockDim.x >> group_shift, gs = 1 << group_shift;
-    const int j0 = threadIdx.x & (gs - 1);
-    const int tasks = rows * heads;
-
-    // head `t` of the block's rows: its source and kind (0 query, 1 key, 2 value)
-    auto source = [&](int t, int& row, int& head, int& kind) -> const T* {
-        row = row0 + t / heads;
-        head = t % heads;
-        kind = head < p.n_q_heads ? 0 : head < p.n_q_heads + p.cache.n_kv_heads ? 1 : 2;
-        head -= kind == 0 ? 0 : kind == 1 ? p.n_q_heads : p.n_q_heads + p.cache.n_kv_heads;
-        return kind == 0   ? static_cast<const T*>(p.q) + row * p.q_row + head * p.q_head
-               : kind == 1 ? static_cast<const T*>(p.k) + row * p.k_row + head * p.k_head
-                           : static_cast<const T*>(p.v) + row * p.v_row + head * p.v_head;
-    };
-    auto load_task = [&](int t, float (&x)[NP][2 * CH]) {
-        if (t >= tasks) return;
-        int row, head, kind;
-        const T* s = source(t, row, head, kind);
+__global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_constant__ RopeParams p, int team_shift,
+                                                               int group_shift) {
+    constexpr int U = NP == 1 ? kBatch : 1;
+    const int lane = threadIdx.x & 31;
+    const int warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+    const int teams = (gridDim.x * (kThreads / 32)) >> team_shift, member = warp & ((1 << team_shift) - 1);
+    const int n_kv = p.cache.n_kv_heads, heads = p.n_q_heads + 2 * n_kv;
+    const int D = p.cache.head_dim, slots = D / (2 * CH), gs = 1 << group_shift;
+    const int sub = lane >> group_shift, j0 = lane & (gs - 1);
+    const int step = 32 >> group_shift;   // heads of a warp at a time
+    int da[NP], db[NP];                   // the lane's chunks of every head
+    bool has[NP], turns[NP];
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const int j = j0 + n * gs;
-            if (j >= slots) break;
-            int a, b;
-            bool turns;
-            slot_dims<CH, kInterleaved>(j, p.half, a, b, turns);
-            load_chunk<CH>(s + a, x[n]);
-            load_chunk<CH>(s + b, x[n] + CH);
-        }
-    };
-
-    float x[NP][2 * CH] = {};
-    load_task(threadIdx.x >> group_shift, x);
-    for (int r = warp; r < rows; r += blockDim.x >> 5) {
-        const RowPlace pl = place_row(p, row0 + r, lane);
-        if (lane == 0) places[r] = pl;
+    for (int n = 0; n < NP; ++n) {
+        slot_dims<CH, kInterleaved>(j0 + n * gs, p.half, da[n], db[n], turns[n]);
+        has[n] = j0 + n * gs < slots;
+        turns[n] = turns[n] && has[n];
     }
-    __syncthreads();
+    // head h of a row: 0 a query, 1 a key, 2 a value
+    const auto kind_of = [&](int h) { return h < p.n_q_heads ? 0 : h < p.n_q_heads + n_kv ? 1 : 2; };
 
-    for (int t0 = 0; t0 < tasks; t0 += groups) {
-        const int t = t0 + (threadIdx.x >> group_shift);
-        if (t0 > 0) load_task(t, x);
-        const bool live = t < tasks;
-        int row = 0, head = 0, kind = 0;
-        RowPlace pl{-1, 0};
-        if (live) {
-            source(t, row, head, kind);
-            pl = places[row - row0];
-        }
-        const float* weight = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
-        float sum = 0.0f;
-        if (live && weight) {
+    for (int row = warp >> team_shift; row < p.batch.n_rows; row += teams) {
+        Chunk<T, CH> raw[U][NP][2];
+        const auto load_batch = [&](int h0) {
 #pragma unroll
-            for (int n = 0; n < NP; ++n)
-                if (j0 + n * gs < slots)
+            for (int u = 0; u < U; ++u) {
+                const int h = h0 + (u << team_shift) * step;
+                if (h >= heads) break;
+                const int kind = kind_of(h);
+                const T* s = kind == 0   ? static_cast<const T*>(p.q) + row * p.q_row + h * p.q_head
+                             : kind == 1 ? static_cast<const T*>(p.k) + row * p.k_row + (h - p.n_q_heads) * p.k_head
+                                         : static_cast<const T*>(p.v) + row * p.v_row + (h - p.n_q_heads - n_kv) * p.v_head;
 #pragma unroll
-                    for (int e = 0; e < 2 * CH; ++e) sum = __fmaf_rn(x[n][e], x[n][e], sum);
-        }
-        for (int o = gs >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (!live || pl.slot < 0) continue;
-        const float rs = __frsqrt_rn(sum / static_cast<float>(D) + p.eps);
-        __nv_bfloat16* dst = kind == 0   ? p.q_out + row * p.q_out_row + head * p.q_out_head
-                             : kind == 1 ? p.cache.k + pl.slot + head * p.cache.head_stride
-                                         : p.cache.v + pl.slot + head * p.cache.head_stride;
-#pragma unroll
-        for (int n = 0; n < NP; ++n) {
-            const int j = j0 + n * gs;
-            if (j >= slots) break;
-            int a, b;
-            bool turns;
-            slot_dims<CH, kInterleaved>(j, p.half, a, b, turns);
-            if (weight) {
-                float w[2 * CH];
-                load_f32<CH>(weight + a, w);
-                load_f32<CH>(weight + b, w + CH);
-#pragma unroll
-                for (int e = 0; e < 2 * CH; ++e) x[n][e] = x[n][e] * rs * w[e];
+                for (int n = 0; n < NP; ++n)
+                    if (has[n]) {
+                        raw[u][n][0].load(s + da[n]);
+                        raw[u][n][1].load(s + db[n]);
+                    }
             }
-            if (kind != 2 && turns) turn<CH, kInterleaved>(p, pl.pos, a, x[n]);
-            store_chunk<CH>(dst + a, x[n]);
-            store_chunk<CH>(dst + b, x[n] + CH);
+        };
+        const int first = member * step + sub;
+        load_batch(first);
+        const RowPlace at = place_row(p, row, lane);
+        if (at.slot < 0) continue;   // the warp's one row
+        Turn<CH, kInterleaved> turn[NP];
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+            if (turns[n]) turn[n].load(p, at.pos, da[n]);
+        float weight[NP][2 * CH];
+        int weight_of = -1;
+        // (a warp's lanes leave together: the norm's sum takes all of them)
+        for (int base = member * step; base < heads; base += (U << team_shift) * step) {
+            if (base > member * step) load_batch(base + sub);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int h0 = base + (u << team_shift) * step, h = h0 + sub;
+                if (h0 >= heads) break;
+                const bool live = h < heads;
+                const int kind = kind_of(h);
+                const float* w = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
+                float x[NP][2 * CH];
+                float sum = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    raw[u][n][0].widen(x[n]);
+                    raw[u][n][1].widen(x[n] + CH);
+                    if (live && w && has[n])
+#pragma unroll
+                        for (int e = 0; e < 2 * CH; ++e) sum = __fmaf_rn(x[n][e], x[n][e], sum);
+                }
+                for (int o = gs >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (!live) continue;
+                if (w && weight_of != kind) {
+                    weight_of = kind;
+#pragma unroll
+                    for (int n = 0; n < NP; ++n)
+                        if (has[n]) {
+                            load_f32<CH>(w + da[n], weight[n]);
+                            load_f32<CH>(w + db[n], weight[n] + CH);
+                        }
+                }
+                const float rs = __frsqrt_rn(sum / static_cast<float>(D) + p.eps);
+                __nv_bfloat16* dst =
+                    kind == 0   ? p.q_out + row * p.q_out_row + h * p.q_out_head
+                    : kind == 1 ? p.cache.k + at.slot + (h - p.n_q_heads) * p.cache.head_stride
+                                : p.cache.v + at.slot + (h - p.n_q_heads - n_kv) * p.cache.head_stride;
+#pragma unroll
+                for (int n = 0; n < NP; ++n) {
+                    if (!has[n]) continue;
+                    if (w)
+#pragma unroll
+                        for (int e = 0; e < 2 * CH; ++e) x[n][e] = x[n][e] * rs * weight[n][e];
+                    if (kind != 2 && turns[n]) turn[n].apply(x[n]);
+                    store_chunk<CH>(dst + da[n], x[n]);
+                    store_chunk<CH>(dst + db[n], x[n] + CH);
+                }
+            }
         }
     }
 }
@@ -292,33 +302,37 @@ bool chunks_fit(const RopeParams& p, int ch) {
 }
 
 template <typename T, int CH, int NP>
-cudaError_t launch_ch(const RopeParams& p, cudaStream_t stream) {
+cudaError_t launch_ch(const RopeParams& p, int sms, cudaStream_t stream) {
     const int heads = p.n_q_heads + 2 * p.cache.n_kv_heads;
     const int slots = p.cache.head_dim / (2 * CH);
-    int shift = 0;
-    while ((1 << shift) < slots && shift < 5) ++shift;
-    const int per_row = heads << shift;
-    const int threads = std::clamp((per_row + 31) / 32 * 32, 128, 512);
-    const int rows = std::clamp(threads / per_row, 1, kMaxRowsPerBlock);
-    const int grid = (p.batch.n_rows + rows - 1) / rows;
+    int group_shift = 0;
+    while ((1 << group_shift) < slots && group_shift < 5) ++group_shift;
+    const int passes = (heads + (32 >> group_shift) - 1) / (32 >> group_shift);
+    // warps to a row: more while some would have nothing to do otherwise
+    const int64_t room = static_cast<int64_t>(sms) * kWarpsPerSm;
+    int team_shift = 0;
+    while (team_shift < 3 && (2 << team_shift) <= passes && (static_cast<int64_t>(p.batch.n_rows) << (team_shift + 1)) <= room)
+        ++team_shift;
+    const int64_t warps = std::min(static_cast<int64_t>(p.batch.n_rows) << team_shift, room);
+    const int grid = static_cast<int>((warps + kThreads / 32 - 1) / (kThreads / 32));
     if (p.interleaved)
-        rope_append_kernel<T, CH, true, NP><<<grid, threads, 0, stream>>>(p, rows, shift);
+        rope_append_kernel<T, CH, true, NP><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
     else
-        rope_append_kernel<T, CH, false, NP><<<grid, threads, 0, stream>>>(p, rows, shift);
+        rope_append_kernel<T, CH, false, NP><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
     return cudaGetLastError();
 }
 
 template <typename T>
-cudaError_t launch_type(const RopeParams& p, cudaStream_t stream) {
-    if (chunks_fit(p, 8)) return launch_ch<T, 8, 1>(p, stream);
-    if (chunks_fit(p, 4)) return launch_ch<T, 4, 1>(p, stream);
-    return launch_ch<T, 1, 4>(p, stream);   // any alignment, any even head_dim <= 256
+cudaError_t launch_type(const RopeParams& p, int sms, cudaStream_t stream) {
+    if (chunks_fit(p, 8)) return launch_ch<T, 8, 1>(p, sms, stream);
+    if (chunks_fit(p, 4)) return launch_ch<T, 4, 1>(p, sms, stream);
+    return launch_ch<T, 1, 4>(p, sms, stream);   // any alignment, any even head_dim <= 256
 }
 
 }  // namespace
 
-cudaError_t launch_rope_append(const RopeParams& p, cudaStream_t stream) {
-    return p.f32 ? launch_type<float>(p, stream) : launch_type<__nv_bfloat16>(p, stream);
+cudaError_t launch_rope_append(const RopeParams& p, int sms, cudaStream_t stream) {
+    return p.f32 ? launch_type<float>(p, sms, stream) : launch_type<__nv_bfloat16>(p, sms, stream);
 }
 
 }  // namespace vw
