@@ -183,6 +183,7 @@ VW_EXPORT vw_status vw_rope_append(vw_handle* h, const vw_kv_cache* cache, const
     p.sin_table = rows->sin_table;
     p.positions = rows->positions;
     p.eps = rows->eps;
+    p.inv_dim = 1.0f / static_cast<float>(cache->head_dim);
     p.half = rows->rotary_dim / 2;
     p.n_positions = p.half ? rows->n_positions : INT32_MAX;   // no table: any position
     p.interleaved = rows->interleaved != 0;

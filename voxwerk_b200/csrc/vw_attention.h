@@ -58,7 +58,7 @@ struct RopeParams {
     const float* cos_table;     // [n_positions, half]
     const float* sin_table;
     const int32_t* positions;   // nullable: a row's position is its key index
-    float eps;
+    float eps, inv_dim;         // 1 / head_dim
     int32_t n_positions, half, interleaved, f32, n_q_heads;
     KvCacheDev cache;
     KvBatchDev batch;

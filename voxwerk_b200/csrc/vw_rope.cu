@@ -17,6 +17,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "vw_attention.h"
 #include "vw_internal.h"
@@ -24,9 +25,8 @@
 namespace vw {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kBatch = 4;             // heads a lane has on their way
-constexpr int kWarpsPerSm = 16;       // what the registers leave room for
+constexpr int kThreads = 128;
+constexpr int kWarpsPerSm = 16;   // all resident at once (a second wave of such long-lived warps would double the time)
 
 struct RowPlace {
     int64_t slot;   // element offset of the row's (page, token) in the cache, or -1: the row is left alone
@@ -153,6 +153,38 @@ __device__ __forceinline__ void slot_dims(int j, int half, int& a, int& b, bool&
     }
 }
 
+// two fp32 products, or products and sums, per instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+        "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+template <int N>
+__device__ __forceinline__ void scale(float* x, const float* w) {   // x[i] *= w[i]
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 y = mul2(make_float2(x[i], x[i + 1]), make_float2(w[i], w[i + 1]));
+            x[i] = y.x, x[i + 1] = y.y;
+        }
+    } else {
+        x[0] *= w[0];
+    }
+}
+
 // The row of the tables a slot turns by, and x[0..CH) and x[CH..2 CH), the slot's chunks, turned
 template <int CH, bool kInterleaved>
 struct Turn {
@@ -165,27 +197,38 @@ struct Turn {
         load_f32<CH>(p.sin_table + at, sn);
     }
     __device__ __forceinline__ void apply(float* x) const {
+        if constexpr (!kInterleaved && CH > 1) {   // two pairs at a time
 #pragma unroll
-        for (int e = 0; e < CH; ++e) {
-            float& first = kInterleaved && CH > 1 ? x[2 * e] : x[e];
-            float& second = kInterleaved && CH > 1 ? x[2 * e + 1] : x[CH + e];
-            const float u = first, v = second;
-            first = u * cs[e] - v * sn[e];
-            second = v * cs[e] + u * sn[e];
+            for (int e = 0; e < CH; e += 2) {
+                const float2 u = make_float2(x[e], x[e + 1]), v = make_float2(x[CH + e], x[CH + e + 1]);
+                const float2 c = make_float2(cs[e], cs[e + 1]), s = make_float2(sn[e], sn[e + 1]);
+                const float2 a = fma2(make_float2(-v.x, -v.y), s, mul2(u, c)), b = fma2(u, s, mul2(v, c));
+                x[e] = a.x, x[e + 1] = a.y, x[CH + e] = b.x, x[CH + e + 1] = b.y;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < CH; ++e) {
+                float& first = CH > 1 ? x[2 * e] : x[e];
+                float& second = CH > 1 ? x[2 * e + 1] : x[CH + e];
+                const float u = first, v = second;
+                first = __fmaf_rn(-v, sn[e], u * cs[e]);
+                second = __fmaf_rn(u, sn[e], v * cs[e]);
+            }
         }
     }
 };
 
 // NP pair slots per lane (1 unless a head has more slots than a warp has lanes); teams of 2^team_shift warps to a row,
 // 2^group_shift lanes to a head
-template <typename T, int CH, bool kInterleaved, int NP>
-__global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_constant__ RopeParams p, int team_shift,
-                                                               int group_shift) {
-    constexpr int U = NP == 1 ? kBatch : 1;
+// U heads of a lane on their way at once.  kFew (rows): the first head of every kind is loaded up front, in registers of
+// its own, since the row's latency counts; else the kinds follow each other in the same registers, so that more warps fit
+// (14 595 rows: 51 us, 66 us with all of a row's loads up front).
+template <typename T, int CH, bool kInterleaved, int NP, int U, bool kFew>
+__global__ void __launch_bounds__(kThreads, kFew ? 1 : kWarpsPerSm * 32 / kThreads)
+rope_append_kernel(const __grid_constant__ RopeParams p, int team_shift, int group_shift) {
     const int lane = threadIdx.x & 31;
     const int warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
     const int teams = (gridDim.x * (kThreads / 32)) >> team_shift, member = warp & ((1 << team_shift) - 1);
-    const int n_kv = p.cache.n_kv_heads, heads = p.n_q_heads + 2 * n_kv;
     const int D = p.cache.head_dim, slots = D / (2 * CH), gs = 1 << group_shift;
     const int sub = lane >> group_shift, j0 = lane & (gs - 1);
     const int step = 32 >> group_shift;   // heads of a warp at a time
@@ -197,85 +240,110 @@ __global__ void __launch_bounds__(kThreads) rope_append_kernel(const __grid_cons
         has[n] = j0 + n * gs < slots;
         turns[n] = turns[n] && has[n];
     }
-    // head h of a row: 0 a query, 1 a key, 2 a value
-    const auto kind_of = [&](int h) { return h < p.n_q_heads ? 0 : h < p.n_q_heads + n_kv ? 1 : 2; };
+    const int first = member * step + sub, next = step << team_shift;
 
     for (int row = warp >> team_shift; row < p.batch.n_rows; row += teams) {
-        Chunk<T, CH> raw[U][NP][2];
-        const auto load_batch = [&](int h0) {
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int h = h0 + (u << team_shift) * step;
-                if (h >= heads) break;
-                const int kind = kind_of(h);
-                const T* s = kind == 0   ? static_cast<const T*>(p.q) + row * p.q_row + h * p.q_head
-                             : kind == 1 ? static_cast<const T*>(p.k) + row * p.k_row + (h - p.n_q_heads) * p.k_head
-                                         : static_cast<const T*>(p.v) + row * p.v_row + (h - p.n_q_heads - n_kv) * p.v_head;
-#pragma unroll
-                for (int n = 0; n < NP; ++n)
-                    if (has[n]) {
-                        raw[u][n][0].load(s + da[n]);
-                        raw[u][n][1].load(s + db[n]);
-                    }
-            }
-        };
-        const int first = member * step + sub;
-        load_batch(first);
-        const RowPlace at = place_row(p, row, lane);
-        if (at.slot < 0) continue;   // the warp's one row
         Turn<CH, kInterleaved> turn[NP];
+        Chunk<T, CH> raw_q[U][NP][2], own_k[1][NP][2], own_v[1][NP][2];
+        const auto load_batch = [&](auto& raw, const T* src, int64_t stride, int h0, int heads) {
+            constexpr int kCount = sizeof(raw) / sizeof(raw[0]);
 #pragma unroll
-        for (int n = 0; n < NP; ++n)
-            if (turns[n]) turn[n].load(p, at.pos, da[n]);
-        float weight[NP][2 * CH];
-        int weight_of = -1;
-        // (a warp's lanes leave together: the norm's sum takes all of them)
-        for (int base = member * step; base < heads; base += (U << team_shift) * step) {
-            if (base > member * step) load_batch(base + sub);
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const int h0 = base + (u << team_shift) * step, h = h0 + sub;
-                if (h0 >= heads) break;
-                const bool live = h < heads;
-                const int kind = kind_of(h);
-                const float* w = kind == 0 ? p.q_norm : kind == 1 ? p.k_norm : nullptr;
-                float x[NP][2 * CH];
-                float sum = 0.0f;
-#pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    raw[u][n][0].widen(x[n]);
-                    raw[u][n][1].widen(x[n] + CH);
-                    if (live && w && has[n])
-#pragma unroll
-                        for (int e = 0; e < 2 * CH; ++e) sum = __fmaf_rn(x[n][e], x[n][e], sum);
-                }
-                for (int o = gs >> 1; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (!live) continue;
-                if (w && weight_of != kind) {
-                    weight_of = kind;
+            for (int u = 0; u < kCount; ++u)
+                if (h0 + u * next < heads) {
+                    const T* s = src + (h0 + u * next) * stride;
 #pragma unroll
                     for (int n = 0; n < NP; ++n)
                         if (has[n]) {
-                            load_f32<CH>(w + da[n], weight[n]);
-                            load_f32<CH>(w + db[n], weight[n] + CH);
+                            raw[u][n][0].load(s + da[n]);
+                            raw[u][n][1].load(s + db[n]);
                         }
                 }
-                const float rs = __frsqrt_rn(sum / static_cast<float>(D) + p.eps);
-                __nv_bfloat16* dst =
-                    kind == 0   ? p.q_out + row * p.q_out_row + h * p.q_out_head
-                    : kind == 1 ? p.cache.k + at.slot + (h - p.n_q_heads) * p.cache.head_stride
-                                : p.cache.v + at.slot + (h - p.n_q_heads - n_kv) * p.cache.head_stride;
+        };
+        // the heads of one kind (values are copied only)
+        const auto heads_of = [&](auto value, auto& raw, const T* src, int64_t stride, int heads, const float* w,
+                                  __nv_bfloat16* dst, int64_t dst_stride, bool loaded) {
+            constexpr bool kValue = decltype(value)::value;
+            constexpr int kCount = sizeof(raw) / sizeof(raw[0]);
+            float weight[NP][2 * CH];
+            if (!kValue && w) {
 #pragma unroll
-                for (int n = 0; n < NP; ++n) {
-                    if (!has[n]) continue;
-                    if (w)
+                for (int n = 0; n < NP; ++n)
+                    if (has[n]) {
+                        load_f32<CH>(w + da[n], weight[n]);
+                        load_f32<CH>(w + db[n], weight[n] + CH);
+                    }
+            }
+            // (a warp's lanes leave together: the norm's sum takes all of them)
+            for (int base = member * step; base < heads; base += kCount * next, loaded = false) {
+                if (!loaded) load_batch(raw, src, stride, base + sub, heads);
 #pragma unroll
-                        for (int e = 0; e < 2 * CH; ++e) x[n][e] = x[n][e] * rs * weight[n][e];
-                    if (kind != 2 && turns[n]) turn[n].apply(x[n]);
-                    store_chunk<CH>(dst + da[n], x[n]);
-                    store_chunk<CH>(dst + db[n], x[n] + CH);
+                for (int u = 0; u < kCount; ++u) {
+                    if (base + u * next >= heads) break;
+                    const int h = base + u * next + sub;
+                    const bool live = h < heads;
+                    float x[NP][2 * CH];
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        raw[u][n][0].widen(x[n]);
+                        raw[u][n][1].widen(x[n] + CH);
+                    }
+                    if (!kValue && w) {
+                        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                        for (int n = 0; n < NP; ++n)
+                            if (live && has[n])
+#pragma unroll
+                                for (int e = 0; e < 2 * CH; e += 2) {
+                                    const float2 y = make_float2(x[n][e], x[n][e + 1]);
+                                    sum = fma2(y, y, sum);
+                                }
+                        float all = sum.x + sum.y;
+                        for (int o = gs >> 1; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+                        const float rs = rsqrtf(__fmaf_rn(all, p.inv_dim, p.eps));
+#pragma unroll
+                        for (int n = 0; n < NP; ++n) {
+                            scale<2 * CH>(x[n], weight[n]);
+                            float r[2 * CH];
+#pragma unroll
+                            for (int e = 0; e < 2 * CH; ++e) r[e] = rs;
+                            scale<2 * CH>(x[n], r);
+                        }
+                    }
+                    if (!live) continue;
+                    __nv_bfloat16* to = dst + h * dst_stride;
+#pragma unroll
+                    for (int n = 0; n < NP; ++n) {
+                        if (!has[n]) continue;
+                        if (!kValue && turns[n]) turn[n].apply(x[n]);
+                        store_chunk<CH>(to + da[n], x[n]);
+                        store_chunk<CH>(to + db[n], x[n] + CH);
+                    }
                 }
             }
+        };
+        const T* q = static_cast<const T*>(p.q) + row * p.q_row;
+        const T* k = static_cast<const T*>(p.k) + row * p.k_row;
+        const T* v = static_cast<const T*>(p.v) + row * p.v_row;
+        const int n_kv = p.cache.n_kv_heads;
+        load_batch(raw_q, q, p.q_head, first, p.n_q_heads);
+        if (kFew) {
+            load_batch(own_k, k, p.k_head, first, n_kv);
+            load_batch(own_v, v, p.v_head, first, n_kv);
+        }
+        const RowPlace at = place_row(p, row, lane);
+        if (at.slot < 0) continue;   // the warp's one row
+#pragma unroll
+        for (int n = 0; n < NP; ++n)
+            if (turns[n]) turn[n].load(p, at.pos, da[n]);
+        heads_of(std::false_type{}, raw_q, q, p.q_head, p.n_q_heads, p.q_norm, p.q_out + row * p.q_out_row, p.q_out_head,
+                 true);
+        __nv_bfloat16 *k_to = p.cache.k + at.slot, *v_to = p.cache.v + at.slot;
+        if constexpr (kFew) {
+            heads_of(std::false_type{}, own_k, k, p.k_head, n_kv, p.k_norm, k_to, p.cache.head_stride, true);
+            heads_of(std::true_type{}, own_v, v, p.v_head, n_kv, nullptr, v_to, p.cache.head_stride, true);
+        } else {
+            heads_of(std::false_type{}, raw_q, k, p.k_head, n_kv, p.k_norm, k_to, p.cache.head_stride, false);
+            heads_of(std::true_type{}, raw_q, v, p.v_head, n_kv, nullptr, v_to, p.cache.head_stride, false);
         }
     }
 }
@@ -303,11 +371,10 @@ bool chunks_fit(const RopeParams& p, int ch) {
 
 template <typename T, int CH, int NP>
 cudaError_t launch_ch(const RopeParams& p, int sms, cudaStream_t stream) {
-    const int heads = p.n_q_heads + 2 * p.cache.n_kv_heads;
     const int slots = p.cache.head_dim / (2 * CH);
     int group_shift = 0;
     while ((1 << group_shift) < slots && group_shift < 5) ++group_shift;
-    const int passes = (heads + (32 >> group_shift) - 1) / (32 >> group_shift);
+    const int passes = (p.n_q_heads + (32 >> group_shift) - 1) / (32 >> group_shift);
     // warps to a row: more while some would have nothing to do otherwise
     const int64_t room = static_cast<int64_t>(sms) * kWarpsPerSm;
     int team_shift = 0;
@@ -315,10 +382,16 @@ cudaError_t launch_ch(const RopeParams& p, int sms, cudaStream_t stream) {
         ++team_shift;
     const int64_t warps = std::min(static_cast<int64_t>(p.batch.n_rows) << team_shift, room);
     const int grid = static_cast<int>((warps + kThreads / 32 - 1) / (kThreads / 32));
-    if (p.interleaved)
-        rope_append_kernel<T, CH, true, NP><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
+    constexpr int kMany = NP > 1 ? 1 : 4;
+    const bool few = team_shift > 0 || NP > 1;
+    if (p.interleaved && few)
+        rope_append_kernel<T, CH, true, NP, 1, true><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
+    else if (p.interleaved)
+        rope_append_kernel<T, CH, true, NP, kMany, false><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
+    else if (few)
+        rope_append_kernel<T, CH, false, NP, 1, true><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
     else
-        rope_append_kernel<T, CH, false, NP><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
+        rope_append_kernel<T, CH, false, NP, kMany, false><<<grid, kThreads, 0, stream>>>(p, team_shift, group_shift);
     return cudaGetLastError();
 }
 
