@@ -22,8 +22,13 @@ import ctypes
 import math
 from typing import Optional
 
+import torch
+
 from ._lib import VW_BF16, VW_F32, VwAttnRows, VwKvBatch, VwKvCache, VwKvPrefix, VwRopeRows, check, lib
 from .sampler import Device
+
+
+_BF16, _F32 = torch.bfloat16, torch.float32
 
 
 def _need(ok: bool, message: str) -> None:
@@ -34,24 +39,30 @@ def _need(ok: bool, message: str) -> None:
 def _cuda(t, dtype: str, dims: int, what: str):
     if not getattr(t, "is_cuda", False):
         raise TypeError(f"{what} must be a CUDA tensor")
-    if str(t.dtype) != "torch." + dtype:
+    if t.dtype is not getattr(torch, dtype):
         raise TypeError(f"{what} must be {dtype}, got {t.dtype}")
     if t.dim() != dims:
         raise ValueError(f"{what} must have {dims} dimensions")
     return t
 
 
-def _strides(t, what: str):
-    """(row, head) strides of [rows, heads, dim]; a dimension of size one has no stride of its own."""
-    rows, heads, dim = t.shape
+def _rows(t, dtype, shape, what: str):
+    """Pointer, row and head stride of a [rows, heads, dim] tensor; a dimension of size one has no stride of its own."""
+    if not getattr(t, "is_cuda", False):
+        raise TypeError(f"{what} must be a CUDA tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{what} must be {str(dtype)[6:]}, got {t.dtype}")
+    if t.shape != shape:
+        raise ValueError(f"{what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     row, head, one = t.stride()
+    rows, heads, dim = shape
     if one != 1 and dim != 1:
         raise ValueError(f"{what}: the last dimension must be contiguous")
     if heads == 1:
         head = (dim + 7) // 8 * 8
     if rows == 1:
         row = heads * head
-    return row, head
+    return t.data_ptr(), row, head
 
 
 class KvCache:
@@ -75,7 +86,6 @@ class KvCache:
 
     @staticmethod
     def empty(n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device="cuda") -> "KvCache":
-        import torch
         shape = (n_pages, page_size, n_kv_heads, head_dim)
         return KvCache(*(torch.empty(shape, dtype=torch.bfloat16, device=device) for _ in range(2)))
 
@@ -133,8 +143,8 @@ class RopeTable:
         _need(cos.shape == sin.shape and cos.is_contiguous() and sin.is_contiguous(),
               "cos and sin must be contiguous and of one shape")
         self.cos, self.sin, self.interleaved = cos, sin, bool(interleaved)
-        self._c = (int(cos.shape[0]), cos.data_ptr(), sin.data_ptr())
         self.rotary_dim = 2 * int(cos.shape[1])
+        self._c = (int(cos.shape[0]), cos.data_ptr(), sin.data_ptr(), self.rotary_dim, int(self.interleaved))
 
     @staticmethod
     def angles(n_positions: int, rotary_dim: int, base: float = 10000.0, linear: float = 1.0,
@@ -143,7 +153,6 @@ class RopeTable:
         factor of YaRN (Peng et al. 2023): frequencies that turn fewer than beta_slow times over `trained_positions`
         are divided by it, those that turn more than beta_fast times are kept, the ones between are blended, and the
         amplitude is 0.1 ln(yarn) + 1."""
-        import torch
         if rotary_dim < 2 or rotary_dim % 2:
             raise ValueError("rotary_dim must be a positive even number")
         half = rotary_dim // 2
@@ -167,9 +176,10 @@ class RopeTable:
                          interleaved)
 
 
-def _norm(w, dim: int, what: str):
-    if w is None:
-        return None
+_NO_ROPE = (0, None, None, 0, 0)
+
+
+def _norm(w, dim: int, what: str) -> int:
     _cuda(w, "float32", 1, what)
     _need(w.shape[0] == dim and w.is_contiguous(), f"{what} must be a contiguous [head_dim]")
     return w.data_ptr()
@@ -181,42 +191,42 @@ def rope_append(device: Device, q, k, v, cache: KvCache, batch: KvBatch, rope: O
     allowed) are normalised per head (weights q_norm / k_norm [D] float32; None: not), turned to their positions (int32
     [n], rows of the table; None: each key's index) and rounded to bfloat16; q goes to q_out, k and v into the cache.
     rope None: nothing turns."""
-    dtype = str(q.dtype)[6:]
-    if dtype not in ("float32", "bfloat16"):
-        raise TypeError(f"q, k and v must be float32 or bfloat16, got {q.dtype}")
-    for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        _cuda(t, dtype, 3, what)
-    _cuda(q_out, "bfloat16", 3, "q_out")
-    n, heads, dim = q.shape
-    kv = (n, cache.n_kv_heads, cache.head_dim)
-    _need(dim == cache.head_dim and k.shape == kv and v.shape == kv, "q [n, Hq, D], k and v [n, Hkv, D] of the cache's Hkv and D")
-    _need(q_out.shape == q.shape, "q_out must have q's shape")
+    dtype, shape = q.dtype, q.shape
+    if dtype is not _BF16 and dtype is not _F32:
+        raise TypeError(f"q, k and v must be float32 or bfloat16, got {dtype}")
+    n, heads, dim = shape if len(shape) == 3 else (0, 0, -1)
+    _need(dim == cache.head_dim, "q must be [n, Hq, D] of the cache's D")
+    kv = (n, cache.n_kv_heads, dim)
+    q_ptr, q_row, q_head = _rows(q, dtype, shape, "q")
+    k_ptr, k_row, k_head = _rows(k, dtype, kv, "k")
+    v_ptr, v_row, v_head = _rows(v, dtype, kv, "v")
+    out_ptr, out_row, out_head = _rows(q_out, _BF16, shape, "q_out")
+    at = None
     if positions is not None:
         _cuda(positions, "int32", 1, "positions")
         _need(positions.shape[0] == n and positions.is_contiguous(), "positions must be a contiguous [n]")
-    if rope is None:
-        n_positions, cos, sin, rotary, interleaved = 0, None, None, 0, 0
-    else:
-        (n_positions, cos, sin), rotary, interleaved = rope._c, rope.rotary_dim, rope.interleaved
-    rows = VwRopeRows(q.data_ptr(), k.data_ptr(), v.data_ptr(), *_strides(q, "q"), *_strides(k, "k"), *_strides(v, "v"),
-                      VW_F32 if dtype == "float32" else VW_BF16, heads, _norm(q_norm, dim, "q_norm"),
-                      _norm(k_norm, dim, "k_norm"), eps, n_positions, cos, sin,
-                      None if positions is None else positions.data_ptr(), rotary, interleaved, q_out.data_ptr(),
-                      *_strides(q_out, "q_out"))
+        at = positions.data_ptr()
+    n_positions, cos, sin, rotary, interleaved = _NO_ROPE if rope is None else rope._c
+    rows = VwRopeRows(q_ptr, k_ptr, v_ptr, q_row, q_head, k_row, k_head, v_row, v_head,
+                      VW_F32 if dtype is _F32 else VW_BF16, heads, None if q_norm is None else _norm(q_norm, dim, "q_norm"),
+                      None if k_norm is None else _norm(k_norm, dim, "k_norm"), eps, n_positions, cos, sin, at, rotary,
+                      interleaved, out_ptr, out_row, out_head)
     check(lib.vw_rope_append(device.handle, cache._ref, batch._rows(n), ctypes.byref(rows), stream), device.handle)
 
 
 def _attn_rows(q, out, lse, cache: KvCache, scale: Optional[float]):
-    _cuda(q, "bfloat16", 3, "q")
-    _cuda(out, "bfloat16", 3, "out")
-    n, heads, dim = q.shape
+    shape = q.shape
+    n, heads, dim = shape if len(shape) == 3 else (0, 0, -1)
     _need(dim == cache.head_dim, "q must be [n, Hq, D] of the cache's D")
-    _need(out.shape == q.shape, "out must have q's shape")
+    q_ptr, q_row, q_head = _rows(q, _BF16, shape, "q")
+    out_ptr, out_row, out_head = _rows(out, _BF16, shape, "out")
+    lse_ptr = None
     if lse is not None:
         _cuda(lse, "float32", 2, "lse")
         _need(lse.shape == (n, heads) and lse.is_contiguous(), "lse must be a contiguous [n, Hq]")
-    return VwAttnRows(q.data_ptr(), *_strides(q, "q"), heads, dim ** -0.5 if scale is None else scale, out.data_ptr(),
-                      *_strides(out, "out"), None if lse is None else lse.data_ptr())
+        lse_ptr = lse.data_ptr()
+    return n, VwAttnRows(q_ptr, q_row, q_head, heads, dim ** -0.5 if scale is None else scale, out_ptr, out_row, out_head,
+                         lse_ptr)
 
 
 def prompt_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, scale: Optional[float] = None, lse=None,
@@ -224,8 +234,8 @@ def prompt_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, sca
     """vw_prompt_attention: causal attention of packed sequences over their keys in the cache.  q and out
     [n, n_q_heads, D] bfloat16 (batch.q_offsets gives each sequence's rows, its last keys), scale 1/sqrt(D) unless
     given, lse optionally [n, n_q_heads] float32.  Rows that see no key get 0 and -inf."""
-    rows = _attn_rows(q, out, lse, cache, scale)
-    check(lib.vw_prompt_attention(device.handle, cache._ref, batch._rows(q.shape[0]), ctypes.byref(rows), stream),
+    n, rows = _attn_rows(q, out, lse, cache, scale)
+    check(lib.vw_prompt_attention(device.handle, cache._ref, batch._rows(n), ctypes.byref(rows), stream),
           device.handle)
 
 
@@ -233,6 +243,6 @@ def decode_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, pre
                      scale: Optional[float] = None, lse=None, stream: Optional[int] = None) -> None:
     """vw_decode_attention: one row per sequence (row s is sequence s; batch.q_offsets is ignored) over all of its keys
     and, with `prefix`, those its group shares, which are read once for the group.  Tensors as in prompt_attention."""
-    rows = _attn_rows(q, out, lse, cache, scale)
-    check(lib.vw_decode_attention(device.handle, cache._ref, batch._rows(q.shape[0]),
+    n, rows = _attn_rows(q, out, lse, cache, scale)
+    check(lib.vw_decode_attention(device.handle, cache._ref, batch._rows(n),
                                   None if prefix is None else prefix._ref, ctypes.byref(rows), stream), device.handle)

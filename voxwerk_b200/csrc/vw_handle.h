@@ -56,6 +56,11 @@ class DeviceGuard {
   public:
     explicit DeviceGuard(int dev) {
         if (cudaGetDevice(&prev_) != cudaSuccess) prev_ = -1;
+        if (prev_ == dev) {   // nothing to set or to restore
+            prev_ = -1;
+            ok_ = true;
+            return;
+        }
         ok_ = cudaSetDevice(dev) == cudaSuccess;
     }
     ~DeviceGuard() {
