@@ -130,6 +130,12 @@ struct DecodeWork {
 DecodePlan plan_decode(const AttnParams& p, int sms);
 cudaError_t launch_decode_attention(const AttnParams& p, const DecodePlan& plan, const DecodeWork& w, cudaStream_t stream);
 
+// Threads of a join block: one for every four dims of the query heads of a key head, at most 256 at a time
+inline int join_threads(int group, int dim) {
+    const int n = (group * dim / 4 + 31) / 32 * 32;
+    return n < 256 ? n : 256;
+}
+
 #ifdef __CUDACC__
 // A sequence's key count, held inside its page table; a count outside it is reported and clamped.
 __device__ __forceinline__ int checked_len(int len, int max_pages, int page_shift, unsigned* err, unsigned bit) {
@@ -277,58 +283,43 @@ __device__ PieceSpan piece_span(const AttnParams& a, const TileWork& w, int s, i
     return at;
 }
 
-// A row's partial results weighed together by one warp, DIM / 32 dims a lane: o = sum_i 2^(lse_i - m) o_i / l,
-// l = sum_i 2^(lse_i - m).
+// Four dims of a row's partial results weighed together by one thread: o = sum_i 2^(lse_i - m) o_i / l,
+// l = sum_i 2^(lse_i - m).  The pieces' loads do not wait for one another.
 template <int DIM>
 struct PartSum {
-    static constexpr int kDims = DIM / 32;
-    float m = -INFINITY, l = 0.0f, o[kDims] = {};
+    float m = -INFINITY, l = 0.0f;
+    float4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 
-    // pieces c0 .. c1, piece c at partial row base + c * stride
-    __device__ void add(const float* part_lse, const float* part_o, int64_t base, int stride, int c0, int c1, int lane) {
-        for (int c = c0; c <= c1; c += 32) {
-            const int n = min(32, c1 - c + 1);
-            const float lse = lane < n ? part_lse[base + static_cast<int64_t>(c + lane) * stride] : -INFINITY;
-            float top = lse;
-#pragma unroll
-            for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
-            raise(top);
-            const float mine = m == -INFINITY ? 0.0f : exp2f(lse - m);
+    // pieces c0 .. c1, piece c at partial row base + c * stride, of it dims d .. d + 3
+    __device__ void add(const float* part_lse, const float* part_o, int64_t base, int stride, int c0, int c1, int d) {
+        float top = m;
 #pragma unroll 4
-            for (int i = 0; i < n; ++i) {
-                const float f = __shfl_sync(0xffffffffu, mine, i);
-                const float* src = part_o + (base + static_cast<int64_t>(c + i) * stride) * DIM + lane * kDims;
-                float x[kDims];
-                if constexpr (kDims == 4) {
-                    const float4 v = *reinterpret_cast<const float4*>(src);
-                    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-                } else {
-                    const float2 v = *reinterpret_cast<const float2*>(src);
-                    x[0] = v.x, x[1] = v.y;
-                }
-                l += f;
-#pragma unroll
-                for (int d = 0; d < kDims; ++d) o[d] = __fmaf_rn(f, x[d], o[d]);
-            }
+        for (int c = c0; c <= c1; ++c) top = fmaxf(top, part_lse[base + static_cast<int64_t>(c) * stride]);
+        const float f = m == -INFINITY ? 0.0f : exp2f(m - top);
+        m = top;
+        l *= f;
+        o.x *= f, o.y *= f, o.z *= f, o.w *= f;
+#pragma unroll 4
+        for (int c = c0; c <= c1; ++c) {
+            const int64_t row = base + static_cast<int64_t>(c) * stride;
+            const float lse = part_lse[row];
+            const float4 v = *reinterpret_cast<const float4*>(part_o + row * DIM + d);
+            const float w = lse == -INFINITY ? 0.0f : exp2f(lse - top);   // (not a number stays one)
+            l += w;
+            o.x = __fmaf_rn(w, v.x, o.x);
+            o.y = __fmaf_rn(w, v.y, o.y);
+            o.z = __fmaf_rn(w, v.z, o.z);
+            o.w = __fmaf_rn(w, v.w, o.w);
         }
     }
-    __device__ void raise(float top) {
-        if (top > m) {
-            const float f = m == -INFINITY ? 0.0f : exp2f(m - top);
-            l *= f;
-#pragma unroll
-            for (int d = 0; d < kDims; ++d) o[d] *= f;
-            m = top;
-        }
-    }
-    __device__ void write(const AttnParams& p, int64_t row, int head, int lane) {
+    __device__ void write(const AttnParams& p, int64_t row, int head, int d) {
         const float r = l == 0.0f ? 0.0f : 1.0f / l;
-        __nv_bfloat16* out = p.rows.out + row * p.rows.out_row + head * p.rows.out_head + lane * kDims;
-        if (lane * kDims < p.cache.head_dim)
-#pragma unroll
-            for (int d = 0; d < kDims; d += 2)
-                *reinterpret_cast<__nv_bfloat162*>(out + d) = __floats2bfloat162_rn(o[d] * r, o[d + 1] * r);
-        if (p.rows.lse && lane == 0)
+        if (d < p.cache.head_dim) {
+            __nv_bfloat162 v[2] = {__floats2bfloat162_rn(o.x * r, o.y * r), __floats2bfloat162_rn(o.z * r, o.w * r)};
+            *reinterpret_cast<uint2*>(p.rows.out + row * p.rows.out_row + head * p.rows.out_head + d) =
+                *reinterpret_cast<const uint2*>(v);
+        }
+        if (p.rows.lse && d == 0)
             p.rows.lse[row * p.rows.n_q_heads + head] = (m + log2f(l)) * 0.693147180559945309f;
     }
 };

@@ -480,10 +480,11 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
             }
             sync_consumers();
             if (*last)
-                for (int r = w; r < live_rows; r += 4) {
+                for (int i = threadIdx.x - 32; i < live_rows * (DP / 4); i += 128) {
+                    const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
                     PartSum<DP> sum;
-                    sum.add(p.w.part_lse, p.w.part_o, part0 + r, rows, it.c0, it.c1, lane);
-                    sum.write(p.a, it.seq, head0 + r, lane);
+                    sum.add(p.w.part_lse, p.w.part_o, part0 + r, rows, it.c0, it.c1, d);
+                    sum.write(p.a, it.seq, head0 + r, d);
                 }
         }
     }   // (the next item's first barrier comes before its writes to the scratch)
@@ -491,31 +492,30 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
     if (p.has_prefix) asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
-// With prefixes: a row's own pieces and those of its group's prefix, one warp per (sequence, query head).
+// With prefixes: the rows' own pieces and those of their group's prefix, a block for each sequence and key head.
 template <int DP>
-__global__ void __launch_bounds__(128) decode_join_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant__ DecodeParams p) {
     const AttnParams& a = p.a;
-    const int lane = threadIdx.x & 31, heads = a.rows.n_q_heads;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int s = static_cast<int>(i / heads), head = static_cast<int>(i % heads);
-    if (s >= a.batch.n_seqs) return;
+    const int lane = threadIdx.x & 31, kv_heads = a.cache.n_kv_heads;
+    const int s = blockIdx.x / kv_heads, kv_head = blockIdx.x % kv_heads, head0 = kv_head * p.group;
     const int g = find_sequence(a.prefix.group_offsets, a.prefix.n_groups, s, lane);
     const int keys = checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, a.cache.page_shift, a.err, kErrKvLens);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int kv_head = head / p.group, sub = head % p.group, row_block = sub / kMaxRows;
     const int chunk = *p.w.chunk, units = max((keys + kKeys * chunk - 1) / (kKeys * chunk), 1);
-    const int j = kv_head * p.plan.row_blocks + row_block;
-    const int64_t per = *p.w.units_per_cta, first = (s > 0 ? p.w.unit_end[s - 1] : 0) + static_cast<int64_t>(j) * units;
-    const int64_t item = static_cast<int64_t>(s) * a.cache.n_kv_heads * p.plan.row_blocks + j;
-    PartSum<DP> sum;
-    sum.add(p.w.part_lse, p.w.part_o, item * p.plan.rows + sub % kMaxRows, p.plan.rows, static_cast<int>(divide(first, per)),
-            static_cast<int>(divide(first + units - 1, per)), lane);
-    if (g >= 0) {
-        const PieceSpan at = piece_span<true>(a, p.w.prefix, g, s, head, p.tile_tokens);
-        if (at.c0 <= at.c1)
-            sum.add(p.w.prefix.part_lse, p.w.prefix.part_o, at.base, kPartRows, at.c0, at.c1, lane);
+    const int64_t per = *p.w.units_per_cta, first_of_seq = s > 0 ? p.w.unit_end[s - 1] : 0;
+    PieceSpan at{0, 1, 0};
+    if (g >= 0) at = piece_span<true>(a, p.w.prefix, g, s, head0, p.tile_tokens);
+    for (int i = threadIdx.x; i < p.group * (DP / 4); i += blockDim.x) {
+        const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
+        const int j = kv_head * p.plan.row_blocks + r / kMaxRows;
+        const int64_t first = first_of_seq + static_cast<int64_t>(j) * units;
+        const int64_t item = static_cast<int64_t>(s) * kv_heads * p.plan.row_blocks + j;
+        PartSum<DP> sum;
+        sum.add(p.w.part_lse, p.w.part_o, item * p.plan.rows + r % kMaxRows, p.plan.rows,
+                static_cast<int>(divide(first, per)), static_cast<int>(divide(first + units - 1, per)), d);
+        if (at.c0 <= at.c1) sum.add(p.w.prefix.part_lse, p.w.prefix.part_o, at.base + r, kPartRows, at.c0, at.c1, d);
+        sum.write(a, s, head0 + r, d);
     }
-    sum.write(a, s, head, lane);
 }
 
 template <int DP>
@@ -548,8 +548,8 @@ cudaError_t launch_dim(DecodeParams& p, cudaStream_t stream) {
     cfg.numAttrs = p.has_prefix ? 1 : 0;
     e = cudaLaunchKernelEx(&cfg, decode_kernel<DP>, q, k, v, p);
     if (e != cudaSuccess || !p.has_prefix) return e;
-    cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.a.batch.n_seqs) * p.a.rows.n_q_heads + 3) / 4));
-    cfg.blockDim = dim3(128);
+    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(p.a.batch.n_seqs) * p.a.cache.n_kv_heads));
+    cfg.blockDim = dim3(join_threads(p.group, DP));
     cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, decode_join_kernel<DP>, p);
 }

@@ -380,8 +380,9 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     unsigned* err = p.a.err;
     const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
-    // the decode kernel that follows the prefixes' may take the SMs as they come free (it waits before it reads here)
-    if (kPrefix) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    // the kernel that follows (the decode kernel behind the prefixes', the join) may take the SMs as they come free; it
+    // waits before it reads here
+    if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (threadIdx.x == 0) {
         auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
         for (int s = 0; s < 4 * S; ++s) init(k_full + 8 * s, 1);
@@ -826,21 +827,22 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     }
 }
 
-// Joins the pieces of the blocks that were split: one warp per (row, query head).
+// Joins the pieces of the blocks that were split: a block for each row and key head.
 template <int DP>
-__global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ TileParams p) {
-    const int lane = threadIdx.x & 31;
-    const int heads = p.a.rows.n_q_heads;
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int row = static_cast<int>(item / heads), head = static_cast<int>(item % heads);
-    if (row >= p.a.batch.n_rows) return;
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ TileParams p) {
+    const int lane = threadIdx.x & 31, kv_heads = p.a.cache.n_kv_heads;
+    const int row = blockIdx.x / kv_heads, head0 = (blockIdx.x % kv_heads) * p.group;
     const int s = p.a.batch.q_offsets ? find_sequence(p.a.batch.q_offsets, p.a.batch.n_seqs, row, lane) : row;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (s < 0 || s >= p.a.batch.n_seqs) return;
-    const PieceSpan at = piece_span<false>(p.a, p.w, s, row, head, p.tile_tokens);
+    const PieceSpan at = piece_span<false>(p.a, p.w, s, row, head0, p.tile_tokens);
     if (at.c0 >= at.c1) return;   // whole (written by the tile kernel), or no row of the sequence
-    PartSum<DP> sum;
-    sum.add(p.w.part_lse, p.w.part_o, at.base, kPartRows, at.c0, at.c1, lane);
-    sum.write(p.a, row, head, lane);
+    for (int i = threadIdx.x; i < p.group * (DP / 4); i += blockDim.x) {
+        const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
+        PartSum<DP> sum;
+        sum.add(p.w.part_lse, p.w.part_o, at.base + r, kPartRows, at.c0, at.c1, d);
+        sum.write(p.a, row, head0 + r, d);
+    }
 }
 
 template <int DP, bool kPrefix>
@@ -918,13 +920,16 @@ cudaError_t launch_prompt_attention(const AttnParams& a, const TilePlan& plan, c
     cudaError_t e = plan.dim == 64 ? launch_tiles<64, false>(p, g, plan.grid, stream)
                                    : launch_tiles<128, false>(p, g, plan.grid, stream);
     if (e != cudaSuccess || !plan.split) return e;
-    const int64_t warps = static_cast<int64_t>(a.batch.n_rows) * a.rows.n_q_heads;
-    const unsigned grid = static_cast<unsigned>((warps + 3) / 4);
-    if (plan.dim == 64)
-        join_kernel<64><<<grid, 128, 0, stream>>>(p);
-    else
-        join_kernel<128><<<grid, 128, 0, stream>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.batch.n_rows) * a.cache.n_kv_heads));
+    cfg.blockDim = dim3(join_threads(g.group, plan.dim));
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // its blocks are there when the tile kernel ends
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return plan.dim == 64 ? cudaLaunchKernelEx(&cfg, join_kernel<64>, p) : cudaLaunchKernelEx(&cfg, join_kernel<128>, p);
 }
 
 }  // namespace vw
