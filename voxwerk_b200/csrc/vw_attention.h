@@ -230,23 +230,25 @@ __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusi
 
 // SMs for the prefixes' tile kernel; the decode kernel, launched behind it, takes the others at once (all when this is
 // all, after the prefixes).  It is bound by HBM and reaches that rate with some 80 of 148 SMs, the prefixes by the SMs, so
-// the two overlap well.  Of 32 counts the one whose later end comes first, by what was measured of each: 12 us and then
-// 1.6 us a unit for a prefix CTA (17 us and 2.45 us where blocks have two row tiles); 8 us, then 64-key tiles at 6.5 TB/s
-// or 0.5 us each on an SM, for the sequences' own keys.  Every CTA of both kernels comes to the same count.
+// the two overlap well.  Of 32 counts the one whose later end comes first, by what was measured of each: 10 us and then
+// 1.7 us a unit for a prefix CTA (16 us and 2.3 us where blocks have two row tiles); 7 us, then 64-key tiles at 6.5 TB/s
+// or 0.45 us each on an SM, an item's end counted as two, for the sequences' own keys.  Every CTA of both kernels comes to
+// the same count.
 __device__ __forceinline__ int prefix_ctas(const AttnParams& a, int64_t units, int sms, int lane) {
     const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
     int tiles = 0;
     for (int s = lane; s < a.batch.n_seqs; s += 32)
         tiles += ceil_div(checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, a.cache.page_shift, a.err,
                                       kErrKvLens), 64);
-    const float own_tiles = static_cast<float>(__reduce_add_sync(0xffffffffu, tiles)) *
-                            (a.cache.n_kv_heads * ((group + 15) / 16));
+    const float items = static_cast<float>(a.cache.n_kv_heads * ((group + 15) / 16));   // of a sequence
+    const float own_tiles = static_cast<float>(__reduce_add_sync(0xffffffffu, tiles)) * items;
+    const float own_units = own_tiles + 2.0f * items * static_cast<float>(a.batch.n_seqs);
     const int mine = (sms * (lane + 1)) >> 5;
     const bool two = a.batch.n_seqs * group > kTileRows;
-    const float prefix_us = (two ? 17.0f : 12.0f) + static_cast<float>(units) * (two ? 2.45f : 1.6f) / static_cast<float>(mine);
+    const float prefix_us = (two ? 16.0f : 10.0f) + static_cast<float>(units) * (two ? 2.3f : 1.7f) / static_cast<float>(mine);
     const float hbm_us = own_tiles * (256.0f * a.cache.head_dim) / 6.5e6f;
     const int rest = mine < sms ? sms - mine : sms;
-    const float own_us = 8.0f + fmaxf(hbm_us, own_tiles * 0.5f / static_cast<float>(rest));
+    const float own_us = 7.0f + fmaxf(hbm_us, own_units * 0.45f / static_cast<float>(rest));
     const float us = mine == 0 ? 1e30f : mine < sms ? fmaxf(prefix_us, own_us) : prefix_us + own_us;
     const unsigned best = __reduce_min_sync(0xffffffffu, __float_as_uint(us));   // (positive floats order as integers)
     const unsigned m = __ballot_sync(0xffffffffu, __float_as_uint(us) == best);

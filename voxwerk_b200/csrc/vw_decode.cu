@@ -32,6 +32,7 @@ constexpr int kThreads = 160;     // producer warp, four warps of 16 keys
 constexpr int kKeys = 64;         // keys per tile
 constexpr int kMaxRows = 16;      // query heads per item: the rows of an mma
 constexpr int kItemSlots = 2;
+constexpr int kItemUnits = 2;     // an item's end costs about what two tiles do
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr uint32_t kSmemBudget = 113 * 1024;   // two CTAs per SM
 
@@ -59,6 +60,11 @@ struct DecodeCfg {
     }
 };
 static_assert(DecodeCfg<128>::stages(16) >= 2 && DecodeCfg<64>::stages(16) >= 2, "ring");
+
+// Units of an item that are tiles; kItemUnits more stand for its end, so that a CTA with many short items has fewer tiles
+__device__ __forceinline__ int units_with_tiles(int keys, int chunk) {
+    return max((keys + kKeys * chunk - 1) / (kKeys * chunk), 1);
+}
 
 struct DecodeItem {
     int32_t valid, seq, kv_head, row_block;
@@ -178,8 +184,9 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         }
         const int64_t spare = static_cast<int64_t>(ctas) - p.plan.items;
         const int chunk = 2 * spare >= ctas ? static_cast<int>(max(divide(total_tiles + spare - 1, spare), int64_t{1})) : 1;
-        auto units_of = [&](int keys) { return max((keys + kKeys * chunk - 1) / (kKeys * chunk), 1); };
-        int64_t total = total_tiles;
+        const int end_units = chunk == 1 ? kItemUnits : 0;
+        auto units_of = [&](int keys) { return units_with_tiles(keys, chunk) + end_units; };
+        int64_t total = total_tiles + p.plan.items * end_units;
         if (chunk > 1) {
             int sum = 0;
             for (int s = lane; s < n_seqs; s += 32) sum += units_of(keys_of(s));
@@ -218,8 +225,7 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
         bool stop = false;
         while (!stop) {
             DecodeItem it;
-            it.valid = unit < unit_end;
-            if (it.valid) {
+            for (it.valid = 0; unit < unit_end && !it.valid;) {
                 int keys = keys_of(seq), units = units_of(keys);
                 while (unit >= first + static_cast<int64_t>(units) * per_seq) {
                     first += static_cast<int64_t>(units) * per_seq;
@@ -228,19 +234,21 @@ decode_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__
                 }
                 const int j = static_cast<int>(divide(unit - first, units));
                 const int64_t item_first = first + static_cast<int64_t>(j) * units;
-                const int tiles = max((keys + kKeys - 1) / kKeys, 1);
+                const int tiles = max((keys + kKeys - 1) / kKeys, 1), real = units - end_units;
                 const int u0 = static_cast<int>(unit - item_first);
                 const int u1 = static_cast<int>(min(unit_end - item_first, static_cast<int64_t>(units)));
+                unit = item_first + u1;
+                if (u0 >= real) continue;   // the end of an item whose tiles are another CTA's
+                it.valid = 1;
                 it.seq = seq;
                 it.kv_head = j / p.plan.row_blocks;
                 it.row_block = j % p.plan.row_blocks;
                 it.keys = keys;
                 it.tile0 = u0 * chunk;
-                it.tile1 = min(u1 * chunk, tiles);
+                it.tile1 = min(min(u1, real) * chunk, tiles);
                 it.c0 = static_cast<int>(divide(item_first, per));
-                it.c1 = static_cast<int>(divide(item_first + units - 1, per));
+                it.c1 = static_cast<int>(divide(item_first + real - 1, per));
                 it.index = seq * per_seq + j;
-                unit = item_first + u1;
             }
             const uint32_t slot = n_items % kItemSlots;
             if (n_items >= kItemSlots && !wait_bounded(item_empty + 8 * slot, (n_items / kItemSlots - 1) & 1, abort, err))
@@ -501,7 +509,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
     const int g = find_sequence(a.prefix.group_offsets, a.prefix.n_groups, s, lane);
     const int keys = checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, a.cache.page_shift, a.err, kErrKvLens);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int chunk = *p.w.chunk, units = max((keys + kKeys * chunk - 1) / (kKeys * chunk), 1);
+    const int chunk = *p.w.chunk, real = units_with_tiles(keys, chunk), units = real + (chunk == 1 ? kItemUnits : 0);
     const int64_t per = *p.w.units_per_cta, first_of_seq = s > 0 ? p.w.unit_end[s - 1] : 0;
     PieceSpan at{0, 1, 0};
     if (g >= 0) at = piece_span<true>(a, p.w.prefix, g, s, head0, p.tile_tokens);
@@ -512,7 +520,7 @@ __global__ void __launch_bounds__(256) decode_join_kernel(const __grid_constant_
         const int64_t item = static_cast<int64_t>(s) * kv_heads * p.plan.row_blocks + j;
         PartSum<DP> sum;
         sum.add(p.w.part_lse, p.w.part_o, item * p.plan.rows + r % kMaxRows, p.plan.rows,
-                static_cast<int>(divide(first, per)), static_cast<int>(divide(first + units - 1, per)), d);
+                static_cast<int>(divide(first, per)), static_cast<int>(divide(first + real - 1, per)), d);
         if (at.c0 <= at.c1) sum.add(p.w.prefix.part_lse, p.w.prefix.part_o, at.base + r, kPartRows, at.c0, at.c1, d);
         sum.write(a, s, head0 + r, d);
     }
