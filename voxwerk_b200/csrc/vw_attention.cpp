@@ -277,6 +277,7 @@ VW_EXPORT vw_status vw_decode_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (r != VW_OK) return r;
     if (p.prefix.n_groups > 0) e = vw::launch_prefix_attention(p, prefix_plan, w.prefix, st);
     if (e == cudaSuccess) e = vw::launch_decode_attention(p, plan, w, st);
+    if (e != cudaSuccess) cudaMemsetAsync(h->d_attn_counts, 0, h->attn_counts_bytes, st);   // the join would have
     if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
     if (e != cudaSuccess) return cuda_fail(h, e, "decode attention");
     if (!stream) return read_device_error(h, st);

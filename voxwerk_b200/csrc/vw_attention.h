@@ -84,7 +84,7 @@ struct TilePlan {
     int64_t unit_ends;
 };
 struct TileWork {
-    int32_t* counters;          // [2] tickets taken, CTAs done; both 0 between calls
+    int32_t* counters;          // [3] tickets taken, CTAs done, CTAs of the decode kernel with units; 0 between calls
     int64_t* units_per_cta;
     int64_t* unit_end;          // [sequences or groups] units up to and including each
     float* part_lse;            // [part_rows] log2 of each partial row's sum, -inf: no key
@@ -219,13 +219,39 @@ __device__ __forceinline__ int64_t divide(int64_t a, int64_t b) {
     if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
     return a / b;
 }
-__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusive
+template <typename T>
+__device__ __forceinline__ T warp_scan(T x, int lane) {   // inclusive
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+        const T y = __shfl_up_sync(0xffffffffu, x, o);
         if (lane >= o) x += y;
     }
     return x;
+}
+
+// The lengths that a CTA's schedule begins with, asked for while it still sets up
+__device__ __forceinline__ void prefetch_lengths(const AttnParams& a, int lane) {
+    for (int s = 32 * lane; s < a.batch.n_seqs; s += 32 * 32)   // (a line holds 32)
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.batch.kv_lens + s));
+    if (lane == 0 && a.prefix.n_groups > 0) {
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.prefix.lens));
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(a.prefix.group_offsets));
+    }
+}
+// 64-key tiles of the sequences' own keys, one at least of each, for one key head.  (Together they fit 32 bits: 2^31 of
+// them would be 2^37 keys.)
+__device__ __forceinline__ int own_tiles(const AttnParams& a, int lane) {
+    int tiles = 0;
+    for (int s0 = lane; s0 < a.batch.n_seqs; s0 += 4 * 32) {
+        int len[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) len[i] = s0 + 32 * i < a.batch.n_seqs ? __ldg(a.batch.kv_lens + s0 + 32 * i) : -1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (s0 + 32 * i < a.batch.n_seqs)
+                tiles += max(ceil_div(checked_len(len[i], a.batch.max_pages, a.cache.page_shift, a.err, kErrKvLens), 64), 1);
+    }
+    return __reduce_add_sync(0xffffffffu, tiles);
 }
 
 // SMs for the prefixes' tile kernel; the decode kernel, launched behind it, takes the others at once (all when this is
@@ -235,14 +261,10 @@ __device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {   // inclusi
 // or 0.45 us each on an SM, an item's end counted as two, for the sequences' own keys.  Every CTA of both kernels comes to
 // the same count.  With 0.42 and 0.5 us in place of 0.45 (16 query heads on 8 of 128 dims): 256 sequences on a prefix of
 // 16001 153 and 155 us against 143, 64 on one of 4099 36.0 and 36.3 against 36.3, 50 on four 27.7 and 26.9 against 27.6.
-__device__ __forceinline__ int prefix_ctas(const AttnParams& a, int64_t units, int sms, int lane) {
+__device__ __forceinline__ int prefix_ctas(const AttnParams& a, int64_t units, int tiles, int sms, int lane) {
     const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
-    int tiles = 0;
-    for (int s = lane; s < a.batch.n_seqs; s += 32)
-        tiles += ceil_div(checked_len(__ldg(a.batch.kv_lens + s), a.batch.max_pages, a.cache.page_shift, a.err,
-                                      kErrKvLens), 64);
     const float items = static_cast<float>(a.cache.n_kv_heads * ((group + 15) / 16));   // of a sequence
-    const float own_tiles = static_cast<float>(__reduce_add_sync(0xffffffffu, tiles)) * items;
+    const float own_tiles = static_cast<float>(tiles) * items;
     const float own_units = own_tiles + 2.0f * items * static_cast<float>(a.batch.n_seqs);
     const int mine = (sms * (lane + 1)) >> 5;
     const bool two = a.batch.n_seqs * group > kTileRows;

@@ -146,6 +146,7 @@ struct Scheduler {
             const auto units_of = [&](int s) {
                 return s < n_seqs ? seq_units<kPrefix>(load_seq<kPrefix>(p.a, s), block_tokens, kv_heads) : 0;
             };
+            const int tiles = kPrefix ? own_tiles(p.a, lane) : 0;
             int64_t total = 0, u = 0, sum = 0;
             for (int s0 = 0; s0 < n_seqs; s0 += 32) {
                 const int s = s0 + lane;
@@ -154,7 +155,7 @@ struct Scheduler {
                 if (blockIdx.x == 0 && s < n_seqs) p.w.unit_end[s] = total + sum;   // for the kernels that join
                 total += __shfl_sync(0xffffffffu, sum, 31);
             }
-            const int ctas = kPrefix ? prefix_ctas(p.a, total, gridDim.x, lane) : gridDim.x;
+            const int ctas = kPrefix ? prefix_ctas(p.a, total, tiles, gridDim.x, lane) : gridDim.x;
             const int64_t per = max(divide(total + ctas - 1, ctas), static_cast<int64_t>(p.min_units));
             if (blockIdx.x == 0 && lane == 0) *p.w.units_per_cta = per;
             unit = min(per * blockIdx.x, total);
@@ -389,6 +390,7 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     // the kernel that follows (the decode kernel behind the prefixes', the join) may take the SMs as they come free; it
     // waits before it reads here
     if (p.split) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (kPrefix && warp == 3) prefetch_lengths(p.a, lane);
     if (threadIdx.x == 0) {
         auto init = [](uint32_t bar, int n) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(n)); };
         for (int s = 0; s < 4 * S; ++s) init(k_full + 8 * s, 1);
