@@ -14,8 +14,9 @@
 // prefixes every item leaves its result there, and a join kernel weighs it with the prefix's.
 //
 // Measured (16 query heads on 8 of 128 dims, prefixes included): 256 sequences of 100-2000 keys on a prefix of 16001
-// 143 us = 5.1 TB/s; 64 of 20-600 on one of 4099 37 us, 50 of 60-900 on four prefixes (32 heads on 4 of 64) 28 us, one of
-// 700 10.6 us (both kernels' start, the items' ends and the join, about 7 us of each, are what is left).
+// 142 us = 5.1 TB/s; 64 of 20-600 on one of 4099 34.5 us, 50 of 60-900 on four prefixes (32 heads on 4 of 64) 23.6 us, one
+// of 700 10.5 us (of the 64's: the prefix kernel's other CTAs leave after 3 us, a schedule takes 4, the first tile is there
+// 2 us later, an item's end costs 0.9 and the join 4).
 //
 // Every mbarrier wait is bounded.
 
@@ -36,7 +37,7 @@ constexpr int kThreads = 160;     // producer warp, four warps of 16 keys
 constexpr int kKeys = 64;         // keys per tile
 constexpr int kMaxRows = 16;      // query heads per item: the rows of an mma
 constexpr int kItemSlots = 2;
-constexpr int kItemUnits = 2;     // an item's end costs about what two tiles do (64 sequences: 36 us, 40 us without)
+constexpr int kItemUnits = 2;     // an item's end costs about what two tiles do (64 sequences: 36 us, 40 without)
 constexpr float kLn2 = 0.693147180559945309f;
 constexpr uint32_t kSmemBudget = 113 * 1024;   // two CTAs per SM
 
