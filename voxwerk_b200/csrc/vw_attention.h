@@ -259,8 +259,9 @@ __device__ __forceinline__ int own_tiles(const AttnParams& a, int lane) {
 // the two overlap well.  Of 32 counts the one whose later end comes first, by what was measured of each: 10 us and then
 // 1.7 us a unit for a prefix CTA (16 us and 2.3 us where the mean group fills two row tiles: 50 sequences in four groups
 // 23.6 us, 27.4 us with the latter); 7 us, then 64-key tiles at 6.5 TB/s or 0.45 us each on an SM, an item's end counted
-// as two, for the sequences' own keys.  Every CTA of both kernels comes to the same count.  With 0.42 and 0.5 us in place of 0.45 (16 query heads on 8 of 128 dims): 256 sequences on a prefix of
-// 16001 153 and 155 us against 142, 64 on one of 4099 33.8 and 34.5 against 34.5.
+// as two, for the sequences' own keys.  Every CTA of both kernels comes to the same count.  With 0.42 and 0.5 us in place of
+// 0.45 (16 query heads on 8 of 128 dims): 256 sequences on a prefix of 16001 153 and 155 us against 142, 64 on one of 4099
+// 33.8 and 34.5 against 34.5.
 __device__ __forceinline__ int prefix_ctas(const AttnParams& a, int64_t units, int tiles, int sms, int lane) {
     const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
     const float items = static_cast<float>(a.cache.n_kv_heads * ((group + 15) / 16));   // of a sequence

@@ -132,7 +132,8 @@ struct Scheduler {
     // by ticket
     int ticket, level, base;
     int64_t before;
-    Seq own;                             // sequence `lane`
+    Seq own;                             // sequence `lane`, its lowest level and blocks
+    int own_level, own_blocks;
     bool taken = false;                  // the first ticket is the CTA's number
     // split
     int64_t unit, unit_end, seq_first;   // the CTA's units; the first unit of sequence `seq`
@@ -179,9 +180,11 @@ struct Scheduler {
         } else {
             ticket = blockIdx.x;
             own = lane < n_seqs ? load_seq<kPrefix>(p.a, lane) : Seq{0, 0, 0, 0};
-            int top = -1;
-            for (int s = lane; s < n_seqs; s += 32) {
-                const Seq q = s < 32 ? own : load_seq<kPrefix>(p.a, s);
+            own_level = first_level(own);
+            own_blocks = ceil_div(own.n, block_tokens);
+            int top = own_blocks > 0 ? own_level + own_blocks - 1 : -1;
+            for (int s = lane + 32; s < n_seqs; s += 32) {
+                const Seq q = load_seq<kPrefix>(p.a, s);
                 if (q.n > 0) top = max(top, first_level(q) + ceil_div(q.n, block_tokens) - 1);
             }
             level = __reduce_max_sync(0xffffffffu, top);
@@ -201,19 +204,21 @@ struct Scheduler {
             ticket = __shfl_sync(0xffffffffu, ticket, 0);
         }
         taken = true;
+        const int wanted = ticket / kv_heads;   // among the (sequence, block) pairs
         while (level >= 0) {
-            const int s = base + lane;
-            Seq q{0, 0, 0, 0};
-            int i = -1;
-            if (s < n_seqs) {
-                q = base == 0 ? own : load_seq<kPrefix>(p.a, s);
+            Seq q = own;
+            int i = level - own_level, blocks = own_blocks;
+            if (base > 0) {
+                q = base + lane < n_seqs ? load_seq<kPrefix>(p.a, base + lane) : Seq{0, 0, 0, 0};
                 i = level - first_level(q);
-                if (q.n <= 0 || i >= ceil_div(q.n, block_tokens)) i = -1;
+                blocks = ceil_div(q.n, block_tokens);
             }
+            if (i >= blocks) i = -1;
             const unsigned m = __ballot_sync(0xffffffffu, i >= 0);
-            const int64_t slot = ticket / kv_heads - before;
+            const int64_t slot = wanted - before;
             if (slot < __popc(m)) {
-                const int at = __fns(m, 0, static_cast<int>(slot) + 1);
+                const int at =
+                    __ffs(__ballot_sync(0xffffffffu, i >= 0 && __popc(m & ((1u << lane) - 1)) == static_cast<int>(slot))) - 1;
                 q.row0 = __shfl_sync(0xffffffffu, q.row0, at);
                 q.n = __shfl_sync(0xffffffffu, q.n, at);
                 q.kv = __shfl_sync(0xffffffffu, q.kv, at);
