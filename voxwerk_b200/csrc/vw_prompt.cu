@@ -23,11 +23,11 @@
 // there are too few blocks for the SMs, the (block, tile) units are dealt evenly instead, a block's pieces leave
 // partial results (O / l and log2-sum in fp32), and a join kernel, or the decode kernel, weighs them together.
 //
-// Measured (16 query heads on 8 of 128 dims): one prompt of 7937 235 us = 1.09 PFLOP/s at the 1.63 GHz that its power
-// allows (bound: a row tile's exponentials and its two products take turns; the pipe of the exponentials is 50 % busy, the
-// tensor cores 49 %); 12 prompts of 170-1300 tokens 46.5 us = 0.39 PFLOP/s (bound: three short blocks an SM, each with
-// 5-8 us before its first product and after its last); one of 37 10 us (latency of one block).  32 heads on 4 of 64:
-// pieces of 130-250 on 9001 cached keys 56 us = 0.42 PFLOP/s (bound: exponentials, twice as many a flop as with 128).
+// Measured (16 query heads on 8 of 128 dims): one prompt of 7937 216 us = 1.19 PFLOP/s at the clock that its power
+// allows (bound: a row tile's exponentials and its two products take turns, half of the time each); 12 prompts of 170-1300
+// tokens 43.3 us = 0.42 PFLOP/s (bound: three short blocks an SM, each with
+// 5-8 us before its first product and after its last); one of 37 9.6 us (latency of one block).  32 heads on 4 of 64:
+// pieces of 130-250 on 9001 cached keys 55 us = 0.42 PFLOP/s (bound: exponentials, twice as many a flop as with 128).
 //
 // Every mbarrier wait is bounded; on expiry an error bit is set, every role stops and drains, tensor memory is freed.
 
@@ -131,7 +131,7 @@ struct Scheduler {
     int lane, n_seqs, block_tokens, kv_heads;
     // by ticket
     int ticket, level, base;
-    int64_t before;
+    int32_t before;
     Seq own;                             // sequence `lane`, its lowest level and blocks
     int own_level, own_blocks;
     bool taken = false;                  // the first ticket is the CTA's number
@@ -215,10 +215,10 @@ struct Scheduler {
             }
             if (i >= blocks) i = -1;
             const unsigned m = __ballot_sync(0xffffffffu, i >= 0);
-            const int64_t slot = wanted - before;
+            const int slot = wanted - before;
             if (slot < __popc(m)) {
                 const int at =
-                    __ffs(__ballot_sync(0xffffffffu, i >= 0 && __popc(m & ((1u << lane) - 1)) == static_cast<int>(slot))) - 1;
+                    __ffs(__ballot_sync(0xffffffffu, i >= 0 && __popc(m & ((1u << lane) - 1)) == slot)) - 1;
                 q.row0 = __shfl_sync(0xffffffffu, q.row0, at);
                 q.n = __shfl_sync(0xffffffffu, q.n, at);
                 q.kv = __shfl_sync(0xffffffffu, q.kv, at);
@@ -514,8 +514,9 @@ attention_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         else loaded_k = st + 1;
                     }
                     page = next;
-                    // the next block is taken near the end of this one (early tickets would deal the blocks out as by turns)
-                    if (t == max(it.tile0, end - 2)) following = sched.next();
+                    // the next block is taken when this one's loads are issued: early tickets would deal the blocks out as by
+                    // turns, and before its last tile the search delayed that (a prompt of 7937: 217 us, 219 a tile before)
+                    if (t == end - 1) following = sched.next();
                 }
             }
             // teardown: the copies in flight land before the CTA may exit
