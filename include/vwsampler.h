@@ -347,7 +347,9 @@ vw_status vw_head_sample(vw_handle* handle, const void* hidden, int64_t hidden_s
  * offsets or group offsets that do not fit give VW_ERR_INVALID_ARG (the reference throws when a cache is full,
  * DecoderStack.cs:154).  Nothing outside the cache and the outputs is read or written in either case.
  * Calls of one handle on different streams are ordered by the library (they share the handle's workspace); work that a
- * caller captures into CUDA graphs it orders itself.
+ * caller captures into CUDA graphs it orders itself.  A capture cannot grow the workspace: an attention call that needs
+ * more than an earlier one outside a capture is refused there (VW_ERR_INVALID_ARG).  A workspace that a captured call
+ * uses stays until vw_destroy, whatever later calls need; graphs must not be replayed after that.
  */
 
 /* The cache: keys and values [n_pages, page_size, n_kv_heads, head_dim] bf16, by the strides given (elements, the same

@@ -1,0 +1,68 @@
+"""The attention operators in a user's hands: calls in graphs, on several streams, of sizes that change, and what they
+report, against the 64-bit forms of tests/attention_ref.py."""
+
+import pytest
+
+from tests import attention_ref as ref
+from tests.test_gpu_attention import Pool, _check_decode, _check_prompt, ints, offsets_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def fresh():
+    """A handle of its own, whose workspace has no size yet."""
+    from voxwerk_b200 import Device
+    with Device(0) as d:
+        yield d
+
+
+@pytest.mark.parametrize("prefixes", [[], [500]], ids=["own keys", "prefix"])
+def test_captured_step_outlives_the_workspace_it_was_captured_with(fresh, prefixes):
+    """A step is captured; eager calls that need more workspace follow; replays still give the formula's values."""
+    import torch
+    from voxwerk_b200 import KvBatch, KvPrefix, decode_attention, prompt_attention
+    pool = Pool(700, 16, 2, 128, seed=21)
+    lens = [700, 3, 450, 1200]
+    table = pool.table(lens)
+    ptable = pool.table(prefixes) if prefixes else None
+    groups = [0, 3] if prefixes else ()
+    prefix = KvPrefix(ptable, ints(prefixes), ints(groups)) if prefixes else None
+    q = pool.normal(4, 4, 128)
+    out = torch.full_like(q, 9.0)
+    batch = KvBatch(table, ints(lens))
+    prompt_lens = [2500, 900, 1100]
+    prompt_table = pool.table(prompt_lens)
+    pq = pool.normal(sum(prompt_lens) // 4, 4, 128)
+    rows = [n // 4 for n in prompt_lens]
+    pq = pq[:sum(rows)]
+    big = KvBatch(prompt_table, ints(prompt_lens), ints(offsets_of(rows)))
+    pout = torch.full_like(pq, 9.0)
+    many = KvBatch(table[:1].expand(3000, table.shape[1]).contiguous(), ints([5] * 3000))
+    mq, mout = pool.normal(3000, 4, 128), torch.empty((3000, 4, 128), dtype=torch.bfloat16, device="cuda")
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    step = lambda: decode_attention(fresh, q, pool.cache, batch, out, prefix=prefix, stream=stream.cuda_stream)
+    step()
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        step()
+    for _ in range(3):
+        out.fill_(9.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        prompt_attention(fresh, pq, pool.cache, big, pout, stream=stream.cuda_stream)
+        with torch.cuda.stream(stream):
+            graph.replay()
+        decode_attention(fresh, mq, pool.cache, many, mout, stream=stream.cuda_stream)
+        out_of_the_way = torch.full((1 << 24,), float("nan"), device="cuda")   # takes what was freed
+        torch.cuda.synchronize()
+        with torch.cuda.stream(stream):
+            graph.replay()
+        fresh.synchronize(stream.cuda_stream)
+        del out_of_the_way
+        _check_decode(pool, table, ptable, q, out, None, lens, prefixes, groups, 128 ** -0.5)
+    _check_prompt(pool, prompt_table, pq, pout, None, rows, prompt_lens, 128 ** -0.5)
+    del graph

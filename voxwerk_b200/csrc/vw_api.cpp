@@ -297,7 +297,8 @@ vw_status read_device_error(vw_handle* h, cudaStream_t st) {
     if (bits) {
         cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
         if (h->d_defer) cudaMemsetAsync(h->d_defer, 0, kDeferHeader * sizeof(int32_t), st);
-        if (h->d_attn_counts) cudaMemsetAsync(h->d_attn_counts, 0, h->attn_counts_bytes, st);
+        if (h->attn_counts.p) cudaMemsetAsync(h->attn_counts.p, 0, h->attn_counts.bytes, st);
+        for (const DeviceBuffer& b : h->old_attn_counts) cudaMemsetAsync(b.p, 0, b.bytes, st);
         cudaStreamSynchronize(st);
     }
     if (bits & vw::kErrTimeout) return fail(h, VW_ERR_TIMEOUT, "a bounded wait in the sampler kernel gave up");
@@ -574,8 +575,10 @@ VW_EXPORT vw_status vw_destroy(vw_handle* h) {
         if (h->d_scratch) cudaFree(h->d_scratch);
         if (h->d_stage) cudaFree(h->d_stage);
         if (h->d_logits) cudaFree(h->d_logits);
-        if (h->d_attn) cudaFree(h->d_attn);
-        if (h->d_attn_counts) cudaFree(h->d_attn_counts);
+        if (h->attn.p) cudaFree(h->attn.p);
+        if (h->attn_counts.p) cudaFree(h->attn_counts.p);
+        for (const DeviceBuffer& b : h->old_attn_counts) cudaFree(b.p);
+        for (const DeviceBuffer& b : h->old_buffers) cudaFree(b.p);
         if (h->attn_done) cudaEventDestroy(h->attn_done);
         if (h->d_opts) cudaFree(h->d_opts);
         if (h->h_opts) cudaFreeHost(h->h_opts);

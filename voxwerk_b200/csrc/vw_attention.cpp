@@ -87,29 +87,37 @@ cudaError_t leave_workspace(vw_handle* h, cudaStream_t st, bool capturing) {
     return cudaEventRecord(h->attn_done, st);
 }
 
-// Grows one of the two attention buffers (cleared: the one whose contents are zero between calls).
-vw_status reserve(vw_handle* h, char** buf, size_t* have, size_t need, bool clear, cudaStream_t st) {
-    if (need <= *have) return VW_OK;
+// Grows one of the two attention buffers (clear: the one whose contents are zero between calls).  Not inside a capture:
+// neither the wait nor the allocation is allowed there.
+vw_status reserve(vw_handle* h, DeviceBuffer* b, size_t need, bool clear, cudaStream_t st, bool capturing) {
+    if (need <= b->bytes) {
+        b->captured = b->captured || capturing;
+        return VW_OK;
+    }
+    if (capturing)
+        return fail(h, VW_ERR_INVALID_ARG, "attention workspace: run a call of this size once before one is captured");
+    constexpr const char* kWhat = "attention workspace";
     cudaError_t e = cudaDeviceSynchronize();   // an earlier call, on any stream, may still use the old buffer
-    if (e == cudaSuccess && *buf) e = cudaFree(*buf);
-    *buf = nullptr;
-    *have = 0;
+    if (e != cudaSuccess) return cuda_fail(h, e, kWhat);
+    const vw_status r = let_go(h, b, clear ? &h->old_attn_counts : &h->old_buffers, kWhat);
+    if (r != VW_OK) return r;
     const size_t bytes = round_up(need + need / 4, 1 << 16);
-    if (e == cudaSuccess) e = cudaMalloc(reinterpret_cast<void**>(buf), bytes);
-    if (e == cudaSuccess && clear) e = cudaMemsetAsync(*buf, 0, bytes, st);
-    if (e != cudaSuccess) return cuda_fail(h, e, "attention workspace");
-    *have = bytes;
+    e = cudaMalloc(reinterpret_cast<void**>(&b->p), bytes);
+    if (e == cudaSuccess && clear) e = cudaMemsetAsync(b->p, 0, bytes, st);
+    if (e == cudaSuccess && clear) e = cudaStreamSynchronize(st);   // whatever stream the next call is on
+    if (e != cudaSuccess) return cuda_fail(h, e, kWhat);
+    b->bytes = bytes;
     return VW_OK;
 }
 
 constexpr size_t kCountsHeader = 256;   // the tile kernel's counters, then the decode kernel's tickets
 
-vw_status reserve_counts(vw_handle* h, int64_t tickets, cudaStream_t st) {
-    return reserve(h, &h->d_attn_counts, &h->attn_counts_bytes, kCountsHeader + static_cast<size_t>(tickets) * 4, true, st);
+vw_status reserve_counts(vw_handle* h, int64_t tickets, cudaStream_t st, bool capturing) {
+    return reserve(h, &h->attn_counts, kCountsHeader + static_cast<size_t>(tickets) * 4, true, st, capturing);
 }
 // The parts buffer, carved twice: without a base for its size, then for the pointers.
 template <typename F>
-vw_status reserve_parts(vw_handle* h, cudaStream_t st, F carve) {
+vw_status reserve_parts(vw_handle* h, cudaStream_t st, bool capturing, F carve) {
     size_t size = 0;
     const auto take = [&size](char* base, int64_t bytes) {
         char* p = base ? base + size : nullptr;
@@ -117,15 +125,15 @@ vw_status reserve_parts(vw_handle* h, cudaStream_t st, F carve) {
         return p;
     };
     carve([&](int64_t bytes) { return take(nullptr, bytes); });
-    const vw_status r = reserve(h, &h->d_attn, &h->attn_bytes, size, false, st);
+    const vw_status r = reserve(h, &h->attn, size, false, st, capturing);
     if (r != VW_OK) return r;
     size = 0;
-    carve([&](int64_t bytes) { return take(h->d_attn, bytes); });
+    carve([&](int64_t bytes) { return take(h->attn.p, bytes); });
     return VW_OK;
 }
 template <typename Take>
 void carve_tiles(vw_handle* h, const vw::TilePlan& plan, Take take, vw::TileWork* w) {
-    w->counters = reinterpret_cast<int32_t*>(h->d_attn_counts);
+    w->counters = reinterpret_cast<int32_t*>(h->attn_counts.p);
     w->units_per_cta = reinterpret_cast<int64_t*>(take(8));
     w->unit_end = reinterpret_cast<int64_t*>(take(plan.unit_ends * 8));
     w->part_lse = reinterpret_cast<float*>(take(plan.part_rows * 4));
@@ -220,8 +228,8 @@ VW_EXPORT vw_status vw_prompt_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (e != cudaSuccess) return cuda_fail(h, e, "prompt attention");
     const vw::TilePlan plan = vw::plan_prompt(p, h->sm_count);
     vw::TileWork w{};
-    r = reserve_counts(h, 0, st);
-    if (r == VW_OK) r = reserve_parts(h, st, [&](auto take) { carve_tiles(h, plan, take, &w); });
+    r = reserve_counts(h, 0, st, capturing);
+    if (r == VW_OK) r = reserve_parts(h, st, capturing, [&](auto take) { carve_tiles(h, plan, take, &w); });
     if (r != VW_OK) return r;
     e = vw::launch_prompt_attention(p, plan, w, st);
     if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
@@ -263,10 +271,10 @@ VW_EXPORT vw_status vw_decode_attention(vw_handle* h, const vw_kv_cache* cache, 
     vw::TilePlan prefix_plan{};
     if (p.prefix.n_groups > 0) prefix_plan = vw::plan_prefix(p, h->sm_count);
     vw::DecodeWork w{};
-    r = reserve_counts(h, plan.items, st);
+    r = reserve_counts(h, plan.items, st, capturing);
     if (r == VW_OK)
-        r = reserve_parts(h, st, [&](auto take) {
-            w.tickets = reinterpret_cast<int32_t*>(h->d_attn_counts + kCountsHeader);
+        r = reserve_parts(h, st, capturing, [&](auto take) {
+            w.tickets = reinterpret_cast<int32_t*>(h->attn_counts.p + kCountsHeader);
             w.units_per_cta = reinterpret_cast<int64_t*>(take(8));
             w.chunk = reinterpret_cast<int32_t*>(take(4));
             w.unit_end = reinterpret_cast<int64_t*>(take(static_cast<int64_t>(p.batch.n_seqs) * 8));
@@ -277,7 +285,7 @@ VW_EXPORT vw_status vw_decode_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (r != VW_OK) return r;
     if (p.prefix.n_groups > 0) e = vw::launch_prefix_attention(p, prefix_plan, w.prefix, st);
     if (e == cudaSuccess) e = vw::launch_decode_attention(p, plan, w, st);
-    if (e != cudaSuccess) cudaMemsetAsync(h->d_attn_counts, 0, h->attn_counts_bytes, st);   // the join would have
+    if (e != cudaSuccess) cudaMemsetAsync(h->attn_counts.p, 0, h->attn_counts.bytes, st);   // the join would have
     if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
     if (e != cudaSuccess) return cuda_fail(h, e, "decode attention");
     if (!stream) return read_device_error(h, st);

@@ -4,6 +4,7 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <new>
 #include <string>
 #include <vector>
 
@@ -15,6 +16,14 @@
 #define VW_EXPORT extern "C" __attribute__((visibility("default")))
 
 constexpr int kCopyStreams = 3;   // host -> device copies of VW_MEM_HOST calls run on this many copy engines
+
+// Device memory that grows with a handle's calls.  The kernels of a captured call keep its address for as long as their
+// graph lives, so a buffer that a capture has used is put aside when it is outgrown, and freed with the handle.
+struct DeviceBuffer {
+    char* p = nullptr;
+    size_t bytes = 0;
+    bool captured = false;
+};
 
 struct vw_handle {
     int device = -1;
@@ -41,10 +50,10 @@ struct vw_handle {
     int force_exact = 0;                     // VW_FORCE_EXACT at creation
     int test_stall_row = -1;                 // VW_TEST_STALL_ROW at creation (first vw_sample call only)
     unsigned long long h2d_bytes = 0;        // host -> device input bytes of VW_MEM_HOST calls (vw_stats.h2d_bytes)
-    char* d_attn = nullptr;                  // attention: partial results (vw_attention.cpp)
-    size_t attn_bytes = 0;
-    char* d_attn_counts = nullptr;           // attention: counters and tickets, zero between calls
-    size_t attn_counts_bytes = 0;
+    DeviceBuffer attn;                       // attention: partial results (vw_attention.cpp)
+    DeviceBuffer attn_counts;                // attention: counters and tickets, zero between calls
+    std::vector<DeviceBuffer> old_attn_counts;   // outgrown ones that captured calls still use
+    std::vector<DeviceBuffer> old_buffers;       // likewise, of any other use
     cudaStream_t attn_stream = nullptr;      // the stream of the last call that used it, and its end on that stream
     cudaEvent_t attn_done = nullptr;
     std::vector<vw_batch*> batches;          // live batches created on this handle (released by vw_destroy)
@@ -85,6 +94,23 @@ inline vw_status cuda_fail(vw_handle* h, cudaError_t e, const char* where) {
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 inline size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+// Lets an outgrown buffer go: put aside where captured calls use it, else freed (the caller has waited for its users).
+inline vw_status let_go(vw_handle* h, DeviceBuffer* b, std::vector<DeviceBuffer>* aside, const char* what) {
+    if (!b->p) return VW_OK;
+    if (b->captured) {
+        try {
+            aside->push_back(*b);
+        } catch (const std::bad_alloc&) {
+            return fail(h, VW_ERR_CUDA, what);
+        }
+    } else {
+        const cudaError_t e = cudaFree(b->p);
+        if (e != cudaSuccess) return cuda_fail(h, e, what);
+    }
+    *b = DeviceBuffer{};
+    return VW_OK;
+}
 
 // Grows a buffer of the handle to `need` bytes (waits for the handle's stream before it frees the old one).
 inline vw_status grow(vw_handle* h, char** buf, size_t* cap, size_t need, const char* what) {
