@@ -137,6 +137,8 @@ const char* vw_last_error(const vw_handle* handle);
  *   returns after the ids are written, reporting device-side errors.  With a stream the call is enqueued and
  *   returns at once; device-side errors (history id out of range, timeout) are reported by the next
  *   vw_synchronize() on that stream.  VW_MEM_HOST calls are always synchronous.
+ *   A call captured into a CUDA graph keeps its buffers and its options until vw_destroy; the graph must not be
+ *   replayed after that.
  */
 vw_status vw_sample(vw_handle* handle, const vw_segment* segments, int32_t n_segments,
                     const vw_options* options, int32_t n_options, int32_t mem, void* stream);

@@ -28,6 +28,8 @@ struct Op {
 static std::vector<Op> ops;
 static std::map<char*, size_t> live;                 // device memory
 static std::map<char*, size_t> freed;
+static std::set<void*> pinned;
+static std::set<const void*> upload_sources;         // pinned memory that a captured copy reads
 static std::set<cudaStream_t> capturing;
 static std::set<cudaEvent_t> recorded;
 static uintptr_t next_handle = 0x1000;
@@ -41,8 +43,9 @@ static size_t count(const char* what, size_t from = 0) {
     for (size_t i = from; i < ops.size(); ++i) n += ops[i].what == what;
     return n;
 }
-static cudaError_t unless_capturing(cudaError_t e = cudaSuccess) {
-    return capturing.empty() ? e : cudaErrorStreamCaptureUnsupported;
+static cudaStreamCaptureMode mode = cudaStreamCaptureModeGlobal;
+static cudaError_t unless_capturing() {
+    return capturing.empty() || mode == cudaStreamCaptureModeRelaxed ? cudaSuccess : cudaErrorStreamCaptureUnsupported;
 }
 
 extern "C" {
@@ -75,11 +78,16 @@ cudaError_t cudaFree(void* p) {
     note("free", nullptr, p);
     return cudaSuccess;
 }
-cudaError_t cudaHostAlloc(void** p, size_t n, unsigned) { return *p = std::calloc(n, 1), cudaSuccess; }
-cudaError_t cudaMallocHost(void** p, size_t n) { return *p = std::calloc(n, 1), cudaSuccess; }
-cudaError_t cudaFreeHost(void* p) { return std::free(p), cudaSuccess; }
+cudaError_t cudaHostAlloc(void** p, size_t n, unsigned) {
+    if (unless_capturing() != cudaSuccess) return cudaErrorStreamCaptureUnsupported;
+    pinned.insert(*p = std::calloc(n, 1));
+    return cudaSuccess;
+}
+cudaError_t cudaMallocHost(void** p, size_t n) { return cudaHostAlloc(p, n, 0); }
+cudaError_t cudaFreeHost(void* p) { return pinned.erase(p) ? cudaSuccess : cudaErrorInvalidValue; }   // (kept too)
 cudaError_t cudaMemcpy(void* d, const void* s, size_t n, cudaMemcpyKind) { return std::memcpy(d, s, n), cudaSuccess; }
-cudaError_t cudaMemcpyAsync(void* d, const void* s, size_t n, cudaMemcpyKind, cudaStream_t) {
+cudaError_t cudaMemcpyAsync(void* d, const void* s, size_t n, cudaMemcpyKind, cudaStream_t st) {
+    if (capturing.count(st)) upload_sources.insert(s);
     return std::memcpy(d, s, n), cudaSuccess;
 }
 cudaError_t cudaMemcpy2DAsync(void*, size_t, const void*, size_t, size_t, size_t, cudaMemcpyKind, cudaStream_t) {
@@ -98,6 +106,7 @@ cudaError_t cudaStreamDestroy(cudaStream_t) { return cudaSuccess; }
 cudaError_t cudaStreamIsCapturing(cudaStream_t s, cudaStreamCaptureStatus* c) {
     return *c = capturing.count(s) ? cudaStreamCaptureStatusActive : cudaStreamCaptureStatusNone, cudaSuccess;
 }
+cudaError_t cudaThreadExchangeStreamCaptureMode(cudaStreamCaptureMode* m) { return std::swap(*m, mode), cudaSuccess; }
 cudaError_t cudaStreamWaitEvent(cudaStream_t s, cudaEvent_t e, unsigned) { return note("wait", s, e), cudaSuccess; }
 cudaError_t cudaEventCreateWithFlags(cudaEvent_t* e, unsigned) {
     return *e = reinterpret_cast<cudaEvent_t>(next_handle += 16), cudaSuccess;
@@ -225,6 +234,26 @@ struct Calls {
         r.dtype = VW_BF16;
         return vw_rope_append(h, &c, &b, &r, st);
     }
+    vw_segment segment(int n, int vocab) {
+        vw_segment s{};
+        s.logits = memory;
+        s.row_stride = s.vocab = vocab;
+        s.n_rows = n;
+        s.kind = VW_ROWS_SUB;
+        s.uniforms = reinterpret_cast<double*>(memory);
+        s.out_ids = ints();
+        return s;
+    }
+    vw_status sample(int n, int vocab, int n_options, cudaStream_t st, float penalty = 1.0f) {
+        const std::vector<vw_options> o(n_options, vw_options{1, 50, 1.0f, 0.9f, penalty});
+        const vw_segment s = segment(n, vocab);
+        return vw_sample(h, &s, 1, o.data(), n_options, VW_MEM_DEVICE, st);
+    }
+    vw_status head(int n, int vocab, cudaStream_t st) {
+        const vw_options o{1, 50, 1.0f, 0.9f, 1.0f};
+        const vw_segment s = segment(n, vocab);
+        return vw_head_sample(h, memory, 64, 64, memory, 64, &s, &o, 1, nullptr, st);
+    }
     cudaStream_t stream() {
         cudaStream_t s;
         cudaStreamCreateWithFlags(&s, 0);
@@ -280,11 +309,46 @@ static void growth_under_capture() {
     expect(live.empty(), "the handle leaves nothing allocated");
 }
 
+// The same for the sampler's buffers: scratch, deferred rows, the head's logits, a batch's logits, options in a table.
+static void captured_sampler() {
+    Calls c;
+    cudaStream_t st = c.stream();
+    const vw_options o{1, 50, 1.0f, 0.9f, 1.0f};
+    vw_batch* b = nullptr;
+    expect(vw_batch_create(c.h, 4000, 64, 10, 3, 0, 0, 0, &b) == VW_OK, "batch");
+    const auto group = [&](int vocab) {
+        return vw_batch_sub_head_step(b, 1, c.memory, 64, 64, c.memory, 64, vocab, &o, 1, c.ints(), nullptr, st);
+    };
+    const auto step = [&] {
+        return c.head(16, 64, st) == VW_OK && c.sample(8, 64, 1, st) == VW_OK && group(64) == VW_OK;
+    };
+    expect(step() && c.sample(8, 64, 40, st) == VW_OK, "before the capture");
+    capturing.insert(st);
+    const size_t from = ops.size();
+    expect(step(), "captured");
+    expect(c.sample(8, 64, 40, st, 1.5f) == VW_OK, "captured, with a table of options");
+    const size_t to = ops.size();
+    capturing.clear();
+    expect(group(8192) == VW_OK, "more of a batch's logits");
+    expect(c.sample(300000, 4096, 100, st) == VW_OK && c.head(5000, 2048, st) == VW_OK, "calls that need more");
+    expect(c.sample(8, 64, 40, st, 1.25f) == VW_OK, "a table as long as the captured one");
+    expect(!in_freed(from, to), "memory of a captured call was freed");
+    for (const void* p : upload_sources) {
+        expect(pinned.count(const_cast<void*>(p)) == 1, "the source of a captured upload was freed");
+        expect(static_cast<const vw_options*>(p)->repetition_penalty == 1.5f, "the source of a captured upload was overwritten");
+    }
+    expect(upload_sources.size() == 1, "one captured upload");
+    vw_batch_destroy(b);
+    vw_destroy(c.h);
+    expect(live.empty() && pinned.empty(), "the handle leaves nothing allocated");
+}
+
 int main(int argc, char** argv) {
     const std::map<std::string, std::function<void()>> scenarios = {
         {"captured_workspace", captured_workspace},
         {"outgrown_workspace", outgrown_workspace},
         {"growth_under_capture", growth_under_capture},
+        {"captured_sampler", captured_sampler},
     };
     const auto it = argc > 1 ? scenarios.find(argv[1]) : scenarios.end();
     if (it == scenarios.end()) return 2;

@@ -23,7 +23,10 @@ def checker(tmp_path_factory):
     return exe
 
 
-@pytest.mark.parametrize("scenario", ["captured_workspace", "outgrown_workspace", "growth_under_capture"])
+SCENARIOS = ["captured_workspace", "outgrown_workspace", "growth_under_capture", "captured_sampler"]
+
+
+@pytest.mark.parametrize("scenario", SCENARIOS)
 def test_host_side(checker, scenario):
     run = subprocess.run([checker, scenario], capture_output=True, text=True, timeout=60)
     assert run.returncode == 0, run.stdout + run.stderr

@@ -137,7 +137,7 @@ template <typename T>
 T* stage_copy(vw_handle* h, const T* src, size_t count, size_t* off, cudaStream_t st, cudaError_t* err) {
     if (!src || count == 0) return nullptr;
     *off = round_up(*off, 256);
-    T* dst = reinterpret_cast<T*>(h->d_stage + *off);
+    T* dst = reinterpret_cast<T*>(h->stage.p + *off);
     *off += count * sizeof(T);
     if (*err == cudaSuccess) *err = cudaMemcpyAsync(dst, src, count * sizeof(T), cudaMemcpyHostToDevice, st);
     h->h2d_bytes += count * sizeof(T);
@@ -183,7 +183,7 @@ template <typename T>
 T* stage_copy_split(vw_handle* h, const T* src, size_t count, size_t* off, cudaError_t* err) {
     if (!src || count == 0) return nullptr;
     *off = round_up(*off, 256);
-    T* dst = reinterpret_cast<T*>(h->d_stage + *off);
+    T* dst = reinterpret_cast<T*>(h->stage.p + *off);
     *off += count * sizeof(T);
     for (int i = 0; i < kCopyStreams && *err == cudaSuccess; ++i) {
         const size_t a = count * i / kCopyStreams, b = count * (i + 1) / kCopyStreams;
@@ -219,7 +219,7 @@ vw_status stage_host_inputs(vw_handle* h, const vw_segment* segs, int n, cudaStr
         need += round_up(static_cast<size_t>(s.n_rows) * 4, 256) + 256;
         if (s.out_probs) need += round_up(static_cast<size_t>(s.n_rows) * s.vocab * 8, 256) + 256;
     }
-    vw_status r = grow(h, &h->d_stage, &h->stage_bytes, need, "staging buffer");
+    vw_status r = grow(h, &h->stage, need, "staging buffer");
     if (r != VW_OK) return r;
     size_t off = 0;
     cudaError_t e = fork_copies(h, st);
@@ -247,7 +247,7 @@ vw_status stage_host_inputs(vw_handle* h, const vw_segment* segs, int n, cudaStr
         }
         if (c_lo < c_hi) {
             off = round_up(off, 256);
-            unsigned char* dst = reinterpret_cast<unsigned char*>(h->d_stage) + off;
+            unsigned char* dst = reinterpret_cast<unsigned char*>(h->stage.p) + off;
             off += nel * es;
             stage_columns(h, s, es, dst, 0, c_lo, &e);
             stage_columns(h, s, es, dst, c_hi, s.vocab, &e);
@@ -264,7 +264,7 @@ vw_status stage_host_inputs(vw_handle* h, const vw_segment* segs, int n, cudaStr
             d.hist_ids = nh ? stage_copy_split(h, s.hist_ids + s.hist_offsets[0], nh, &off, &e) : nullptr;
             if (!d.hist_ids) {
                 off = round_up(off, 256);
-                d.hist_ids = reinterpret_cast<int32_t*>(h->d_stage + off);   // never read: every history empty
+                d.hist_ids = reinterpret_cast<int32_t*>(h->stage.p + off);   // never read: every history empty
             }
         } else {
             d.hist_offsets = nullptr;
@@ -274,11 +274,11 @@ vw_status stage_host_inputs(vw_handle* h, const vw_segment* segs, int n, cudaStr
         d.opt_index = stage_copy(h, s.opt_index, s.opt_index ? s.n_rows : 0, &off, st, &e);
         d.uniforms = stage_copy(h, s.uniforms, s.uniforms ? s.n_rows : 0, &off, st, &e);
         off = round_up(off, 256);
-        d.out_ids = reinterpret_cast<int32_t*>(h->d_stage + off);
+        d.out_ids = reinterpret_cast<int32_t*>(h->stage.p + off);
         off += static_cast<size_t>(s.n_rows) * 4;
         if (s.out_probs) {
             off = round_up(off, 256);
-            d.out_probs = reinterpret_cast<double*>(h->d_stage + off);
+            d.out_probs = reinterpret_cast<double*>(h->stage.p + off);
             off += static_cast<size_t>(s.n_rows) * s.vocab * 8;
         }
     }
@@ -296,7 +296,8 @@ vw_status read_device_error(vw_handle* h, cudaStream_t st) {
     const unsigned bits = *h->h_err;
     if (bits) {
         cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-        if (h->d_defer) cudaMemsetAsync(h->d_defer, 0, kDeferHeader * sizeof(int32_t), st);
+        if (h->defer.p) cudaMemsetAsync(h->defer.p, 0, kDeferHeader * sizeof(int32_t), st);
+        for (const DeviceBuffer& b : h->old_defers) cudaMemsetAsync(b.p, 0, kDeferHeader * sizeof(int32_t), st);
         if (h->attn_counts.p) cudaMemsetAsync(h->attn_counts.p, 0, h->attn_counts.bytes, st);
         for (const DeviceBuffer& b : h->old_attn_counts) cudaMemsetAsync(b.p, 0, b.bytes, st);
         cudaStreamSynchronize(st);
@@ -322,6 +323,52 @@ struct SegExtra {
     const int32_t* active;
 };
 
+// Where a table of more than kInlineOptions options is uploaded, and its pinned source.  A captured call's copy reads its
+// source again at every replay, so it has a pair of its own for the handle's life.
+vw_status option_table(vw_handle* h, int n_opts, cudaStream_t st, bool capturing, vw::DevOptions** dev,
+                       vw::DevOptions** host) {
+    const size_t bytes = sizeof(vw::DevOptions) * n_opts;
+    constexpr const char* kWhat = "options table";
+    if (capturing) {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;   // nothing of this capture is touched
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        DeviceBuffer b;
+        b.captured = true;
+        cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&b.p), bytes);
+        if (e == cudaSuccess) e = cudaMallocHost(reinterpret_cast<void**>(host), bytes);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        *dev = reinterpret_cast<vw::DevOptions*>(b.p);
+        if (e != cudaSuccess) {
+            if (b.p) cudaFree(b.p);
+            return cuda_fail(h, e, kWhat);
+        }
+        vw_status r = let_go(h, &b, &h->old_buffers, kWhat);
+        try {
+            if (r == VW_OK) h->captured_opts.push_back(*host);
+        } catch (const std::bad_alloc&) {
+            r = fail(h, VW_ERR_CUDA, kWhat);
+        }
+        return r;
+    }
+    if (static_cast<size_t>(n_opts) > h->opts_cap) {
+        cudaStreamSynchronize(st);
+        if (h->d_opts) cudaFree(h->d_opts);
+        if (h->h_opts) cudaFreeHost(h->h_opts);
+        h->d_opts = nullptr;
+        h->h_opts = nullptr;
+        h->opts_cap = 0;
+        cudaError_t e = cudaMalloc(&h->d_opts, bytes);
+        if (e == cudaSuccess) e = cudaMallocHost(&h->h_opts, bytes);
+        if (e != cudaSuccess) return cuda_fail(h, e, kWhat);
+        h->opts_cap = n_opts;
+    } else {
+        cudaEventSynchronize(h->opts_done);   // the previous upload has left the pinned buffer
+    }
+    *dev = h->d_opts;
+    *host = h->h_opts;
+    return VW_OK;
+}
+
 vw_status sample_impl(vw_handle* h, const vw_segment* segs, int32_t n_segs, const vw_options* opts, int32_t n_opts,
                       int32_t mem, void* stream, const SegExtra* extra = nullptr) {
     if (!h) return VW_ERR_INVALID_ARG;
@@ -345,7 +392,7 @@ vw_status sample_impl(vw_handle* h, const vw_segment* segs, int32_t n_segs, cons
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, VW_ERR_CUDA, "cudaSetDevice failed");
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
-    const bool sync = (stream == nullptr);
+    const bool sync = (stream == nullptr), capturing = !sync && is_capturing(st);
 
     HostStaging hs;
     const vw_segment* run = segs;
@@ -415,26 +462,14 @@ vw_status sample_impl(vw_handle* h, const vw_segment* segs, int32_t n_segs, cons
         std::memcpy(p.inl_opts, opts, sizeof(vw_options) * n_opts);
         fill_inline_constants(p);
     } else {
-        if (static_cast<size_t>(n_opts) > h->opts_cap) {
-            cudaStreamSynchronize(st);
-            if (h->d_opts) cudaFree(h->d_opts);
-            if (h->h_opts) cudaFreeHost(h->h_opts);
-            h->d_opts = nullptr;
-            h->h_opts = nullptr;
-            h->opts_cap = 0;
-            cudaError_t e = cudaMalloc(&h->d_opts, sizeof(vw::DevOptions) * n_opts);
-            if (e == cudaSuccess) e = cudaMallocHost(&h->h_opts, sizeof(vw::DevOptions) * n_opts);
-            if (e != cudaSuccess) return cuda_fail(h, e, "options table");
-            h->opts_cap = n_opts;
-        } else {
-            cudaEventSynchronize(h->opts_done);   // the previous upload has left the pinned buffer
-        }
-        std::memcpy(h->h_opts, opts, sizeof(vw_options) * n_opts);
-        cudaError_t e = cudaMemcpyAsync(h->d_opts, h->h_opts, sizeof(vw::DevOptions) * n_opts,
-                                        cudaMemcpyHostToDevice, st);
-        if (e == cudaSuccess) e = cudaEventRecord(h->opts_done, st);
+        vw::DevOptions *dev = nullptr, *host = nullptr;
+        r = option_table(h, n_opts, st, capturing, &dev, &host);
+        if (r != VW_OK) return r;
+        std::memcpy(host, opts, sizeof(vw_options) * n_opts);
+        cudaError_t e = cudaMemcpyAsync(dev, host, sizeof(vw::DevOptions) * n_opts, cudaMemcpyHostToDevice, st);
+        if (e == cudaSuccess && !capturing) e = cudaEventRecord(h->opts_done, st);
         if (e != cudaSuccess) return cuda_fail(h, e, "options upload");
-        p.dev_opts = h->d_opts;
+        p.dev_opts = dev;
     }
     p.stage_logit_bytes = logit_bytes;
     p.stage_hist_cap = hist_cap;
@@ -467,25 +502,26 @@ vw_status sample_impl(vw_handle* h, const vw_segment* segs, int32_t n_segs, cons
         return fail(h, VW_ERR_INVALID_ARG, "rows too large for shared memory");
     const int grid_g = plan.grid_general;
     p.gscratch_stride = vw::sampler_gscratch_stride(vmax);
-    r = grow(h, &h->d_scratch, &h->scratch_bytes, static_cast<size_t>(grid_g) * p.gscratch_stride, "scratch");
+    r = grow(h, &h->scratch, static_cast<size_t>(grid_g) * p.gscratch_stride, "scratch", capturing);
     if (r != VW_OK) return r;
-    p.gscratch = h->d_scratch;
+    p.gscratch = h->scratch.p;
     // deferred-row list: total_rows entries after four counters (deferred rows, whole-row CTAs done, two spare),
     // all zero between calls
-    if (static_cast<size_t>(p.total_rows) + kDeferHeader > h->defer_cap) {
-        cudaError_t e = cudaStreamSynchronize(st);
-        if (e == cudaSuccess && h->d_defer) e = cudaFree(h->d_defer);
-        h->d_defer = nullptr;
-        h->defer_cap = 0;
-        const size_t cap = static_cast<size_t>(p.total_rows) + kDeferHeader + 4096;
-        if (e == cudaSuccess) e = cudaMalloc(&h->d_defer, cap * sizeof(int32_t));
-        if (e == cudaSuccess) e = cudaMemset(h->d_defer, 0, kDeferHeader * sizeof(int32_t));
-        if (e != cudaSuccess) return cuda_fail(h, e, "deferred-row list");
-        h->defer_cap = cap;
+    const size_t had = h->defer.bytes;
+    r = grow(h, &h->defer, (static_cast<size_t>(p.total_rows) + kDeferHeader) * sizeof(int32_t), "deferred-row list",
+             capturing, &h->old_defers);
+    if (r != VW_OK) return r;
+    if (h->defer.bytes != had) {
+        const cudaError_t e = cudaMemset(h->defer.p, 0, kDeferHeader * sizeof(int32_t));
+        if (e != cudaSuccess) {
+            h->defer.bytes = 0;   // not for the next call either
+            return cuda_fail(h, e, "deferred-row list");
+        }
     }
-    p.deferred_count = reinterpret_cast<uint32_t*>(h->d_defer);
-    p.done_count = reinterpret_cast<uint32_t*>(h->d_defer) + 1;
-    p.deferred_rows = h->d_defer + kDeferHeader;
+    int32_t* defer = reinterpret_cast<int32_t*>(h->defer.p);
+    p.deferred_count = reinterpret_cast<uint32_t*>(defer);
+    p.done_count = reinterpret_cast<uint32_t*>(defer) + 1;
+    p.deferred_rows = defer + kDeferHeader;
 
     cudaError_t e = cudaSuccess;
     if (sync) e = cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
@@ -572,20 +608,17 @@ VW_EXPORT vw_status vw_destroy(vw_handle* h) {
         if (h->stream) cudaStreamSynchronize(h->stream);
         for (vw_batch* b : h->batches) orphan_batch(b);   // the caller still owns (and destroys) the structs
         h->batches.clear();
-        if (h->d_scratch) cudaFree(h->d_scratch);
-        if (h->d_stage) cudaFree(h->d_stage);
-        if (h->d_logits) cudaFree(h->d_logits);
-        if (h->attn.p) cudaFree(h->attn.p);
-        if (h->attn_counts.p) cudaFree(h->attn_counts.p);
-        for (const DeviceBuffer& b : h->old_attn_counts) cudaFree(b.p);
-        for (const DeviceBuffer& b : h->old_buffers) cudaFree(b.p);
+        for (const DeviceBuffer* b : {&h->scratch, &h->stage, &h->logits, &h->defer, &h->attn, &h->attn_counts})
+            if (b->p) cudaFree(b->p);
+        for (const auto* old : {&h->old_attn_counts, &h->old_defers, &h->old_buffers})
+            for (const DeviceBuffer& b : *old) cudaFree(b.p);
         if (h->attn_done) cudaEventDestroy(h->attn_done);
         if (h->d_opts) cudaFree(h->d_opts);
         if (h->h_opts) cudaFreeHost(h->h_opts);
+        for (vw::DevOptions* p : h->captured_opts) cudaFreeHost(p);
         if (h->d_err) cudaFree(h->d_err);
         if (h->d_stats) cudaFree(h->d_stats);
         if (h->d_guess) cudaFree(h->d_guess);
-        if (h->d_defer) cudaFree(h->d_defer);
         if (h->h_err) cudaFreeHost(h->h_err);
         if (h->opts_done) cudaEventDestroy(h->opts_done);
         if (h->stream) cudaStreamDestroy(h->stream);
@@ -647,8 +680,7 @@ struct vw_batch {
     vw::BatchDevice d{};
     double* d_uniforms = nullptr;   // [n_slots] the step's draws
     void* mem = nullptr;            // one allocation for every array
-    float* d_logits = nullptr;      // head steps: [n_slots, vocab] logits of the batch's own GEMM
-    size_t logits_bytes = 0;
+    DeviceBuffer logits;            // head steps: [n_slots, vocab] logits of the batch's own GEMM
     int32_t vocab = 0, sup_lo = 0, sup_hi = 0, min_new = 0;
 };
 
@@ -656,10 +688,9 @@ namespace {
 
 void orphan_batch(vw_batch* b) {
     if (b->mem) cudaFree(b->mem);
-    if (b->d_logits) cudaFree(b->d_logits);
+    if (b->logits.p) cudaFree(b->logits.p);
     b->mem = nullptr;
-    b->d_logits = nullptr;
-    b->logits_bytes = 0;
+    b->logits = DeviceBuffer{};
     b->h = nullptr;   // every later call on the batch returns VW_ERR_INVALID_ARG
 }
 
@@ -930,21 +961,15 @@ vw_status batch_head_step(vw_batch* b, int which, int group, const void* hidden,
     if (!guard.ok()) return fail(h, VW_ERR_CUDA, "cudaSetDevice failed");
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
     const size_t need = static_cast<size_t>(b->d.n_slots) * static_cast<size_t>(vocab) * 4;
-    if (need > b->logits_bytes) {
-        cudaError_t e = cudaStreamSynchronize(st);   // an earlier step may still read the old buffer
-        if (e == cudaSuccess && b->d_logits) e = cudaFree(b->d_logits);
-        b->d_logits = nullptr;
-        b->logits_bytes = 0;
-        if (e == cudaSuccess) e = cudaMalloc(&b->d_logits, need);
-        if (e != cudaSuccess) return cuda_fail(h, e, "batch logits buffer");
-        b->logits_bytes = need;
-    }
+    r = grow(h, &b->logits, need, "batch logits buffer", stream && is_capturing(st));
+    if (r != VW_OK) return r;
+    float* logits = reinterpret_cast<float*>(b->logits.p);
     cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
     if (e == cudaSuccess)
         e = vw::launch_head_gemm(hidden, hidden_stride, weight, weight_stride, b->d.n_slots, vocab, hidden_size,
-                                 b->d_logits, vocab, h->d_err, st);
+                                 logits, vocab, h->d_err, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "head GEMM");
-    r = batch_step(b, which, b->d_logits, vocab, vocab, VW_F32, options, n_options, out_ids, out_done, st,
+    r = batch_step(b, which, logits, vocab, vocab, VW_F32, options, n_options, out_ids, out_done, st,
                    embed ? &emb : nullptr);
     if (r != VW_OK) return r;
     if (which == 1) {
@@ -1102,9 +1127,9 @@ VW_EXPORT vw_status vw_head_sample(vw_handle* h, const void* hidden, int64_t hid
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
     float* logits = out_logits;
     if (!logits) {
-        r = grow(h, &h->d_logits, &h->logits_bytes, static_cast<size_t>(sg.n_rows) * sg.vocab * 4, "logits buffer");
+        r = grow(h, &h->logits, static_cast<size_t>(sg.n_rows) * sg.vocab * 4, "logits buffer", stream && is_capturing(st));
         if (r != VW_OK) return r;
-        logits = reinterpret_cast<float*>(h->d_logits);
+        logits = reinterpret_cast<float*>(h->logits.p);
     }
     cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
     if (e == cudaSuccess)
@@ -1136,10 +1161,10 @@ VW_EXPORT vw_status vw_apply_repetition_penalty(vw_handle* h, float* logits, int
     cudaError_t e = cudaSuccess;
     if (mem == VW_MEM_HOST) {
         const size_t need = round_up(static_cast<size_t>(vocab) * 4, 256) + static_cast<size_t>(history_len) * 4 + 256;
-        vw_status r = grow(h, &h->d_stage, &h->stage_bytes, need, "staging buffer");
+        vw_status r = grow(h, &h->stage, need, "staging buffer");
         if (r != VW_OK) return r;
-        d_logits = reinterpret_cast<float*>(h->d_stage);
-        int32_t* dh = reinterpret_cast<int32_t*>(h->d_stage + round_up(static_cast<size_t>(vocab) * 4, 256));
+        d_logits = reinterpret_cast<float*>(h->stage.p);
+        int32_t* dh = reinterpret_cast<int32_t*>(h->stage.p + round_up(static_cast<size_t>(vocab) * 4, 256));
         e = cudaMemcpyAsync(d_logits, logits, static_cast<size_t>(vocab) * 4, cudaMemcpyHostToDevice, st);
         if (e == cudaSuccess)
             e = cudaMemcpyAsync(dh, history, static_cast<size_t>(history_len) * 4, cudaMemcpyHostToDevice, st);
@@ -1178,10 +1203,10 @@ VW_EXPORT vw_status vw_select(vw_handle* h, const float* logits, int32_t vocab, 
     int32_t* d_id = nullptr;
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, VW_ERR_CUDA, "cudaSetDevice failed");
-    vw_status r = grow(h, &h->d_stage, &h->stage_bytes, 512, "staging buffer");
+    vw_status r = grow(h, &h->stage, 512, "staging buffer");
     if (r != VW_OK) return r;
-    d_u = reinterpret_cast<double*>(h->d_stage);
-    d_id = reinterpret_cast<int32_t*>(h->d_stage + 256);
+    d_u = reinterpret_cast<double*>(h->stage.p);
+    d_id = reinterpret_cast<int32_t*>(h->stage.p + 256);
     cudaError_t e = cudaMemcpyAsync(d_u, &u, sizeof u, cudaMemcpyHostToDevice, h->stream);
     if (e != cudaSuccess) return cuda_fail(h, e, "select");
     s.uniforms = d_u;

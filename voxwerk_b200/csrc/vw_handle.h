@@ -33,16 +33,14 @@ struct vw_handle {
     int sm_count = 0;
     unsigned* d_err = nullptr;      // device error word (kErr* bits)
     unsigned* h_err = nullptr;      // pinned mirror
-    char* d_scratch = nullptr;      // general-path scratch, one slice per CTA
-    size_t scratch_bytes = 0;
-    char* d_stage = nullptr;        // VW_MEM_HOST: device copies of the caller's arrays
-    char* d_logits = nullptr;       // vw_head_sample: the GEMM's logits when the caller keeps none
-    size_t logits_bytes = 0;
-    int32_t* d_defer = nullptr;     // four counters + the rows the warp-per-row kernel defers
-    size_t defer_cap = 0;
-    size_t stage_bytes = 0;
+    DeviceBuffer scratch;           // general-path scratch, one slice per CTA
+    DeviceBuffer stage;             // VW_MEM_HOST: device copies of the caller's arrays
+    DeviceBuffer logits;            // vw_head_sample: the GEMM's logits when the caller keeps none
+    DeviceBuffer defer;             // four counters + the rows the warp-per-row kernel defers
+    std::vector<DeviceBuffer> old_defers;   // outgrown ones that captured calls still use
     vw::DevOptions* d_opts = nullptr;
     vw::DevOptions* h_opts = nullptr;   // pinned upload buffer for option tables > kInlineOptions
+    std::vector<vw::DevOptions*> captured_opts;   // upload buffers of captured calls, one each
     size_t opts_cap = 0;
     cudaEvent_t opts_done = nullptr;
     unsigned long long* d_stats = nullptr;   // vw::kNumStats per-path row counters
@@ -112,20 +110,32 @@ inline vw_status let_go(vw_handle* h, DeviceBuffer* b, std::vector<DeviceBuffer>
     return VW_OK;
 }
 
-// Grows a buffer of the handle to `need` bytes (waits for the handle's stream before it frees the old one).
-inline vw_status grow(vw_handle* h, char** buf, size_t* cap, size_t need, const char* what) {
-    if (need <= *cap) return VW_OK;
-    if (*buf) {
-        cudaError_t e = cudaStreamSynchronize(h->stream);
+// Whether work enqueued on `st` goes into a CUDA graph instead of running.
+inline bool is_capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
+}
+
+// Grows a buffer of the handle to `need` bytes, for a call that is being captured or not.  The old one is freed when the
+// device is done with it; inside a capture, where that cannot be waited for, it is put aside.
+inline vw_status grow(vw_handle* h, DeviceBuffer* b, size_t need, const char* what, bool capturing = false,
+                      std::vector<DeviceBuffer>* aside = nullptr) {
+    if (need <= b->bytes) {
+        b->captured = b->captured || capturing;
+        return VW_OK;
+    }
+    if (b->p) {
+        b->captured = b->captured || capturing;
+        const cudaError_t e = capturing ? cudaSuccess : cudaDeviceSynchronize();
         if (e != cudaSuccess) return cuda_fail(h, e, what);
-        cudaFree(*buf);
-        *buf = nullptr;
-        *cap = 0;
+        const vw_status r = let_go(h, b, aside ? aside : &h->old_buffers, what);
+        if (r != VW_OK) return r;
     }
     const size_t n = round_up(need + need / 4, 1 << 20);
-    cudaError_t e = cudaMalloc(reinterpret_cast<void**>(buf), n);
+    const cudaError_t e = cudaMalloc(reinterpret_cast<void**>(&b->p), n);
     if (e != cudaSuccess) return cuda_fail(h, e, what);
-    *cap = n;
+    b->bytes = n;
+    b->captured = capturing;
     return VW_OK;
 }
 
