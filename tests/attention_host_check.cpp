@@ -33,6 +33,8 @@ static std::set<const void*> upload_sources;         // pinned memory that a cap
 static std::set<cudaStream_t> capturing;
 static std::set<cudaEvent_t> recorded;
 static uintptr_t next_handle = 0x1000;
+static unsigned* late_word = nullptr;                // gets late_bits when the host next waits for a stream
+static unsigned late_bits = 0;
 static cudaError_t next_launch = cudaSuccess;        // what the next decode launch returns
 
 static void note(const char* what, cudaStream_t st = nullptr, const void* p = nullptr, size_t n = 0) {
@@ -98,7 +100,11 @@ cudaError_t cudaMemsetAsync(void* p, int v, size_t n, cudaStream_t st) {
     return std::memset(p, v, n), note("memset", st, p, n), cudaSuccess;
 }
 cudaError_t cudaDeviceSynchronize() { return note("device sync"), unless_capturing(); }
-cudaError_t cudaStreamSynchronize(cudaStream_t st) { return note("stream sync", st), unless_capturing(); }
+cudaError_t cudaStreamSynchronize(cudaStream_t st) {
+    if (late_word) *late_word |= late_bits;
+    late_word = nullptr;
+    return note("stream sync", st), unless_capturing();
+}
 cudaError_t cudaStreamCreateWithFlags(cudaStream_t* s, unsigned) {
     return *s = reinterpret_cast<cudaStream_t>(next_handle += 16), cudaSuccess;
 }
@@ -343,12 +349,51 @@ static void captured_sampler() {
     expect(live.empty() && pinned.empty(), "the handle leaves nothing allocated");
 }
 
+static size_t clears(const char* base, size_t bytes, size_t from) {   // of memory [base, base + bytes) since ops[from]
+    size_t n = 0;
+    for (size_t i = from; i < ops.size(); ++i) {
+        const char* p = static_cast<const char*>(ops[i].ptr);
+        n += ops[i].what == "memset" && p >= base && p < base + bytes;
+    }
+    return n;
+}
+// An error of one stream's call, read there, leaves alone what a call that runs on another stream counts with, and an
+// error that arrives meanwhile.  Only a wait that gave up leaves counters to clear, once nothing runs.
+static void error_on_another_stream() {
+    Calls c;
+    cudaStream_t a = c.stream(), b = c.stream();
+    expect(c.decode(40, b, 2) == VW_OK && c.prompt(300, b) == VW_OK && c.sample(8, 64, 1, b) == VW_OK, "calls on one stream");
+    for (unsigned bit = 1; bit <= vw::kErrKvLens; bit *= 2) {
+        const size_t from = ops.size();
+        *c.h->d_err |= bit;
+        late_word = c.h->d_err;
+        late_bits = bit == vw::kErrPosition ? vw::kErrCodeRange : vw::kErrPosition;
+        expect(vw_synchronize(c.h, a) != VW_OK, "an error is reported");
+        const size_t cleared = clears(c.h->attn_counts.p, c.h->attn_counts.bytes, from) +
+                               clears(c.h->defer.p, c.h->defer.bytes, from);
+        if (bit == vw::kErrTimeout) {
+            size_t waited = ops.size();
+            for (size_t i = ops.size(); i-- > from;)
+                if (ops[i].what == "device sync") waited = i;
+            expect(cleared == 2 && clears(c.h->attn_counts.p, c.h->attn_counts.bytes, waited) == 1 &&
+                       clears(c.h->defer.p, c.h->defer.bytes, waited) == 1,
+                   "counters are cleared once nothing runs");
+        } else {
+            expect(cleared == 0, "counters of another stream's calls were cleared");
+        }
+        expect(vw_synchronize(c.h, b) != VW_OK, "an error that arrived meanwhile is reported too");
+        expect(vw_synchronize(c.h, b) == VW_OK && *c.h->d_err == 0, "each once");
+    }
+    vw_destroy(c.h);
+}
+
 int main(int argc, char** argv) {
     const std::map<std::string, std::function<void()>> scenarios = {
         {"captured_workspace", captured_workspace},
         {"outgrown_workspace", outgrown_workspace},
         {"growth_under_capture", growth_under_capture},
         {"captured_sampler", captured_sampler},
+        {"error_on_another_stream", error_on_another_stream},
     };
     const auto it = argc > 1 ? scenarios.find(argv[1]) : scenarios.end();
     if (it == scenarios.end()) return 2;

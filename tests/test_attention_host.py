@@ -23,7 +23,8 @@ def checker(tmp_path_factory):
     return exe
 
 
-SCENARIOS = ["captured_workspace", "outgrown_workspace", "growth_under_capture", "captured_sampler"]
+SCENARIOS = ["captured_workspace", "outgrown_workspace", "growth_under_capture", "captured_sampler",
+             "error_on_another_stream"]
 
 
 @pytest.mark.parametrize("scenario", SCENARIOS)

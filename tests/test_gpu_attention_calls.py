@@ -66,3 +66,40 @@ def test_captured_step_outlives_the_workspace_it_was_captured_with(fresh, prefix
         _check_decode(pool, table, ptable, q, out, None, lens, prefixes, groups, 128 ** -0.5)
     _check_prompt(pool, prompt_table, pq, pout, None, rows, prompt_lens, 128 ** -0.5)
     del graph
+
+
+def test_an_error_read_on_one_stream_leaves_calls_of_another_alone(device):
+    """Prompts and steps run on one stream while another's calls fail and their errors are read."""
+    import torch
+    from voxwerk_b200 import KvBatch, KvPrefix, VwOutOfRange, decode_attention, prompt_attention, rope_append
+    pool = Pool(1300, 16, 2, 128, seed=22)
+    lens, prefixes = [40 + 37 * i for i in range(30)], [900]
+    table, ptable = pool.table(lens), pool.table(prefixes)
+    q = pool.normal(30, 4, 128)
+    rows = [n // 2 for n in lens]
+    pq = pool.normal(sum(rows), 4, 128)
+    batch, prefix = KvBatch(table, ints(lens)), KvPrefix(ptable, ints(prefixes), ints([0, 30]))
+    prompts = KvBatch(table, ints(lens), ints(offsets_of(rows)))
+    outs = [(torch.full_like(q, 9.0), torch.full_like(pq, 9.0), torch.full_like(q, 9.0)) for _ in range(40)]
+    bad = table[:1].clone()
+    bad[0, 0] = 1300
+    bad_batch = KvBatch(bad, ints([5]))
+    bad_q, bad_k = pool.normal(1, 4, 128), pool.normal(1, 2, 128)
+    bad_out = torch.empty_like(bad_q)
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for step, prompt, alone in outs:
+        decode_attention(device, q, pool.cache, batch, step, prefix=prefix, stream=b.cuda_stream)
+        prompt_attention(device, pq, pool.cache, prompts, prompt, stream=b.cuda_stream)
+        decode_attention(device, q, pool.cache, batch, alone, stream=b.cuda_stream)
+        rope_append(device, bad_q, bad_k, bad_k, pool.cache, bad_batch, None, bad_out, stream=a.cuda_stream)
+        with pytest.raises(VwOutOfRange, match="page"):
+            device.synchronize(a.cuda_stream)
+    device.synchronize(b.cuda_stream)
+    first = outs[0]
+    _check_decode(pool, table, ptable, q, first[0], None, lens, prefixes, [0, 30], 128 ** -0.5)
+    _check_prompt(pool, table, pq, first[1], None, rows, lens, 128 ** -0.5)
+    _check_decode(pool, table, None, q, first[2], None, lens, [], [], 128 ** -0.5)
+    for other in outs[1:]:
+        for x, y in zip(first, other):
+            assert torch.equal(x.view(torch.int16), y.view(torch.int16))

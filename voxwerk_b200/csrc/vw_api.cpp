@@ -294,15 +294,20 @@ vw_status read_device_error(vw_handle* h, cudaStream_t st) {
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     if (e != cudaSuccess) return cuda_fail(h, e, "synchronize");
     const unsigned bits = *h->h_err;
-    if (bits) {
-        cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-        if (h->defer.p) cudaMemsetAsync(h->defer.p, 0, kDeferHeader * sizeof(int32_t), st);
-        for (const DeviceBuffer& b : h->old_defers) cudaMemsetAsync(b.p, 0, kDeferHeader * sizeof(int32_t), st);
-        if (h->attn_counts.p) cudaMemsetAsync(h->attn_counts.p, 0, h->attn_counts.bytes, st);
-        for (const DeviceBuffer& b : h->old_attn_counts) cudaMemsetAsync(b.p, 0, b.bytes, st);
-        cudaStreamSynchronize(st);
+    if (bits & vw::kErrTimeout) {   // its kernel may have left counters behind; calls on other streams still use them
+        e = cudaDeviceSynchronize();
+        const auto clear = [&](const DeviceBuffer& b, size_t bytes) {
+            if (b.p && e == cudaSuccess) e = cudaMemsetAsync(b.p, 0, bytes, st);
+        };
+        clear(h->defer, kDeferHeader * sizeof(int32_t));
+        for (const DeviceBuffer& b : h->old_defers) clear(b, kDeferHeader * sizeof(int32_t));
+        clear(h->attn_counts, h->attn_counts.bytes);
+        for (const DeviceBuffer& b : h->old_attn_counts) clear(b, b.bytes);
     }
-    if (bits & vw::kErrTimeout) return fail(h, VW_ERR_TIMEOUT, "a bounded wait in the sampler kernel gave up");
+    if (bits && e == cudaSuccess) e = vw::clear_error_bits(h->d_err, bits, st);
+    if (bits && e == cudaSuccess) e = cudaStreamSynchronize(st);
+    if (e != cudaSuccess) return cuda_fail(h, e, "error word");
+    if (bits & vw::kErrTimeout) return fail(h, VW_ERR_TIMEOUT, "a bounded wait in a kernel gave up");
     if (bits & vw::kErrHistRange) return fail(h, VW_ERR_OUT_OF_RANGE, "a history id is outside [0, vocab)");
     if (bits & vw::kErrBadOption) return fail(h, VW_ERR_INVALID_ARG, "a row's opt_index is outside the options table");
     if (bits & vw::kErrHistOffsets) return fail(h, VW_ERR_INVALID_ARG, "hist_offsets are negative or decrease");

@@ -230,6 +230,9 @@ cudaError_t launch_exp_diagnostic(const double* x, int64_t n, double* y_libm, do
 cudaError_t launch_head_gemm(const void* a, int64_t lda, const void* b, int64_t ldb, int M, int N, int K, float* out,
                              int64_t ldo, unsigned* err, cudaStream_t stream);
 
+// *err &= ~bits: the errors that were read; others may have been set since.
+cudaError_t clear_error_bits(unsigned* err, unsigned bits, cudaStream_t stream);
+
 // Sampler.ApplyRepetitionPenalty on one device row, in place.
 cudaError_t launch_apply_penalty(float* logits, int vocab, const int32_t* hist, int64_t hist_len, float penalty,
                                  unsigned* err, cudaStream_t stream);

@@ -1879,6 +1879,13 @@ cudaError_t launch_apply_penalty(float* logits, int vocab, const int32_t* hist, 
     return cudaGetLastError();
 }
 
+__global__ void clear_bits_kernel(unsigned* word, unsigned bits) { atomicAnd(word, ~bits); }
+
+cudaError_t clear_error_bits(unsigned* err, unsigned bits, cudaStream_t stream) {
+    clear_bits_kernel<<<1, 1, 0, stream>>>(err, bits);
+    return cudaGetLastError();
+}
+
 }  // namespace vw
 
 namespace vw {
