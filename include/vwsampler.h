@@ -136,7 +136,8 @@ const char* vw_last_error(const vw_handle* handle);
  * stream: a cudaStream_t for VW_MEM_DEVICE calls, or NULL.  With NULL the call runs on the handle's stream and
  *   returns after the ids are written, reporting device-side errors.  With a stream the call is enqueued and
  *   returns at once; device-side errors (history id out of range, timeout) are reported by the next
- *   vw_synchronize() on that stream.  VW_MEM_HOST calls are always synchronous.
+ *   vw_synchronize() on that stream, or by the next call that returns after its work, if that comes first.
+ *   VW_MEM_HOST calls are always synchronous.
  *   A call captured into a CUDA graph keeps its buffers and its options until vw_destroy; the graph must not be
  *   replayed after that.
  */

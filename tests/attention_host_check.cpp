@@ -387,6 +387,46 @@ static void error_on_another_stream() {
     vw_destroy(c.h);
 }
 
+// A call that returns after its work reports what calls enqueued before it left, too.
+static void error_of_an_enqueued_call() {
+    Calls c;
+    vw_batch* b = nullptr;
+    expect(vw_batch_create(c.h, 4, 64, 10, 3, 0, 0, 0, &b) == VW_OK, "batch");
+    const vw_options o{1, 50, 1.0f, 0.9f, 1.0f};
+    const int32_t ids[1] = {0};
+    float row[4] = {};
+    float* out = reinterpret_cast<float*>(c.memory);
+    const uint16_t* table[1] = {reinterpret_cast<uint16_t*>(c.memory)};
+    const std::vector<std::pair<const char*, std::function<vw_status()>>> calls = {
+        {"prompt", [&] { return c.prompt(20, nullptr); }},
+        {"decode", [&] { return c.decode(5, nullptr); }},
+        {"decode with a prefix", [&] { return c.decode(5, nullptr, 2); }},
+        {"append", [&] { return c.append(5, nullptr); }},
+        {"sample", [&] { return c.sample(8, 64, 1, nullptr); }},
+        {"head and sample", [&] { return c.head(8, 64, nullptr); }},
+        {"head", [&] { return vw_head_logits(c.h, c.memory, 64, 64, c.memory, 64, 8, 64, out, nullptr); }},
+        {"batch head", [&] {
+             return vw_batch_sub_head_step(b, 1, c.memory, 64, 64, c.memory, 64, 64, &o, 1, c.ints(), nullptr, nullptr);
+         }},
+        {"code embedding", [&] { return vw_batch_code_embedding(b, 1, c.memory, 8, 8, out, 8, nullptr); }},
+        {"frame embedding", [&] {
+             return vw_frame_embedding(c.h, c.ints(), 2, 2, 8, table[0], 8, table, 8, nullptr, out, nullptr);
+         }},
+        {"penalty", [&] { return vw_apply_repetition_penalty(c.h, row, 4, ids, 1, 1.5f, VW_MEM_HOST); }},
+    };
+    for (const auto& call : calls) {
+        expect(call.second() == VW_OK, call.first);
+        *c.h->d_err |= vw::kErrPageRange;
+        if (call.second() != VW_ERR_OUT_OF_RANGE) {
+            expect(false, "an earlier call's error was lost by");
+            std::printf("    %s\n", call.first);
+        }
+        expect(call.second() == VW_OK, "and is reported once");
+    }
+    vw_batch_destroy(b);
+    vw_destroy(c.h);
+}
+
 int main(int argc, char** argv) {
     const std::map<std::string, std::function<void()>> scenarios = {
         {"captured_workspace", captured_workspace},
@@ -394,6 +434,7 @@ int main(int argc, char** argv) {
         {"growth_under_capture", growth_under_capture},
         {"captured_sampler", captured_sampler},
         {"error_on_another_stream", error_on_another_stream},
+        {"error_of_an_enqueued_call", error_of_an_enqueued_call},
     };
     const auto it = argc > 1 ? scenarios.find(argv[1]) : scenarios.end();
     if (it == scenarios.end()) return 2;

@@ -103,3 +103,29 @@ def test_an_error_read_on_one_stream_leaves_calls_of_another_alone(device):
     for other in outs[1:]:
         for x, y in zip(first, other):
             assert torch.equal(x.view(torch.int16), y.view(torch.int16))
+
+
+def test_a_call_that_waits_reports_an_enqueued_call_s_error(fresh):
+    """Whichever call waits next: an attention call, or the sampler's."""
+    import torch
+    from voxwerk_b200 import (KvBatch, SamplingOptions, Segment, VwInvalidArgument, decode_attention, prompt_attention,
+                              rope_append, sample_rows, vw_options)
+    pool = Pool(20, 16, 2, 64, seed=23)
+    table = pool.table([20, 30])
+    q, k = pool.normal(2, 4, 64), pool.normal(2, 2, 64)
+    out = torch.empty_like(q)
+    good, bad = KvBatch(table, ints([20, 30])), KvBatch(table, ints([20, -1]))
+    ids = torch.empty(2, dtype=torch.int32, device="cuda")
+    segment = Segment(torch.randn((2, 64), device="cuda"), out_ids=ids)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for waits in (lambda: prompt_attention(fresh, q, pool.cache, good, out),
+                  lambda: decode_attention(fresh, q, pool.cache, good, out),
+                  lambda: rope_append(fresh, q, k, k, pool.cache, good, None, out),
+                  lambda: sample_rows(fresh, [segment], [vw_options(SamplingOptions.greedy())])):
+        waits()
+        decode_attention(fresh, q, pool.cache, bad, out, stream=stream.cuda_stream)
+        stream.synchronize()
+        with pytest.raises(VwInvalidArgument, match="kv_lens"):
+            waits()
+        waits()

@@ -528,9 +528,7 @@ vw_status sample_impl(vw_handle* h, const vw_segment* segs, int32_t n_segs, cons
     p.done_count = reinterpret_cast<uint32_t*>(defer) + 1;
     p.deferred_rows = defer + kDeferHeader;
 
-    cudaError_t e = cudaSuccess;
-    if (sync) e = cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess) e = vw::launch_sampler(p, plan, st);
+    cudaError_t e = vw::launch_sampler(p, plan, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "sampler launch");
     if (mem == VW_MEM_HOST) {
         for (int i = 0; i < n_segs && e == cudaSuccess; ++i) {
@@ -969,10 +967,8 @@ vw_status batch_head_step(vw_batch* b, int which, int group, const void* hidden,
     r = grow(h, &b->logits, need, "batch logits buffer", stream && is_capturing(st));
     if (r != VW_OK) return r;
     float* logits = reinterpret_cast<float*>(b->logits.p);
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess)
-        e = vw::launch_head_gemm(hidden, hidden_stride, weight, weight_stride, b->d.n_slots, vocab, hidden_size,
-                                 logits, vocab, h->d_err, st);
+    cudaError_t e = vw::launch_head_gemm(hidden, hidden_stride, weight, weight_stride, b->d.n_slots, vocab,
+                                         hidden_size, logits, vocab, h->d_err, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "head GEMM");
     r = batch_step(b, which, logits, vocab, vocab, VW_F32, options, n_options, out_ids, out_done, st,
                    embed ? &emb : nullptr);
@@ -1015,9 +1011,7 @@ VW_EXPORT vw_status vw_batch_code_embedding(vw_batch* b, int32_t group, const vo
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, VW_ERR_CUDA, "cudaSetDevice failed");
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess)
-        e = vw::launch_batch_code_embedding(b->d, group, emb, h->d_err, st);
+    cudaError_t e = vw::launch_batch_code_embedding(b->d, group, emb, h->d_err, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "code embedding");
     if (!stream) return read_device_error(h, st);
     return VW_OK;
@@ -1084,10 +1078,8 @@ VW_EXPORT vw_status vw_frame_embedding(vw_handle* h, const int32_t* codes, int32
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, VW_ERR_CUDA, "cudaSetDevice failed");
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess)
-        e = vw::launch_frame_embedding(codes, n_rows, n_groups, hidden, tables, vocab, cp_vocab, text, out, h->d_err,
-                                       st);
+    cudaError_t e = vw::launch_frame_embedding(codes, n_rows, n_groups, hidden, tables, vocab, cp_vocab, text, out,
+                                               h->d_err, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "frame embedding");
     if (!stream) return read_device_error(h, st);
     return VW_OK;
@@ -1106,10 +1098,8 @@ VW_EXPORT vw_status vw_head_logits(vw_handle* h, const void* hidden, int64_t hid
     DeviceGuard guard(h->device);
     if (!guard.ok()) return fail(h, VW_ERR_CUDA, "cudaSetDevice failed");
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess)
-        e = vw::launch_head_gemm(hidden, hidden_stride, weight, weight_stride, n_rows, vocab, hidden_size, out_logits,
-                                 vocab, h->d_err, st);
+    cudaError_t e = vw::launch_head_gemm(hidden, hidden_stride, weight, weight_stride, n_rows, vocab, hidden_size,
+                                         out_logits, vocab, h->d_err, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "head GEMM");
     if (!stream) return read_device_error(h, st);
     return VW_OK;
@@ -1136,10 +1126,8 @@ VW_EXPORT vw_status vw_head_sample(vw_handle* h, const void* hidden, int64_t hid
         if (r != VW_OK) return r;
         logits = reinterpret_cast<float*>(h->logits.p);
     }
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess)
-        e = vw::launch_head_gemm(hidden, hidden_stride, weight, weight_stride, sg.n_rows, sg.vocab, hidden_size,
-                                 logits, sg.vocab, h->d_err, st);
+    cudaError_t e = vw::launch_head_gemm(hidden, hidden_stride, weight, weight_stride, sg.n_rows, sg.vocab,
+                                         hidden_size, logits, sg.vocab, h->d_err, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "head GEMM");
     sg.logits = logits;
     sg.row_stride = sg.vocab;
@@ -1175,7 +1163,6 @@ VW_EXPORT vw_status vw_apply_repetition_penalty(vw_handle* h, float* logits, int
             e = cudaMemcpyAsync(dh, history, static_cast<size_t>(history_len) * 4, cudaMemcpyHostToDevice, st);
         d_hist = dh;
     }
-    if (e == cudaSuccess) e = cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
     if (e == cudaSuccess) e = vw::launch_apply_penalty(d_logits, vocab, d_hist, history_len, penalty, h->d_err, st);
     if (e == cudaSuccess && mem == VW_MEM_HOST)
         e = cudaMemcpyAsync(logits, d_logits, static_cast<size_t>(vocab) * 4, cudaMemcpyDeviceToHost, st);

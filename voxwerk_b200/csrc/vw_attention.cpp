@@ -200,8 +200,7 @@ VW_EXPORT vw_status vw_rope_append(vw_handle* h, const vw_kv_cache* cache, const
     p.cache = cache_dev(*cache);
     p.batch = batch_dev(*batch);
     p.err = h->d_err;
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
-    if (e == cudaSuccess) e = vw::launch_rope_append(p, h->sm_count, st);
+    const cudaError_t e = vw::launch_rope_append(p, h->sm_count, st);
     if (e != cudaSuccess) return cuda_fail(h, e, "rope append");
     if (!stream) return read_device_error(h, st);
     return VW_OK;
@@ -222,9 +221,8 @@ VW_EXPORT vw_status vw_prompt_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (!guard.ok()) return fail(h, VW_ERR_CUDA, "cudaSetDevice failed");
     cudaStream_t st = stream ? static_cast<cudaStream_t>(stream) : h->stream;
     vw::AttnParams p{rows_dev(*rows), cache_dev(*cache), batch_dev(*batch), vw::KvPrefixDev{}, h->d_err};
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
     bool capturing = false;
-    if (e == cudaSuccess) e = enter_workspace(h, st, &capturing);
+    cudaError_t e = enter_workspace(h, st, &capturing);
     if (e != cudaSuccess) return cuda_fail(h, e, "prompt attention");
     const vw::TilePlan plan = vw::plan_prompt(p, h->sm_count);
     vw::TileWork w{};
@@ -263,9 +261,8 @@ VW_EXPORT vw_status vw_decode_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (prefix && prefix->n_groups > 0)
         p.prefix = {prefix->page_table, prefix->page_table_stride, prefix->max_pages, prefix->n_groups, prefix->lens,
                     prefix->group_offsets};
-    cudaError_t e = stream ? cudaSuccess : cudaMemsetAsync(h->d_err, 0, sizeof(unsigned), st);
     bool capturing = false;
-    if (e == cudaSuccess) e = enter_workspace(h, st, &capturing);
+    cudaError_t e = enter_workspace(h, st, &capturing);
     if (e != cudaSuccess) return cuda_fail(h, e, "decode attention");
     const vw::DecodePlan plan = vw::plan_decode(p, h->sm_count);
     vw::TilePlan prefix_plan{};
