@@ -427,6 +427,45 @@ static void error_of_an_enqueued_call() {
     vw_destroy(c.h);
 }
 
+// Attention calls share the workspace: each waits for the one before it, whatever its stream's handle says (a new stream
+// may have a destroyed one's), also where that one stopped half way.
+static void workspace_order() {
+    Calls c;
+    cudaStream_t a = c.stream(), b = c.stream();
+    const auto waits_for_the_last = [&](const char* what, const std::function<vw_status()>& call, cudaStream_t st) {
+        size_t launch = 0;   // the last launch so far, and the record behind it
+        for (size_t i = 0; i < ops.size(); ++i)
+            if (ops[i].what == "launch") launch = i;
+        const void* event = nullptr;
+        for (size_t i = launch; i < ops.size(); ++i)
+            if (ops[i].what == "record" && ops[i].stream == ops[launch].stream) event = ops[i].ptr;
+        const size_t from = ops.size();
+        expect(call() == VW_OK, what);
+        bool waited = false, launched_before = false;
+        for (size_t i = from; i < ops.size(); ++i) {
+            launched_before = launched_before || ops[i].what == "launch";
+            waited = waited || (!launched_before && ops[i].what == "wait" && ops[i].stream == st && ops[i].ptr == event);
+        }
+        expect(event && waited, what);
+    };
+    expect(c.decode(40, a, 2) == VW_OK && c.prompt(300, a) == VW_OK, "first calls");
+    waits_for_the_last("on another stream", [&] { return c.decode(40, b, 2); }, b);
+    waits_for_the_last("on a stream with the same handle", [&] { return c.decode(40, b, 2); }, b);
+    waits_for_the_last("a prompt on it", [&] { return c.prompt(300, b); }, b);
+    waits_for_the_last("on the handle's stream", [&] { return c.prompt(300, nullptr); }, c.h->stream);
+    next_launch = cudaErrorInvalidValue;
+    expect(c.decode(40, a, 2) == VW_ERR_CUDA, "a call whose second kernel does not start");
+    next_launch = cudaSuccess;
+    waits_for_the_last("after a call that stopped half way", [&] { return c.decode(40, b); }, b);
+    // within a capture no event of uncaptured work is waited for, and none is recorded
+    capturing.insert(a);
+    const size_t from = ops.size();
+    expect(c.decode(40, a, 2) == VW_OK && c.prompt(300, a) == VW_OK, "captured");
+    expect(count("wait", from) == 0 && count("record", from) == 0, "captured calls are ordered by their graph");
+    capturing.clear();
+    vw_destroy(c.h);
+}
+
 int main(int argc, char** argv) {
     const std::map<std::string, std::function<void()>> scenarios = {
         {"captured_workspace", captured_workspace},
@@ -435,6 +474,7 @@ int main(int argc, char** argv) {
         {"captured_sampler", captured_sampler},
         {"error_on_another_stream", error_on_another_stream},
         {"error_of_an_enqueued_call", error_of_an_enqueued_call},
+        {"workspace_order", workspace_order},
     };
     const auto it = argc > 1 ? scenarios.find(argv[1]) : scenarios.end();
     if (it == scenarios.end()) return 2;

@@ -24,7 +24,7 @@ def checker(tmp_path_factory):
 
 
 SCENARIOS = ["captured_workspace", "outgrown_workspace", "growth_under_capture", "captured_sampler",
-             "error_on_another_stream", "error_of_an_enqueued_call"]
+             "error_on_another_stream", "error_of_an_enqueued_call", "workspace_order"]
 
 
 @pytest.mark.parametrize("scenario", SCENARIOS)

@@ -70,21 +70,21 @@ vw::AttnRowsDev rows_dev(const vw_attn_rows& r) {
             static_cast<__nv_bfloat16*>(r.out), r.out_row_stride, r.out_head_stride, r.lse, r.n_q_heads, r.scale};
 }
 
-// The attention workspace is one buffer of the handle: a call on another stream than the last one waits for it.  Inside
-// a stream capture no order is added (an event of uncaptured work cannot be waited for there): the caller orders its
-// graphs.
+// The attention workspace is one buffer of the handle: a call waits for the one before it, whose stream may be another
+// though its handle is the same (a new stream can have a destroyed one's; one handle names every thread's default
+// stream).  Inside a stream capture no order is added (an event of uncaptured work cannot be waited for there): the caller
+// orders its graphs.
 cudaError_t enter_workspace(vw_handle* h, cudaStream_t st, bool* capturing) {
     cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
     cudaError_t e = cudaStreamIsCapturing(st, &cap);
     *capturing = cap != cudaStreamCaptureStatusNone;
-    if (e == cudaSuccess && !*capturing && h->attn_stream && h->attn_stream != st)
-        e = cudaStreamWaitEvent(st, h->attn_done, 0);
+    if (e == cudaSuccess && !*capturing) e = cudaStreamWaitEvent(st, h->attn_done, 0);   // (no call yet: nothing to wait for)
     return e;
 }
-cudaError_t leave_workspace(vw_handle* h, cudaStream_t st, bool capturing) {
-    if (capturing) return cudaSuccess;
-    h->attn_stream = st;
-    return cudaEventRecord(h->attn_done, st);
+// `e` is how the call's launches went: what they enqueued is recorded in either case.
+cudaError_t leave_workspace(vw_handle* h, cudaStream_t st, bool capturing, cudaError_t e) {
+    const cudaError_t r = capturing ? cudaSuccess : cudaEventRecord(h->attn_done, st);
+    return e != cudaSuccess ? e : r;
 }
 
 // Grows one of the two attention buffers (clear: the one whose contents are zero between calls).  Not inside a capture:
@@ -230,7 +230,7 @@ VW_EXPORT vw_status vw_prompt_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (r == VW_OK) r = reserve_parts(h, st, capturing, [&](auto take) { carve_tiles(h, plan, take, &w); });
     if (r != VW_OK) return r;
     e = vw::launch_prompt_attention(p, plan, w, st);
-    if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
+    e = leave_workspace(h, st, capturing, e);
     if (e != cudaSuccess) return cuda_fail(h, e, "prompt attention");
     if (!stream) return read_device_error(h, st);
     return VW_OK;
@@ -283,7 +283,7 @@ VW_EXPORT vw_status vw_decode_attention(vw_handle* h, const vw_kv_cache* cache, 
     if (p.prefix.n_groups > 0) e = vw::launch_prefix_attention(p, prefix_plan, w.prefix, st);
     if (e == cudaSuccess) e = vw::launch_decode_attention(p, plan, w, st);
     if (e != cudaSuccess) cudaMemsetAsync(h->attn_counts.p, 0, h->attn_counts.bytes, st);   // the join would have
-    if (e == cudaSuccess) e = leave_workspace(h, st, capturing);
+    e = leave_workspace(h, st, capturing, e);
     if (e != cudaSuccess) return cuda_fail(h, e, "decode attention");
     if (!stream) return read_device_error(h, st);
     return VW_OK;

@@ -52,8 +52,7 @@ struct vw_handle {
     DeviceBuffer attn_counts;                // attention: counters and tickets, zero between calls
     std::vector<DeviceBuffer> old_attn_counts;   // outgrown ones that captured calls still use
     std::vector<DeviceBuffer> old_buffers;       // likewise, of any other use
-    cudaStream_t attn_stream = nullptr;      // the stream of the last call that used it, and its end on that stream
-    cudaEvent_t attn_done = nullptr;
+    cudaEvent_t attn_done = nullptr;         // the end of the last call that used them
     std::vector<vw_batch*> batches;          // live batches created on this handle (released by vw_destroy)
     std::string last_error;
 };
