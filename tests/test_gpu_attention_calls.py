@@ -129,3 +129,18 @@ def test_a_call_that_waits_reports_an_enqueued_call_s_error(fresh):
         with pytest.raises(VwInvalidArgument, match="kv_lens"):
             waits()
         waits()
+
+
+def test_prompt_with_fewer_rows_than_sequences(device):
+    """Without q_offsets row s is sequence s; sequences past the last row have none, which is no error."""
+    import torch
+    from voxwerk_b200 import KvBatch, prompt_attention
+    pool = Pool(60, 16, 2, 64, seed=24)
+    lens = [70, 5, 33, 0, 90]
+    table = pool.table(lens)
+    for rows in (1, 2, 3, 5):
+        q = pool.normal(rows, 4, 64)
+        out, ls = torch.full_like(q, 9.0), torch.full((rows, 4), 9.0, device="cuda")
+        torch.cuda.synchronize()
+        prompt_attention(device, q, pool.cache, KvBatch(table, ints(lens)), out, lse=ls)
+        _check_prompt(pool, table, q, out, ls, [1] * rows, lens[:rows], 0.125)

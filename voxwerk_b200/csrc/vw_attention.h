@@ -176,7 +176,7 @@ __device__ __forceinline__ Seq load_seq(const AttnParams& a, int s) {
     const int shift = a.cache.page_shift;
     const int32_t* o = kPrefix ? a.prefix.group_offsets : a.batch.q_offsets;
     const int limit = kPrefix ? a.batch.n_seqs : a.batch.n_rows;
-    int begin = s, end = min(s + 1, limit);
+    int begin = min(s, limit), end = min(s + 1, limit);   // (fewer rows than sequences: the later ones have none)
     if (o) {
         begin = __ldg(o + s);
         end = __ldg(o + s + 1);
