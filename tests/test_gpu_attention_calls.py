@@ -144,3 +144,35 @@ def test_prompt_with_fewer_rows_than_sequences(device):
         torch.cuda.synchronize()
         prompt_attention(device, q, pool.cache, KvBatch(table, ints(lens)), out, lse=ls)
         _check_prompt(pool, table, q, out, ls, [1] * rows, lens[:rows], 0.125)
+
+
+@pytest.mark.parametrize("n,rows", [(2, 20), (70, 500), (300, 4)])
+def test_append_reports_row_offsets_that_do_not_fit(device, n, rows):
+    """Offsets past the rows, below zero or descending are reported, as by the attention calls; the rows of a sequence
+    whose own offsets do not fit are left alone."""
+    import torch
+    from voxwerk_b200 import KvBatch, VwInvalidArgument, rope_append
+    pool = Pool(8 * n + 1, 16, 1, 64, seed=25)
+    lens = [100] * n
+    table = pool.table(lens, fill=False)
+    q, k = pool.normal(rows, 2, 64), pool.normal(rows, 1, 64)
+    q_out = torch.full_like(q, 9.0)
+    good = [rows * s // n for s in range(n + 1)]
+    past, below, descending = list(good), list(good), list(good)
+    past[n] = rows + 1
+    below[0] = -3
+    descending[n // 2 + 1] = good[n // 2] - 1
+    torch.cuda.synchronize()
+    for offsets, alone in ((past, [n - 1]), (below, [0]), (descending, [])):
+        q_out.fill_(9.0), pool.k.fill_(float("nan"))
+        torch.cuda.synchronize()
+        with pytest.raises(VwInvalidArgument, match="q_offsets"):
+            rope_append(device, q, k, k, pool.cache, KvBatch(table, ints(lens), ints(offsets)), None, q_out)
+        for s in alone:
+            assert bool((q_out[max(offsets[s], 0):min(offsets[s + 1], rows)] == 9.0).all()), "rows were written"
+            assert bool(torch.isnan(pool.k[table[s].long()]).all()), "keys were written"
+        others = [s for s in range(n) if s not in alone and offsets is not descending]
+        for s in others:
+            assert torch.equal(q_out[offsets[s]:offsets[s + 1]], q[offsets[s]:offsets[s + 1]])
+    rope_append(device, q, k, k, pool.cache, KvBatch(table, ints(lens), ints(good)), None, q_out)
+    assert torch.equal(q_out, q)

@@ -43,6 +43,7 @@ __device__ RowPlace place_row(const RopeParams& p, int row, int lane) {
         if (seq < 0) return r;
         begin = b.q_offsets[seq];
         end = b.q_offsets[seq + 1];
+        if (begin < 0 || end > b.n_rows) return r;   // (offsets_fit reports it)
     }
     if (row < begin || row >= end) return r;   // a padding row
     const int len = b.kv_lens[seq];
@@ -64,6 +65,17 @@ __device__ RowPlace place_row(const RopeParams& p, int row, int lane) {
     r.slot = page * p.cache.page_stride + (index & (p.cache.page_size - 1)) * p.cache.token_stride;
     r.pos = pos;
     return r;
+}
+
+// Reports row offsets that are negative, descend or pass the rows, of every thread's share of the sequences.
+__device__ __forceinline__ void offsets_fit(const RopeParams& p) {
+    const KvBatchDev& b = p.batch;
+    if (!b.q_offsets) return;
+    const int threads = gridDim.x * kThreads;
+    for (int s = blockIdx.x * kThreads + threadIdx.x; s < b.n_seqs; s += threads) {
+        const int begin = b.q_offsets[s], end = b.q_offsets[s + 1];
+        if (begin < 0 || end < begin || end > b.n_rows) atomicOr(p.err, kErrKvLens);
+    }
 }
 
 // CH elements as they were loaded
@@ -361,6 +373,7 @@ rope_append_kernel(const __grid_constant__ RopeParams p, int team_shift, int gro
             heads_of(std::true_type{}, raw_q, v, p.v_head, n_kv, nullptr, v_to, p.cache.head_stride, false);
         }
     }
+    offsets_fit(p);   // last: what it reads was read for the rows before, so that it costs them nothing
 }
 
 bool multiple(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
