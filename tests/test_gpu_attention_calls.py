@@ -176,3 +176,48 @@ def test_append_reports_row_offsets_that_do_not_fit(device, n, rows):
             assert torch.equal(q_out[offsets[s]:offsets[s + 1]], q[offsets[s]:offsets[s + 1]])
     rope_append(device, q, k, k, pool.cache, KvBatch(table, ints(lens), ints(good)), None, q_out)
     assert torch.equal(q_out, q)
+
+
+def _us(call, times=5):
+    """The shortest of some calls, on the device."""
+    import torch
+    best = float("inf")
+    for _ in range(times):
+        start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        start.record()
+        call()
+        end.record()
+        torch.cuda.synchronize()
+        best = min(best, start.elapsed_time(end) * 1e3)
+    return best
+
+
+@pytest.mark.parametrize("n,heads,kv", [(256, 16, 2), (4096, 64, 1)])
+def test_prompts_after_very_different_numbers_of_keys(device, n, heads, kv):
+    """Many short prompts and one that continues 8000 cached keys: right, and no slower than the two apart.  The long one's
+    block is one CTA's work, 63 key tiles of at most 2.3 us each; twice the sum, for the timing's sake."""
+    import torch
+    from voxwerk_b200 import KvBatch, prompt_attention
+    pool = Pool(n + 40, 256, kv, 64, seed=26)
+    rows = [1 + i % 3 for i in range(n)]
+    short = list(rows)
+    mixed = list(rows)
+    mixed[n // 3] += 8000
+    stream = torch.cuda.Stream()
+
+    def batch(total, new):
+        table = pool.table(total)
+        q = pool.normal(sum(new), heads, 64)
+        out = torch.full_like(q, 9.0)
+        b = KvBatch(table, ints(total), ints(offsets_of(new)))
+        torch.cuda.synchronize()
+        return (table, q, out), lambda: prompt_attention(device, q, pool.cache, b, out, stream=stream.cuda_stream)
+
+    (table, q, out), call = batch(mixed, rows)
+    with torch.cuda.stream(stream):
+        together = _us(call)
+        _check_prompt(pool, table, q, out, None, rows, mixed, 0.125)
+        pool.free = list(range(n + 40))
+        apart = _us(batch(short, rows)[1]) + 63 * 2.3
+    device.synchronize(stream.cuda_stream)
+    assert together < 2 * apart, f"{together:.0f} us together, {apart:.0f} us apart"
