@@ -345,10 +345,12 @@ vw_status vw_head_sample(vw_handle* handle, const void* hidden, int64_t hidden_s
  *   vw_prompt_attention   rows of several tokens per sequence (whole prompts, or the next piece of one), causal
  *   vw_decode_attention   one row per sequence; groups of sequences may share a prefix (a voice prompt)
  * All pointers in these structs are device memory of the handle's device; tensors of 16-bit elements are bf16 bits.
- * stream as in vw_sample: NULL runs on the handle's stream and returns device-side errors, a stream enqueues.  Device-
- * side errors: a page outside the cache or a position outside the table gives VW_ERR_OUT_OF_RANGE; key counts, row
- * offsets or group offsets that do not fit give VW_ERR_INVALID_ARG (the reference throws when a cache is full,
- * DecoderStack.cs:154).  Nothing outside the cache and the outputs is read or written in either case.
+ * stream as in vw_sample: NULL runs on the handle's stream and returns device-side errors, a stream enqueues.  The
+ * handle's stream waits for no other, so with NULL everything that a call reads has to be there already; the default
+ * stream itself is passed as cudaStreamLegacy.  Device-side errors: a page outside the cache or a position outside the
+ * table gives VW_ERR_OUT_OF_RANGE; key counts, row offsets or group offsets that do not fit give VW_ERR_INVALID_ARG (the
+ * reference throws when a cache is full, DecoderStack.cs:154).  Nothing outside the cache and the outputs is read or
+ * written in either case.
  * Calls of one handle on different streams are ordered by the library (they share the handle's workspace); work that a
  * caller captures into CUDA graphs it orders itself.  A capture cannot grow the workspace: an attention call that needs
  * more than an earlier one outside a capture is refused there (VW_ERR_INVALID_ARG).  A workspace that a captured call

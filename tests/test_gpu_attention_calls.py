@@ -221,3 +221,46 @@ def test_prompts_after_very_different_numbers_of_keys(device, n, heads, kv):
         apart = _us(batch(short, rows)[1]) + 63 * 2.3
     device.synchronize(stream.cuda_stream)
     assert together < 2 * apart, f"{together:.0f} us together, {apart:.0f} us apart"
+
+
+@pytest.mark.parametrize("how", ["no stream", "no stream, on a side stream", "default stream"])
+def test_inputs_that_the_current_stream_still_makes(device, how):
+    """A call is in order with the kernels that make its inputs and with those that read its outputs."""
+    import contextlib
+    import torch
+    from voxwerk_b200 import KvBatch, decode_attention, prompt_attention, rope_append
+    pool = Pool(40, 16, 2, 64, seed=27)
+    lens = [100, 60, 33]
+    table = pool.table(lens)
+    batch, prompts = KvBatch(table, ints(lens)), KvBatch(table, ints(lens), ints([0, 40, 60, 90]))
+    made, pmade, kmade = pool.normal(3, 4, 64), pool.normal(90, 4, 64), pool.normal(3, 2, 64)
+    q, pq, k = torch.zeros_like(made), torch.zeros_like(pmade), torch.zeros_like(kmade)
+    out, pout, q_out = torch.full_like(q, 9.0), torch.full_like(pq, 9.0), torch.full_like(q, 9.0)
+    side = torch.cuda.Stream()
+    work = torch.randn((4096, 4096), device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side) if "side" in how else contextlib.nullcontext():
+        stream = 0 if how == "default stream" else None
+        if stream == 0:
+            assert torch.cuda.current_stream().cuda_stream == 0
+        for _ in range(10):
+            work = torch.relu(work @ work) * 1e-4      # some milliseconds
+        q.copy_(made), pq.copy_(pmade), k.copy_(kmade)
+        decode_attention(device, q, pool.cache, batch, out, stream=stream)
+        prompt_attention(device, pq, pool.cache, prompts, pout, stream=stream)
+        got, pgot = out.clone(), pout.clone()
+        q.zero_()
+        for _ in range(10):
+            work = torch.relu(work @ work) * 1e-4
+        q.copy_(made)
+        rope_append(device, q, k, k, pool.cache, batch, None, q_out, stream=stream)
+        written = q_out.clone()
+    torch.cuda.synchronize()
+    device.synchronize()
+    assert torch.equal(written, made)
+    last = [n - 1 for n in lens]
+    assert all(torch.equal(pool.k[table[s, n // 16].long(), n % 16], kmade[s]) for s, n in enumerate(last))
+    keep = Pool(40, 16, 2, 64, seed=27)        # the cache before the last call wrote to it
+    assert torch.equal(keep.table(lens), table)
+    _check_decode(keep, table, None, made, got, None, lens, [], [], 0.125)
+    _check_prompt(keep, table, pmade, pgot, None, [40, 20, 30], lens, 0.125)

@@ -11,9 +11,9 @@ projections, over its ``KvCache`` (:21), for a batch of sequences whose keys and
     decode_attention(device, q_out, cache, batch, out, prefix=KvPrefix(...))    # one row per sequence
 
 ``KvCache``, ``KvBatch``, ``KvPrefix`` and ``RopeTable`` hold references to CUDA tensors; they are built once and keep
-describing the same tensors as their contents change from step to step.  As elsewhere in this package ``stream`` is a
-cudaStream_t (an int): given, a call is enqueued on it; None runs on the device handle's stream, waits, and raises what
-the kernels reported.
+describing the same tensors as their contents change from step to step.  ``stream`` is a cudaStream_t (an int, as
+``torch.cuda.Stream.cuda_stream``; 0 is torch's default stream): given, a call is enqueued on it, behind what the caller
+put there.  None runs on torch's current stream, waits for it, and raises what the kernels reported.
 """
 
 from __future__ import annotations
@@ -29,6 +29,7 @@ from .sampler import Device
 
 
 _BF16, _F32 = torch.bfloat16, torch.float32
+_DEFAULT_STREAM = 1   # cudaStreamLegacy; its other handle, NULL, means the device handle's own stream to the library
 
 
 def _need(ok: bool, message: str) -> None:
@@ -44,6 +45,18 @@ def _cuda(t, dtype: str, dims: int, what: str):
     if t.dim() != dims:
         raise ValueError(f"{what} must have {dims} dimensions")
     return t
+
+
+def _call(function, device: Device, stream: Optional[int], *args) -> None:
+    handle = device.handle
+    if stream is not None:
+        check(function(handle, *args, stream or _DEFAULT_STREAM), handle)
+        return
+    if torch.cuda.is_current_stream_capturing():
+        raise ValueError("a call that is captured takes the capturing stream")
+    stream = torch.cuda.current_stream(device.device).cuda_stream or _DEFAULT_STREAM
+    check(function(handle, *args, stream), handle)
+    check(lib.vw_synchronize(handle, stream), handle)
 
 
 def _rows(t, dtype, shape, what: str):
@@ -211,7 +224,7 @@ def rope_append(device: Device, q, k, v, cache: KvCache, batch: KvBatch, rope: O
                       VW_F32 if dtype is _F32 else VW_BF16, heads, None if q_norm is None else _norm(q_norm, dim, "q_norm"),
                       None if k_norm is None else _norm(k_norm, dim, "k_norm"), eps, n_positions, cos, sin, at, rotary,
                       interleaved, out_ptr, out_row, out_head)
-    check(lib.vw_rope_append(device.handle, cache._ref, batch._rows(n), ctypes.byref(rows), stream), device.handle)
+    _call(lib.vw_rope_append, device, stream, cache._ref, batch._rows(n), ctypes.byref(rows))
 
 
 def _attn_rows(q, out, lse, cache: KvCache, scale: Optional[float]):
@@ -235,8 +248,7 @@ def prompt_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, sca
     [n, n_q_heads, D] bfloat16 (batch.q_offsets gives each sequence's rows, its last keys), scale 1/sqrt(D) unless
     given, lse optionally [n, n_q_heads] float32.  Rows that see no key get 0 and -inf."""
     n, rows = _attn_rows(q, out, lse, cache, scale)
-    check(lib.vw_prompt_attention(device.handle, cache._ref, batch._rows(n), ctypes.byref(rows), stream),
-          device.handle)
+    _call(lib.vw_prompt_attention, device, stream, cache._ref, batch._rows(n), ctypes.byref(rows))
 
 
 def decode_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, prefix: Optional[KvPrefix] = None,
@@ -244,5 +256,5 @@ def decode_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, pre
     """vw_decode_attention: one row per sequence (row s is sequence s; batch.q_offsets is ignored) over all of its keys
     and, with `prefix`, those its group shares, which are read once for the group.  Tensors as in prompt_attention."""
     n, rows = _attn_rows(q, out, lse, cache, scale)
-    check(lib.vw_decode_attention(device.handle, cache._ref, batch._rows(n),
-                                  None if prefix is None else prefix._ref, ctypes.byref(rows), stream), device.handle)
+    _call(lib.vw_decode_attention, device, stream, cache._ref, batch._rows(n), None if prefix is None else prefix._ref,
+          ctypes.byref(rows))
