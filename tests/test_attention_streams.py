@@ -96,3 +96,20 @@ def test_a_call_that_waits_is_refused_inside_a_capture(calls):
         assert library.calls == []
         call(0x5550)
         assert library.calls == [(name, 0x5550)]
+
+
+def test_a_batch_serves_calls_of_different_numbers_of_rows_at_a_time(calls):
+    """Two threads may share a KvBatch: the struct that one call hands over is not changed by the next."""
+    _, library, _, _ = calls
+    cache = attention.KvCache(Tensor(4, 16, 2, 64), Tensor(4, 16, 2, 64))
+    batch = attention.KvBatch(Tensor(2, 2, dtype=torch.int32), Tensor(2, dtype=torch.int32))
+    given = []
+    library.vw_prompt_attention = library.vw_decode_attention = library.vw_rope_append = \
+        lambda handle, cache, batch, *rest: given.append(batch._obj) or 0
+    for n in (2, 5, 3):
+        q, k = Tensor(n, 4, 64), Tensor(n, 2, 64)
+        attention.prompt_attention(FakeDevice, q, cache, batch, Tensor(n, 4, 64), stream=1)
+        attention.decode_attention(FakeDevice, q, cache, batch, Tensor(n, 4, 64), stream=1)
+        attention.rope_append(FakeDevice, q, k, k, cache, batch, None, Tensor(n, 4, 64), stream=1)
+    assert [b.n_rows for b in given] == [2, 2, 2, 5, 5, 5, 3, 3, 3]
+    assert all(b.n_seqs == 2 and b.page_table == batch.page_table.data_ptr() for b in given)

@@ -117,14 +117,16 @@ class KvBatch:
             _cuda(q_offsets, "int32", 1, "q_offsets")
             _need(q_offsets.shape[0] == n + 1 and q_offsets.is_contiguous(), "q_offsets must be a contiguous [n_seqs + 1]")
         self.page_table, self.kv_lens, self.q_offsets, self.n_seqs = page_table, kv_lens, q_offsets, n
-        self.c = VwKvBatch(page_table.data_ptr(), page_table.stride(0) if n > 1 else page_table.shape[1],
-                           page_table.shape[1], n, kv_lens.data_ptr(),
-                           None if q_offsets is None else q_offsets.data_ptr(), 0)
-        self._ref = ctypes.byref(self.c)
+        self._c = (page_table.data_ptr(), page_table.stride(0) if n > 1 else page_table.shape[1], page_table.shape[1], n,
+                   kv_lens.data_ptr(), None if q_offsets is None else q_offsets.data_ptr())
+        self._last = None, None
 
-    def _rows(self, n: int):
-        self.c.n_rows = n
-        return self._ref
+    def _rows(self, n: int):   # a struct once made does not change: threads with a handle each may share a batch
+        rows, ref = self._last
+        if rows != n:
+            ref = ctypes.byref(VwKvBatch(*self._c, n))
+            self._last = n, ref
+        return ref
 
 
 class KvPrefix:
