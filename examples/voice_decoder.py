@@ -94,7 +94,10 @@ class VoiceDecoder:
         return x
 
     def read_voices(self, x):
-        """x [sum(voice_lens), hidden] bfloat16: the voices' prompts, one after the other."""
+        """x [sum(voice_lens), hidden] bfloat16: the voices' prompts, one after the other, as the current stream makes
+        them."""
+        self.stream.wait_stream(torch.cuda.current_stream())
+        x.record_stream(self.stream)      # its memory is not given out again before it has been read
         with torch.cuda.stream(self.stream):
             q = torch.empty((x.shape[0], self.heads, self.dim), dtype=torch.bfloat16, device="cuda")
             out = torch.empty_like(q)

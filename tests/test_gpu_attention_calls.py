@@ -264,3 +264,29 @@ def test_inputs_that_the_current_stream_still_makes(device, how):
     assert torch.equal(keep.table(lens), table)
     _check_decode(keep, table, None, made, got, None, lens, [], [], 0.125)
     _check_prompt(keep, table, pmade, pgot, None, [40, 20, 30], lens, 0.125)
+
+
+def test_voices_that_the_current_stream_still_makes():
+    """The example's prompts may come straight from kernels that are still running, and be dropped at once."""
+    import torch
+    from examples.voice_decoder import VoiceDecoder
+    from voxwerk_b200 import Device
+    with Device(0) as device:
+        make = lambda: VoiceDecoder(device, [37, 80], [0, 1, 1], 4, layers=1, hidden=256, heads=4, kv_heads=2, dim=64,
+                                    inner=512, vocab=512, seed=3)
+        a, b = make(), make()
+        x = torch.randn((117, 256), generator=torch.Generator().manual_seed(4)).to(torch.bfloat16).cuda()
+        work = torch.randn((4096, 4096), device="cuda")
+        torch.cuda.synchronize()
+        want = a.read_voices(x)
+        a.check()
+        for _ in range(10):
+            work = torch.relu(work @ work) * 1e-4      # some milliseconds
+        made = torch.zeros_like(x)
+        made.copy_(x)
+        got = b.read_voices(made)
+        del made
+        reused = [torch.full_like(x, float("nan")) for _ in range(4)]
+        b.check()
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+        del reused
