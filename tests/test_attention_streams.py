@@ -16,6 +16,9 @@ class Tensor:
         self._t = torch.zeros(shape, dtype=dtype)
         self.device = torch.device("cuda", 0)
 
+    def get_device(self):
+        return 0
+
     def __getattr__(self, name):
         return getattr(self._t, name)
 
@@ -113,3 +116,39 @@ def test_a_batch_serves_calls_of_different_numbers_of_rows_at_a_time(calls):
         attention.rope_append(FakeDevice, q, k, k, cache, batch, None, Tensor(n, 4, 64), stream=1)
     assert [b.n_rows for b in given] == [2, 2, 2, 5, 5, 5, 3, 3, 3]
     assert all(b.n_seqs == 2 and b.page_table == batch.page_table.data_ptr() for b in given)
+
+
+def test_tensors_of_another_gpu_are_refused(calls):
+    """The kernels would read them through addresses that the handle's device may not map."""
+    _, library, _, _ = calls
+
+    class Elsewhere(Tensor):
+        def get_device(self):
+            return 1
+
+    def make(where, **other):
+        t = lambda name, *a, **k: (Elsewhere if name == where else Tensor)(*a, **k)
+        ints = dict(dtype=torch.int32)
+        cache = attention.KvCache(t("cache", 4, 16, 2, 64), t("cache", 4, 16, 2, 64))
+        batch = attention.KvBatch(t("batch", 2, 2, **ints), t("batch", 2, **ints))
+        prefix = attention.KvPrefix(t("prefix", 1, 2, **ints), t("prefix", 1, **ints), t("prefix", 2, **ints))
+        rope = attention.RopeTable(t("rope", 9, 32, dtype=torch.float32), t("rope", 9, 32, dtype=torch.float32))
+        q, k, v, out = t("q", 2, 4, 64), t("k", 2, 2, 64), t("v", 2, 2, 64), t("out", 2, 4, 64)
+        norm, lse = t("norm", 64, dtype=torch.float32), t("lse", 2, 4, dtype=torch.float32)
+        positions = t("positions", 2, **ints)
+        return (lambda: attention.rope_append(FakeDevice, q, k, v, cache, batch, rope, out, q_norm=norm, k_norm=norm,
+                                              positions=positions, stream=1),
+                lambda: attention.prompt_attention(FakeDevice, q, cache, batch, out, lse=lse, stream=1),
+                lambda: attention.decode_attention(FakeDevice, q, cache, batch, out, prefix=prefix, lse=lse, stream=1))
+
+    for call in make(None):
+        call()
+    assert len(library.calls) == 3
+    library.calls.clear()
+    for where, callers in (("cache", (0, 1, 2)), ("batch", (0, 1, 2)), ("q", (0, 1, 2)), ("out", (0, 1, 2)), ("k", (0,)),
+                           ("v", (0,)), ("rope", (0,)), ("norm", (0,)), ("positions", (0,)), ("lse", (1, 2)),
+                           ("prefix", (2,))):
+        for i in callers:
+            with pytest.raises(ValueError, match="cuda:1"):
+                make(where)[i]()
+    assert library.calls == []

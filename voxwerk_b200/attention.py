@@ -47,6 +47,17 @@ def _cuda(t, dtype: str, dims: int, what: str):
     return t
 
 
+def _same_gpu(gpu: int, index: int, what: str) -> None:
+    if index != gpu:
+        raise ValueError(f"{what} is on cuda:{index}, the device handle on cuda:{gpu}")
+
+
+def _one_gpu(first, *others) -> int:
+    for t in others:
+        _need(t.get_device() == first.get_device(), "the tensors must be on one GPU")
+    return first.get_device()
+
+
 def _call(function, device: Device, stream: Optional[int], *args) -> None:
     handle = device.handle
     if stream is not None:
@@ -59,10 +70,17 @@ def _call(function, device: Device, stream: Optional[int], *args) -> None:
     check(lib.vw_synchronize(handle, stream), handle)
 
 
-def _rows(t, dtype, shape, what: str):
+def _no_gpu() -> int:
+    return -1
+
+
+def _rows(gpu: int, t, dtype, shape, what: str):
     """Pointer, row and head stride of a [rows, heads, dim] tensor; a dimension of size one has no stride of its own."""
-    if not getattr(t, "is_cuda", False):
-        raise TypeError(f"{what} must be a CUDA tensor")
+    index = getattr(t, "get_device", _no_gpu)()
+    if index != gpu:
+        if not getattr(t, "is_cuda", False):
+            raise TypeError(f"{what} must be a CUDA tensor")
+        _same_gpu(gpu, index, what)
     if t.dtype is not dtype:
         raise TypeError(f"{what} must be {str(dtype)[6:]}, got {t.dtype}")
     if t.shape != shape:
@@ -89,6 +107,7 @@ class KvCache:
         _need(k.shape == v.shape and k.stride() == v.stride(), "k and v must have the same shape and strides")
         _need(k.stride(3) == 1, "k and v: the last dimension must be contiguous")
         self.k, self.v = k, v
+        self._gpu = _one_gpu(k, v)
         pages, size, heads, dim = k.shape
         self.n_kv_heads, self.head_dim = heads, dim
         page, token, head, _ = k.stride()
@@ -117,6 +136,7 @@ class KvBatch:
             _cuda(q_offsets, "int32", 1, "q_offsets")
             _need(q_offsets.shape[0] == n + 1 and q_offsets.is_contiguous(), "q_offsets must be a contiguous [n_seqs + 1]")
         self.page_table, self.kv_lens, self.q_offsets, self.n_seqs = page_table, kv_lens, q_offsets, n
+        self._gpu = _one_gpu(page_table, kv_lens, *([] if q_offsets is None else [q_offsets]))
         self._c = (page_table.data_ptr(), page_table.stride(0) if n > 1 else page_table.shape[1], page_table.shape[1], n,
                    kv_lens.data_ptr(), None if q_offsets is None else q_offsets.data_ptr())
         self._last = None, None
@@ -143,6 +163,7 @@ class KvPrefix:
         _need(group_offsets.shape[0] == n + 1 and group_offsets.is_contiguous(),
               "group_offsets must be a contiguous [n_groups + 1]")
         self.page_table, self.lens, self.group_offsets = page_table, lens, group_offsets
+        self._gpu = _one_gpu(page_table, lens, group_offsets)
         self.c = VwKvPrefix(page_table.data_ptr(), page_table.stride(0) if n > 1 else page_table.shape[1],
                             page_table.shape[1], n, lens.data_ptr(), group_offsets.data_ptr())
         self._ref = ctypes.byref(self.c)
@@ -158,6 +179,7 @@ class RopeTable:
         _need(cos.shape == sin.shape and cos.is_contiguous() and sin.is_contiguous(),
               "cos and sin must be contiguous and of one shape")
         self.cos, self.sin, self.interleaved = cos, sin, bool(interleaved)
+        self._gpu = _one_gpu(cos, sin)
         self.rotary_dim = 2 * int(cos.shape[1])
         self._c = (int(cos.shape[0]), cos.data_ptr(), sin.data_ptr(), self.rotary_dim, int(self.interleaved))
 
@@ -194,8 +216,15 @@ class RopeTable:
 _NO_ROPE = (0, None, None, 0, 0)
 
 
-def _norm(w, dim: int, what: str) -> int:
+def _held_elsewhere(gpu: int, *held) -> None:
+    for h in held:
+        if h is not None:
+            _same_gpu(gpu, h._gpu, type(h).__name__)
+
+
+def _norm(gpu: int, w, dim: int, what: str) -> int:
     _cuda(w, "float32", 1, what)
+    _same_gpu(gpu, w.get_device(), what)
     _need(w.shape[0] == dim and w.is_contiguous(), f"{what} must be a contiguous [head_dim]")
     return w.data_ptr()
 
@@ -206,38 +235,44 @@ def rope_append(device: Device, q, k, v, cache: KvCache, batch: KvBatch, rope: O
     allowed) are normalised per head (weights q_norm / k_norm [D] float32; None: not), turned to their positions (int32
     [n], rows of the table; None: each key's index) and rounded to bfloat16; q goes to q_out, k and v into the cache.
     rope None: nothing turns."""
+    gpu = device.device
+    if cache._gpu != gpu or batch._gpu != gpu or (rope is not None and rope._gpu != gpu):
+        _held_elsewhere(gpu, cache, batch, rope)
     dtype, shape = q.dtype, q.shape
     if dtype is not _BF16 and dtype is not _F32:
         raise TypeError(f"q, k and v must be float32 or bfloat16, got {dtype}")
     n, heads, dim = shape if len(shape) == 3 else (0, 0, -1)
     _need(dim == cache.head_dim, "q must be [n, Hq, D] of the cache's D")
     kv = (n, cache.n_kv_heads, dim)
-    q_ptr, q_row, q_head = _rows(q, dtype, shape, "q")
-    k_ptr, k_row, k_head = _rows(k, dtype, kv, "k")
-    v_ptr, v_row, v_head = _rows(v, dtype, kv, "v")
-    out_ptr, out_row, out_head = _rows(q_out, _BF16, shape, "q_out")
+    q_ptr, q_row, q_head = _rows(gpu, q, dtype, shape, "q")
+    k_ptr, k_row, k_head = _rows(gpu, k, dtype, kv, "k")
+    v_ptr, v_row, v_head = _rows(gpu, v, dtype, kv, "v")
+    out_ptr, out_row, out_head = _rows(gpu, q_out, _BF16, shape, "q_out")
     at = None
     if positions is not None:
         _cuda(positions, "int32", 1, "positions")
+        _same_gpu(gpu, positions.get_device(), "positions")
         _need(positions.shape[0] == n and positions.is_contiguous(), "positions must be a contiguous [n]")
         at = positions.data_ptr()
     n_positions, cos, sin, rotary, interleaved = _NO_ROPE if rope is None else rope._c
     rows = VwRopeRows(q_ptr, k_ptr, v_ptr, q_row, q_head, k_row, k_head, v_row, v_head,
-                      VW_F32 if dtype is _F32 else VW_BF16, heads, None if q_norm is None else _norm(q_norm, dim, "q_norm"),
-                      None if k_norm is None else _norm(k_norm, dim, "k_norm"), eps, n_positions, cos, sin, at, rotary,
+                      VW_F32 if dtype is _F32 else VW_BF16, heads,
+                      None if q_norm is None else _norm(gpu, q_norm, dim, "q_norm"),
+                      None if k_norm is None else _norm(gpu, k_norm, dim, "k_norm"), eps, n_positions, cos, sin, at, rotary,
                       interleaved, out_ptr, out_row, out_head)
     _call(lib.vw_rope_append, device, stream, cache._ref, batch._rows(n), ctypes.byref(rows))
 
 
-def _attn_rows(q, out, lse, cache: KvCache, scale: Optional[float]):
+def _attn_rows(gpu: int, q, out, lse, cache: KvCache, scale: Optional[float]):
     shape = q.shape
     n, heads, dim = shape if len(shape) == 3 else (0, 0, -1)
     _need(dim == cache.head_dim, "q must be [n, Hq, D] of the cache's D")
-    q_ptr, q_row, q_head = _rows(q, _BF16, shape, "q")
-    out_ptr, out_row, out_head = _rows(out, _BF16, shape, "out")
+    q_ptr, q_row, q_head = _rows(gpu, q, _BF16, shape, "q")
+    out_ptr, out_row, out_head = _rows(gpu, out, _BF16, shape, "out")
     lse_ptr = None
     if lse is not None:
         _cuda(lse, "float32", 2, "lse")
+        _same_gpu(gpu, lse.get_device(), "lse")
         _need(lse.shape == (n, heads) and lse.is_contiguous(), "lse must be a contiguous [n, Hq]")
         lse_ptr = lse.data_ptr()
     return n, VwAttnRows(q_ptr, q_row, q_head, heads, dim ** -0.5 if scale is None else scale, out_ptr, out_row, out_head,
@@ -249,7 +284,10 @@ def prompt_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, sca
     """vw_prompt_attention: causal attention of packed sequences over their keys in the cache.  q and out
     [n, n_q_heads, D] bfloat16 (batch.q_offsets gives each sequence's rows, its last keys), scale 1/sqrt(D) unless
     given, lse optionally [n, n_q_heads] float32.  Rows that see no key get 0 and -inf."""
-    n, rows = _attn_rows(q, out, lse, cache, scale)
+    gpu = device.device
+    if cache._gpu != gpu or batch._gpu != gpu:
+        _held_elsewhere(gpu, cache, batch)
+    n, rows = _attn_rows(gpu, q, out, lse, cache, scale)
     _call(lib.vw_prompt_attention, device, stream, cache._ref, batch._rows(n), ctypes.byref(rows))
 
 
@@ -257,6 +295,9 @@ def decode_attention(device: Device, q, cache: KvCache, batch: KvBatch, out, pre
                      scale: Optional[float] = None, lse=None, stream: Optional[int] = None) -> None:
     """vw_decode_attention: one row per sequence (row s is sequence s; batch.q_offsets is ignored) over all of its keys
     and, with `prefix`, those its group shares, which are read once for the group.  Tensors as in prompt_attention."""
-    n, rows = _attn_rows(q, out, lse, cache, scale)
+    gpu = device.device
+    if cache._gpu != gpu or batch._gpu != gpu or (prefix is not None and prefix._gpu != gpu):
+        _held_elsewhere(gpu, cache, batch, prefix)
+    n, rows = _attn_rows(gpu, q, out, lse, cache, scale)
     _call(lib.vw_decode_attention, device, stream, cache._ref, batch._rows(n), None if prefix is None else prefix._ref,
           ctypes.byref(rows))
