@@ -290,3 +290,64 @@ def test_voices_that_the_current_stream_still_makes():
         b.check()
         assert torch.equal(got.view(torch.int16), want.view(torch.int16))
         del reused
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.07, -1.5, 1e-6])
+def test_scales_of_every_sign(device, scale):
+    """Also those under which every key weighs the same, or the least alike the most."""
+    from tests.test_gpu_attention import _decode, _prompt
+    lens = [1, 0, 70, 33, 129, 400]
+    _decode(device, 4, 2, 128, 16, lens, seed=28, scale=scale)
+    _decode(device, 6, 2, 64, 32, lens, [300, 17], [0, 4, 6], seed=29, scale=scale)
+    _decode(device, 34, 2, 128, 64, lens, [300], [1, 5], seed=30, scale=scale)
+    _prompt(device, 4, 2, 128, 16, [1, 70, 0, 33, 129], [0, 0, 5, 100, 3], seed=31, scale=scale)
+    _prompt(device, 8, 1, 64, 64, [5, 64], [3000, 500], seed=32, scale=scale)
+
+
+@pytest.mark.parametrize("where", ["own keys", "prefix"])
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64)])
+def test_decode_keys_that_are_not_finite(device, where, dim, page):
+    """A key of NaN makes the rows that see it NaN; one whose score is -inf has no weight, +inf leaves nothing finite.  Rows
+    that do not see it do not notice."""
+    import torch
+    from voxwerk_b200 import KvBatch, KvPrefix, decode_attention
+    lens, prefixes, groups = [200, 90, 75, 300, 0], [500, 130], [0, 3, 5]
+    for bad, place in ((float("nan"), 70), (float("inf"), 70), (float("inf"), 0), (-float("inf"), 74)):
+        pool = Pool(120, page, 2, dim, seed=33)
+        table, ptable = pool.table(lens), pool.table(prefixes)
+        row, sees = (table[2], [2]) if where == "own keys" else (ptable[0], [0, 1, 2])
+        at = row.long()[place // page], place % page
+        pool.k[at[0], at[1], :, 3] = bad       # one dim: the score is bad times the query's sign
+        q = pool.normal(5, 4, dim)
+        out, ls = torch.full_like(q, 9.0), torch.full((5, 4), 9.0, device="cuda")
+        torch.cuda.synchronize()
+        decode_attention(device, q, pool.cache, KvBatch(table, ints(lens)), out, lse=ls,
+                         prefix=KvPrefix(ptable, ints(prefixes), ints(groups)))
+        shared = [tuple(ref.keys_of(c, ptable[g], p) for c in (pool.k, pool.v)) for g, p in enumerate(prefixes)]
+        for s, n in enumerate(lens):
+            k, v = (ref.keys_of(c, table[s], n) for c in (pool.k, pool.v))
+            k, v = torch.cat([shared[s > 2][0], k]), torch.cat([shared[s > 2][1], v])
+            if s in sees:
+                keep = torch.isfinite(k).flatten(1).all(1)
+                assert int((~keep).sum()) == 1
+                k, v = k[keep], v[keep]
+            want, lse, bound, lse_bound = ref.attend(q[s:s + 1], k, v, dim ** -0.5)
+            if s not in sees:
+                ref.check(out[s:s + 1], want, bound, f"sequence {s}")
+                ref.check(ls[s:s + 1], lse, lse_bound, f"sequence {s} lse")
+                continue
+            for h in range(4):
+                if bad != bad or float(q[s, h, 3]) * bad > 0:
+                    assert bool(torch.isnan(out[s, h].float()).all()), f"sequence {s} head {h} of a key of {bad}"
+                    assert not bool(torch.isfinite(ls[s, h]))
+                else:
+                    ref.check(out[s:s + 1, h], want[:, h], bound[:, h], f"sequence {s} head {h}")
+                    ref.check(ls[s:s + 1, h], lse[:, h], lse_bound[:, h], f"sequence {s} head {h} lse")
+
+
+def test_prompts_of_many_lengths_behind_many_numbers_of_keys(device):
+    """More sequences than a warp has lanes, their blocks on many levels of key counts with gaps between."""
+    from tests.test_gpu_attention import _prompt
+    n = 90
+    _prompt(device, 8, 2, 64, 64, [1 + (29 * i) % 50 for i in range(n)], [(613 * i) % 3000 for i in range(n)], seed=34)
+    _prompt(device, 16, 1, 128, 16, [(7 * i) % 40 for i in range(200)], [(i % 3) * 800 for i in range(200)], seed=35)
