@@ -374,7 +374,8 @@ typedef struct vw_kv_cache {
 
 /* A batch of sequences: sequence s holds kv_lens[s] keys (those of the call's own rows included), key j in page
  * page_table[s * page_table_stride + j / page_size].  Its rows of the call are q_offsets[s] .. q_offsets[s + 1) and
- * are its last keys; q_offsets NULL: row s, one per sequence.  Rows past the last offset are left alone. */
+ * are its last keys; q_offsets NULL: row s, one per sequence (sequences from n_rows on have none).  Rows past the last
+ * offset are left alone. */
 typedef struct vw_kv_batch {
     const int32_t* page_table;   /* [n_seqs, page_table_stride], max_pages of them valid */
     int64_t page_table_stride;
@@ -445,7 +446,7 @@ typedef struct vw_attn_rows {
 /*
  * Causal attention of packed sequences: row i of the n rows of a sequence with m keys sees its keys j <= m - n + i.  A
  * row that sees no key gets out = 0 and lse = -inf.  Rounding: scores and sums in fp32, the probabilities rounded to
- * bf16 for their product with the values, out rounded once.  A value that is not finite reaches the rows of its own
+ * bf16 for their product with the values (which are bf16: the tensor cores take both in one type), out rounded once.  A value that is not finite reaches the rows of its own
  * sequence only, but there also rows before it.
  */
 vw_status vw_prompt_attention(vw_handle* handle, const vw_kv_cache* cache, const vw_kv_batch* batch,

@@ -261,7 +261,9 @@ __device__ __forceinline__ int own_tiles(const AttnParams& a, int lane) {
 // 23.6 us, 27.4 us with the latter); 7 us, then 64-key tiles at 6.5 TB/s or 0.45 us each on an SM, an item's end counted
 // as two, for the sequences' own keys.  Every CTA of both kernels comes to the same count.  With 0.42 and 0.5 us in place of
 // 0.45 (16 query heads on 8 of 128 dims): 256 sequences on a prefix of 16001 153 and 155 us against 142, 64 on one of 4099
-// 33.8 and 34.5 against 34.5.
+// 33.8 and 34.5 against 34.5.  The times are those of three batches (these two, and the 50 sequences of 32 heads on 4 of 64);
+// for others the count is as good as the model: a unit's cost does not follow head_dim, and groups of very different sizes
+// count as their mean.
 __device__ __forceinline__ int prefix_ctas(const AttnParams& a, int64_t units, int tiles, int sms, int lane) {
     const int group = a.rows.n_q_heads / a.cache.n_kv_heads;
     const float items = static_cast<float>(a.cache.n_kv_heads * ((group + 15) / 16));   // of a sequence

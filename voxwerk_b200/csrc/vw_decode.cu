@@ -13,10 +13,13 @@
 // by a CTA boundary leaves its pieces in the workspace, and the CTA that finishes last joins them in order; with
 // prefixes every item leaves its result there, and a join kernel weighs it with the prefix's.
 //
-// Measured (16 query heads on 8 of 128 dims, prefixes included): 256 sequences of 100-2000 keys on a prefix of 16001
-// 142 us = 5.1 TB/s; 64 of 20-600 on one of 4099 34.5 us, 50 of 60-900 on four prefixes (32 heads on 4 of 64) 23.6 us, one
-// of 700 10.5 us (of the 64's: the prefix kernel's other CTAs leave after 3 us, a schedule takes 4, the first tile is there
-// 2 us later, an item's end costs 0.9 and the join 4).
+// P is rounded to bf16 for its product with V, as in vw_prompt.cu (an mma's operands are of one 16-bit type).
+//
+// Measured (16 query heads on 8 of 128 dims, prefixes included; device time, CUDA graphs one after the other): 256
+// sequences of 100-2000 keys on a prefix of 16001 142-146 us = 5.0-5.1 TB/s; 64 of 20-600 on one of 4099 33-35 us, 50 of
+// 60-900 on four prefixes (32 heads on 4 of 64) 24-25 us, one of 700 12.3 us (of the 64's: the prefix kernel's other CTAs
+// leave after 3 us, a schedule takes 4, the first tile is there 2 us later, an item's end costs 0.9 and the join 4).
+// Without a prefix: the 256 120 us = 5.5 TB/s, the 64 20.5 us, the 50 14.4 us, 16 of 200-4000 27 us, 512 of 1-900 86 us.
 //
 // Every mbarrier wait is bounded.
 
@@ -80,7 +83,6 @@ struct DecodeItem {
     int64_t first, last;     // the units of its tiles, in all of the call's
     int64_t per;             // units of a CTA
 };
-static_assert(sizeof(DecodeItem) <= 64, "item slots");
 static_assert(sizeof(DecodeItem) <= 64, "item slots");
 
 struct DecodeParams {

@@ -23,11 +23,17 @@
 // there are too few blocks for the SMs, the (block, tile) units are dealt evenly instead, a block's pieces leave
 // partial results (O / l and log2-sum in fp32), and a join kernel, or the decode kernel, weighs them together.
 //
-// Measured (16 query heads on 8 of 128 dims): one prompt of 7937 216 us = 1.19 PFLOP/s at the clock that its power
-// allows (bound: a row tile's exponentials and its two products take turns, half of the time each); 12 prompts of 170-1300
-// tokens 43.3 us = 0.42 PFLOP/s (bound: three short blocks an SM, each with
-// 5-8 us before its first product and after its last); one of 37 9.6 us (latency of one block).  32 heads on 4 of 64:
-// pieces of 130-250 on 9001 cached keys 55 us = 0.42 PFLOP/s (bound: exponentials, twice as many a flop as with 128).
+// Rounding.  P is rounded to bf16 for its product with V (scores, sums and O stay fp32): one tcgen05.mma takes two
+// operands of one 16-bit type, and V is bf16.  Outputs are then 0.0017-0.0023 (relative) from the 64-bit values, where
+// their own rounding to bf16 makes 0.0016-0.0017.  tf32 for both would halve the rate and double V's space; P in two
+// bf16 terms would take 1.5 times the products and 128 columns of tensor memory more than there are.
+//
+// Measured (16 query heads on 8 of 128 dims; device time, CUDA graphs one after the other): one prompt of 7937 214-219 us
+// = 1.18-1.21 PFLOP/s for the first 25 ms, then the power limit takes the clock from 1965 to 1620-1710 MHz and it takes
+// 242-254 us = 1.02-1.07 PFLOP/s (bound: a row tile's exponentials and its two products take turns, half of the time
+// each); 12 prompts of 170-1300 tokens 43.4 us = 0.42 PFLOP/s (bound: three short blocks an SM, each with 5-8 us before
+// its first product and after its last); one of 37 10.3 us (latency of one block).  32 heads on 4 of 64: pieces of 130-250
+// on 9001 cached keys 56-57 us = 0.42 PFLOP/s (bound: exponentials, twice as many a flop as with 128).
 //
 // Every mbarrier wait is bounded; on expiry an error bit is set, every role stops and drains, tensor memory is freed.
 
