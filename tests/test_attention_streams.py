@@ -152,3 +152,17 @@ def test_tensors_of_another_gpu_are_refused(calls):
             with pytest.raises(ValueError, match="cuda:1"):
                 make(where)[i]()
     assert library.calls == []
+
+
+def test_synchronize_waits_for_the_stream_that_was_given(monkeypatch):
+    """0 is the default stream here as in the operators: what they enqueued there is waited for, and its errors are read."""
+    from voxwerk_b200 import sampler
+    library = Library()
+    monkeypatch.setattr(sampler, "lib", library)
+    device = sampler.Device.__new__(sampler.Device)
+    device._h, device.device = None, 0
+    monkeypatch.setattr(sampler.Device, "handle", None)
+    for stream, handle in ((None, None), (0, 1), (0x7770, 0x7770)):
+        library.calls.clear()
+        device.synchronize(stream)
+        assert library.calls == [("vw_synchronize", handle)]

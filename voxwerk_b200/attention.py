@@ -25,11 +25,10 @@ from typing import Optional
 import torch
 
 from ._lib import VW_BF16, VW_F32, VwAttnRows, VwKvBatch, VwKvCache, VwKvPrefix, VwRopeRows, check, lib
-from .sampler import Device
+from .sampler import DEFAULT_STREAM, Device
 
 
 _BF16, _F32 = torch.bfloat16, torch.float32
-_DEFAULT_STREAM = 1   # cudaStreamLegacy; its other handle, NULL, means the device handle's own stream to the library
 
 
 def _need(ok: bool, message: str) -> None:
@@ -61,11 +60,11 @@ def _one_gpu(first, *others) -> int:
 def _call(function, device: Device, stream: Optional[int], *args) -> None:
     handle = device.handle
     if stream is not None:
-        check(function(handle, *args, stream or _DEFAULT_STREAM), handle)
+        check(function(handle, *args, stream or DEFAULT_STREAM), handle)
         return
     if torch.cuda.is_current_stream_capturing():
         raise ValueError("a call that is captured takes the capturing stream")
-    stream = torch.cuda.current_stream(device.device).cuda_stream or _DEFAULT_STREAM
+    stream = torch.cuda.current_stream(device.device).cuda_stream or DEFAULT_STREAM
     check(function(handle, *args, stream), handle)
     check(lib.vw_synchronize(handle, stream), handle)
 

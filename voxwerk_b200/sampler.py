@@ -30,6 +30,9 @@ from .dotnet_random import DotNetRandom
 from .qwen3_tts import (CODEC_EOS_ID, CP_VOCAB_SIZE, MIN_NEW_TOKENS, NUM_CODE_GROUPS, SUPPRESS_SPAN,  # noqa: F401
                         VOCAB_SIZE)
 
+DEFAULT_STREAM = 1   # cudaStreamLegacy; its other handle, NULL, means a device handle's own stream to the library
+
+
 @dataclass(frozen=True)
 class SamplingOptions:
     """SamplingOptions (Sampler.cs:4-13): one stage's decoding settings."""
@@ -109,8 +112,9 @@ class Device:
         return st.as_dict()
 
     def synchronize(self, stream: Optional[int] = None) -> None:
-        """vw_synchronize: waits for `stream` and raises any device-side error latched by earlier calls."""
-        check(lib.vw_synchronize(self.handle, ctypes.c_void_p(stream) if stream else None), self.handle)
+        """vw_synchronize: waits for `stream` (0: the default stream; None: the handle's own) and raises any device-side
+        error latched by earlier calls."""
+        check(lib.vw_synchronize(self.handle, stream if stream is None else stream or DEFAULT_STREAM), self.handle)
 
 
 # ----------------------------------------------------------------------------- batched rows
